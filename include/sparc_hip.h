@@ -449,6 +449,55 @@ typedef struct {
 int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
                     double eps, double weight_decay, int64_t step, sparc_stream_t stream);
 
+/* ---- gradient norm and clipping -------------------------------------------------------
+ * The reference steps Adam on the gradients as they are (src/SpectralTrainer.py:237-238) and has no clipping; here the
+ * trainers take an optional max_grad_norm.  N = sqrt(sum over all tensors of the sum of squares), coefficient
+ * c = min(1, max_norm / (N + 1e-6)); a norm that is not finite gives what this formula gives, max_norm = infinity gives 1.
+ * tensors: a HOST array of records of device pointers, elements dense in memory, in any order, at any element alignment.
+ *   sparc_grad_norm          the sums of squares (float64) as at most 1024 partial sums: parts[0 .. *n_parts), n_parts a
+ *                            HOST word written before the call returns; parts: the query's bytes, 8-byte aligned.
+ *   sparc_grad_scale         g <- c g, rounded to nearest, in place, and *norm_out = N (one device float)
+ *   sparc_adam_step_clipped  sparc_adam_step on c g (the gradients themselves stay), any number of tensors, and *norm_out
+ * The two consumers add the partial sums up themselves, in a fixed order. */
+#define SPARC_F32 0
+#define SPARC_BF16 1
+#define SPARC_F16 2
+#define SPARC_GRAD_MAX_TENSORS 128            /* of one launch; longer lists take several */
+#define SPARC_GRAD_MAX_ELEMS (1LL << 34)      /* of one tensor */
+typedef struct {
+    void* p;
+    int64_t n;
+    int64_t dtype; /* SPARC_F32, SPARC_BF16 or SPARC_F16 */
+} sparc_grad_tensor_t;
+size_t sparc_grad_norm_workspace_bytes(int64_t n_tensors);
+int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double* parts, size_t parts_bytes,
+                    int64_t* n_parts, sparc_stream_t stream);
+int sparc_grad_scale(int64_t n_tensors, const sparc_grad_tensor_t* tensors, const double* parts, int64_t n_parts,
+                     double max_norm, float* norm_out, sparc_stream_t stream);
+int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
+                            double eps, double weight_decay, int64_t step, const double* parts, int64_t n_parts,
+                            double max_norm, float* norm_out, sparc_stream_t stream);
+
+/* ---- table lookup by token, and its gradient ----------------------------------------------
+ * For node features that are categories or node numbers: the reference's model starts at a float matrix
+ * (src/SpectralTrainer.py:28-39) and has no table.  table [rows][dim] with row stride ld (elements), out and g rows with
+ * strides ldo and ldg; dtype of table, out and g: SPARC_F32, SPARC_BF16 or SPARC_F16; ids: n tokens, int32, or int64 with
+ * ids_64 != 0; any element alignment.
+ *   sparc_embedding_fwd   out[i] = round(scale * table[ids[i]]), product in float32; a token outside [0, rows) reads
+ *                         nothing and gives a row of NaN.
+ *   sparc_embedding_grad  out[v] = round(scale * sum over ids[i] = v of g[i]) for ALL rows v (dense [rows][dim]; rows
+ *                         without a token, and row padding_idx when it is a row, are 0); tokens outside the table are left
+ *                         out.  Sums in float32, of long rows joined in float64, in an order fixed by the tokens alone.
+ * The gradient needs the query's workspace (256-byte aligned; 0 for sizes that are refused). */
+#define SPARC_EMBEDDING_MAX 2147483647LL      /* tokens, and rows */
+#define SPARC_EMBEDDING_MAX_DIM 1048576LL
+int sparc_embedding_fwd(int64_t n, int64_t rows, int64_t dim, int dtype, const void* ids, int ids_64, const void* table,
+                        int64_t ld, double scale, void* out, int64_t ldo, sparc_stream_t stream);
+size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t dim, int dtype);
+int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dtype, const void* ids, int ids_64, const void* g,
+                         int64_t ldg, double scale, int64_t padding_idx, void* out, void* ws, size_t ws_bytes,
+                         sparc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@ import torch.optim as optim
 
 from .graph import require_gpu
 from .ops import ACT_NONE, ACT_RELU, LinearAct
+from .optim import clip_grad_norm_
 
 
 def _run(seq: nn.Sequential, x: torch.Tensor) -> torch.Tensor:
@@ -66,6 +67,7 @@ class AETrainer:
         self.n_samples = self.ae_config["n_samples"]
         self.batch_size = self.ae_config["batch_size"]
         self.architecture = self.ae_config["architecture"]
+        self.max_grad_norm = self.ae_config.get("max_grad_norm")   # not a reference key: clip the global gradient norm
         self.output_dim = self.architecture["output_dim"]
         self.weights_path = f"./weights/{self.dataset}/ae_weights_{self.output_dim}.pth"
 
@@ -97,6 +99,8 @@ class AETrainer:
                 self.optimizer.zero_grad()
                 loss = self.criterion(self.ae_net(feats[pid]), feats[pid])
                 loss.backward()
+                if self.max_grad_norm is not None:
+                    clip_grad_norm_(self.ae_net.parameters(), self.max_grad_norm)
                 self.optimizer.step()
                 train_loss += loss.detach()
             train_loss = float(train_loss) / batches                  # the epoch's host sync

@@ -26,6 +26,8 @@ class SpectralNet:
         parts, features_batches, support_batches, y_train_batches, train_mask_batches = train
         idx_parts, val_features_batches, val_support_batches, y_val_batches, val_mask_batches = val
         if self.config.get("should_use_ae", False):
+            if self.config["spectral"].get("node_table") is not None:
+                raise ValueError("spectral.node_table takes tokens, the autoencoder stage features: one of the two")
             from .AETrainer import AETrainer
             ae_trainer = AETrainer(self.config, self.device)
             self.ae_net = ae_trainer.train(features_batches, val_features_batches)
@@ -62,7 +64,8 @@ class SpectralNet:
         self.spec_net.eval()
         with torch.no_grad():
             for a in range(0, n, chunk_rows):
-                x = X[a:a + chunk_rows].to(self.device, dtype=torch.float32)
+                x = X[a:a + chunk_rows]
+                x = x.to(self.device, dtype=x.dtype if self.spec_net.node_table is not None else torch.float32)
                 if self.config.get("should_use_ae", False):
                     x = self.ae_net.encode(x)
                 out[a:a + chunk_rows] = self.spec_net(x, should_update_orth_weights=False).cpu().numpy()

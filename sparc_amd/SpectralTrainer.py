@@ -21,15 +21,20 @@ import torch
 import torch.nn as nn
 import torch.optim as optim
 
+from .embedding import NodeTable
 from .graph import ClusterBatch, require_gpu
 from .ops import (ACT_RELU, ACT_TANH, ORTH_CHOLESKY, ORTH_REFERENCE, LapLoss, LinearAct, OrthApply, OrthPair, OrthWeights,
                   SpectralMLP, SpectralMLPGram, SplitRows)
 
 
 class SpectralNetModel(nn.Module):
-    """MLP + orthonormalisation layer (src/SpectralTrainer.py:16-108)."""
+    """MLP + orthonormalisation layer (src/SpectralTrainer.py:16-108).
 
-    def __init__(self, architecture: dict, input_dim: int, device: torch.device, orth_mode: str = "reference"):
+    node_table: None, or {"rows", "dim", "scale" (1.0), "padding_idx" (None)}: the inputs are then not features but int32 or
+    int64 tokens (node numbers, categories), [m] or [m, T]; a learned table in front of the MLP turns a node's T tokens into
+    T * dim = input_dim features."""
+
+    def __init__(self, architecture: dict, input_dim: int, device: torch.device, orth_mode: str = "reference", node_table=None):
         super().__init__()
         self.architecture = architecture
         self.num_of_layers = self.architecture["n_layers"]
@@ -40,6 +45,12 @@ class SpectralNetModel(nn.Module):
         self.rotation_matrix = None
         self.grad_ready_hook = None   # hook(layer, dW, db) -> (dW, db), called during the backward (ops._layer_done)
         self.orth_mode = {"reference": ORTH_REFERENCE, "cholesky": ORTH_CHOLESKY}[orth_mode]
+        self.node_table = None
+        if node_table is not None:
+            self.node_table = NodeTable(int(node_table["rows"]), int(node_table["dim"]), node_table.get("scale", 1.0),
+                                        node_table.get("padding_idx"))
+            if self.input_dim % self.node_table.weight.shape[1]:
+                raise ValueError("input_dim must be a multiple of the node table's width")
 
         current_dim = self.input_dim
         for layer, dim in self.architecture.items():
@@ -51,6 +62,10 @@ class SpectralNetModel(nn.Module):
                 self.layers.append(nn.Sequential(nn.Linear(current_dim, dim), nn.ReLU()))
                 current_dim = dim
 
+    def mlp_parameters(self):
+        """[W0, b0, W1, b1, ...]: the parameters whose gradients the backward reports layer by layer."""
+        return [p for layer in self.layers for p in layer.parameters()]
+
     def _make_orthonorm_weights(self, Y: torch.Tensor, top_idx=None) -> torch.Tensor:
         """sqrt(m) * inverse(R @ diag(sign(diag R))) of the reference (:62-68), from the Gram
         matrix.  top_idx: the rows that lead the reference's (permuted) batch; default 0..k-1."""
@@ -59,6 +74,8 @@ class SpectralNetModel(nn.Module):
     def embed_pre_orth(self, x: torch.Tensor, gram_rows: int = 0):
         """The MLP's output for the rows of x.  gram_rows > 0: (output, G) with G = output[:gram_rows]^T output[:gram_rows]
         in float64 when the output layer's kernel took the product along, None otherwise."""
+        if self.node_table is not None:
+            x = self.node_table(x).flatten(1)
         kinds = [isinstance(layer[1], nn.Tanh) for layer in self.layers]
         if kinds[-1] and not any(kinds[:-1]) and x.dtype == torch.float32:   # ReLU ... ReLU, Tanh: the fused MLP
             params = [p for layer in self.layers for p in (layer[0].weight, layer[0].bias)]
@@ -141,6 +158,8 @@ class SpectralTrainer:
         self.weights_path = f"./weights/{self.dataset}/spectralnet_weights.pth"
         self.orth_weights_path = f"./weights/{self.dataset}/spectralnet_orthonorm_weights.pth"
         self.orth_mode = self.spectral_config.get("orth_mode", "reference")
+        self.node_table = self.spectral_config.get("node_table")
+        self.max_grad_norm = self.spectral_config.get("max_grad_norm")
         self._batches = {}
 
     # -- the reference's two helpers, returning device-resident operators -------------------
@@ -183,7 +202,21 @@ class SpectralTrainer:
     def _setup_model(self, input_dim: int):
         self.criterion = SpectralNetLoss()
         self.spectral_net = SpectralNetModel(self.architecture, input_dim=input_dim, device=self.device,
-                                             orth_mode=self.orth_mode).to(self.device)
+                                             orth_mode=self.orth_mode, node_table=self.node_table).to(self.device)
+
+    def _input_dim(self, features) -> int:
+        """Columns of the MLP's input for a batch's features (or, with a node table, tokens)."""
+        if self.node_table is None:
+            return int(features.shape[1])
+        return int(self.node_table["dim"]) * (int(features.shape[1]) if features.dim() == 2 else 1)
+
+    def _to_device(self, features) -> torch.Tensor:
+        """A batch's features as the model takes them: float32, or the tokens as they are."""
+        if self.node_table is None:
+            return features.to(self.device, dtype=torch.float32)
+        if features.dtype not in (torch.int32, torch.int64) or features.dim() not in (1, 2):
+            raise ValueError("with a node table the features are int32 or int64 tokens, [m] or [m, T]")
+        return features.to(self.device)
 
     def _setup_optimizer(self, hip_graph: bool):
         self._lr_tensor = None
@@ -193,7 +226,9 @@ class SpectralTrainer:
         else:
             if torch.device(self.device).type == "cuda":   # all parameter tensors in one launch that fills the chip
                 from .optim import Adam
-                self.optimizer = Adam(self.spectral_net.parameters(), lr=self.lr)
+                self.optimizer = Adam(self.spectral_net.parameters(), lr=self.lr, max_grad_norm=self.max_grad_norm)
+            elif self.max_grad_norm is not None:
+                raise ValueError("spectral.max_grad_norm needs the model on an MI355X")
             else:
                 self.optimizer = optim.Adam(self.spectral_net.parameters(), lr=self.lr)
         self.scheduler = optim.lr_scheduler.ReduceLROnPlateau(self.optimizer, mode="min", factor=self.lr_decay,
@@ -204,10 +239,10 @@ class SpectralTrainer:
         `mine_val`, both lists of indices into the tuples train() received)."""
         measure = self.spectral_config.get("kernel_choice", "rule") == "measure"
         sizes = self._cluster_sizes()
-        feats = [self.features_batches[b].to(self.device, dtype=torch.float32) for b in mine]
+        feats = [self._to_device(self.features_batches[b]) for b in mine]
         sup = [self._get_support_matrix(self.support_batches[b], sizes[b] if sizes else None).warm(k, measure=measure)
                for b in mine]
-        vfeats = [self.val_features_batches[b].to(self.device, dtype=torch.float32) for b in mine_val]
+        vfeats = [self._to_device(self.val_features_batches[b]) for b in mine_val]
         vsup = [self._get_support_matrix(self.val_support_batches[b]).warm(k, training=False, measure=measure)
                 for b in mine_val]
         return feats, sup, vfeats, vsup
@@ -224,14 +259,16 @@ class SpectralTrainer:
         Config keys beyond the reference's, all optional: spectral.orth_mode ("reference" | "cholesky"),
         spectral.hip_graph (whole steps replayed as HIP graphs; one GPU), spectral.kernel_choice ("rule": the kernel
         of a batch follows from its structure, so runs repeat bit for bit; "measure": the candidates are timed on
-        the batch and the fastest kept)."""
+        the batch and the fastest kept), spectral.max_grad_norm (the global gradient norm is clipped there),
+        spectral.node_table ({"rows", "dim", "scale", "padding_idx"}: the feature batches hold tokens, see
+        SpectralNetModel; the table is trained with the MLP)."""
         require_gpu(self.device)
         self.parts, self.features_batches, self.support_batches, self.y_train_batches, self.train_mask_batches = train
         self.idx_parts, self.val_features_batches, self.val_support_batches, self.y_val_batches, self.val_mask_batches = val
         self.idx_parts = list(range(len(self.parts)))
         self.counter = 0
         OrthWeights.check_and_reset(self.device)   # failures of earlier, unrelated calls do not belong to this run
-        self._setup_model(self.features_batches[0].shape[1])
+        self._setup_model(self._input_dim(self.features_batches[0]))
         world, rank = self._world()
         # spectral.hip_graph (not a reference key; default off): whole steps replayed as HIP graphs, one launch per step
         hip_graph = bool(self.spectral_config.get("hip_graph", False)) and world == 1
@@ -242,7 +279,8 @@ class SpectralTrainer:
         graphed = None
         if hip_graph:
             from .stepgraph import GraphedSteps
-            graphed = GraphedSteps(self.spectral_net, self.criterion, self.optimizer, feats, sup, k, self.device)
+            graphed = GraphedSteps(self.spectral_net, self.criterion, self.optimizer, feats, sup, k, self.device,
+                                   max_grad_norm=self.max_grad_norm)
         return self._run_epochs(feats, sup, vfeats, vsup, k, graphed, n_val_total=len(self.val_features_batches))
 
     @staticmethod
@@ -265,11 +303,10 @@ class SpectralTrainer:
         world, rank = self._world()
         reducer = None
         if world > 1:
-            from .parallel import LayerwiseReducer, all_reduce_sum, broadcast
-            params = list(self.spectral_net.parameters())
-            for p in params:                      # every replica starts from rank 0's weights
+            from .parallel import LayerwiseReducer, all_reduce_sum, broadcast, reduce_gradients, reported_parameters
+            for p in self.spectral_net.parameters():   # every replica starts from rank 0's weights
                 broadcast(p.data, 0)
-            reducer = LayerwiseReducer(params)
+            reducer = LayerwiseReducer(reported_parameters(self.spectral_net))
             self.spectral_net.grad_ready_hook = reducer   # (called as hook(layer, dW, db); its destination() lets the backward write into the buckets)
         min_val_loss = 1000000000
         batches = len(feats)
@@ -301,9 +338,8 @@ class SpectralTrainer:
                 W = self._get_valid_affinity_matrix(sup[pid], feats[pid])
                 loss = self.criterion(W, Y, is_normalized=True)
                 loss.backward(gradient=LapLoss.unit_gradient(loss))
-                if reducer is not None and reducer.finish() == 0:
-                    from .parallel import all_reduce_mean_gradients
-                    all_reduce_mean_gradients(list(self.spectral_net.parameters()))
+                if reducer is not None:
+                    reduce_gradients(self.spectral_net, reducer)
                 self.optimizer.step()
                 train_loss += loss.detach()
 

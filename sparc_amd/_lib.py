@@ -91,6 +91,14 @@ _SIGS = {
     "sparc_dgrad_wide_first_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "sparc_dgrad_wide_first": (c_int, [c_int64, c_int, c_int, c_int, P, c_int64, P, P, c_int64, P, P, P, P, c_size_t, P]),
     "sparc_adam_step": (c_int, [c_int, P, c_double, c_double, c_double, c_double, c_double, c_int64, P]),
+    "sparc_grad_norm_workspace_bytes": (c_size_t, [c_int64]),
+    "sparc_grad_norm": (c_int, [c_int64, P, P, c_size_t, P, P]),
+    "sparc_grad_scale": (c_int, [c_int64, P, P, c_int64, c_double, P, P]),
+    "sparc_adam_step_clipped": (c_int, [c_int64, P, c_double, c_double, c_double, c_double, c_double, c_int64, P, c_int64, c_double,
+                                        P, P]),
+    "sparc_embedding_fwd": (c_int, [c_int64, c_int64, c_int64, c_int, P, c_int, P, c_int64, c_double, P, c_int64, P]),
+    "sparc_embedding_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "sparc_embedding_grad": (c_int, [c_int64, c_int64, c_int64, c_int, P, c_int, P, c_int64, c_double, c_int64, P, P, c_size_t, P]),
     "sparc_row_rank_values": (c_int, [c_int64, c_int64, P, c_int64, c_int, P, P, P]),
     "sparc_label_scores": (c_int, [c_int64, P, P, P, P, c_int64, P, c_int, P, P, P, P]),
     "sparc_subblock_workspace_bytes": (c_size_t, [c_int64, c_int64]),

@@ -8,7 +8,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libsparc_hip.so")
-SOURCES = ["spmm.hip", "affinity_prep.hip", "orth.hip", "mlp.hip", "csr_build.hip", "subblock.hip", "select.hip", "blocks.hip", "partition.hip", "adam.hip"]
+SOURCES = ["spmm.hip", "affinity_prep.hip", "orth.hip", "mlp.hip", "csr_build.hip", "subblock.hip", "select.hip", "blocks.hip", "partition.hip", "adam.hip",
+           "clip.hip", "embedding.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-pass-failed",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # no v_pk_{add,mul,fma}_f32: some of their forms have given wrong
 #                                     results on this part, rarely and without an error (3.724 -> 3.741 ms per bench step)

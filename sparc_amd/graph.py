@@ -164,6 +164,16 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def launch(what: str, fn, device, *args) -> None:
+    """fn(*args, stream): an entry point of the library on `device` (made current where it is not) and its current stream."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, what)
+
+
 class Workspace:
     """One growing scratch buffer per device; every kernel call on the current stream shares it."""
     _buffers = {}

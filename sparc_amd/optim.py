@@ -1,22 +1,147 @@
 """torch.optim.Adam as the reference configures it (src/SpectralTrainer.py:188: defaults apart from the learning rate)
-with the update of all parameter tensors in one launch of libsparc_hip.so (sparc_adam_step).  A torch Optimizer:
-param_groups, state_dict and learning-rate schedulers (src/SpectralTrainer.py:189-192) work as with torch's own."""
+with the update of all parameter tensors in one launch of libsparc_hip.so (sparc_adam_step), the global gradient norm
+over many tensors, and clipping by it, in place (clip_grad_norm_) or on the way into the update (max_grad_norm).  Adam is a
+torch Optimizer: param_groups, state_dict and learning-rate schedulers (src/SpectralTrainer.py:189-192) work as with
+torch's own."""
 from __future__ import annotations
 
 import ctypes
 
 import torch
 
-from ._lib import AdamTensor, check, lib
+from ._lib import AdamTensor, lib
+from .embedding import DTYPES
+from .graph import launch, require_gpu
 
 MAX_TENSORS = 32
 
 
+def _dense(t: torch.Tensor) -> bool:
+    """Every element once in numel() consecutive places, in any order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def _norm_of(grads, device):
+    """(list records for the C calls, partial sums of the squares on the device, how many)."""
+    n = len(grads)
+    flat = []
+    for g in grads:
+        if g.device != device:
+            raise ValueError("the gradients of one norm live on one device")
+        code = DTYPES.get(g.dtype)
+        if code is None or g.is_sparse or not _dense(g):
+            raise ValueError("gradients must be dense float32, bfloat16 or float16 tensors")
+        flat += (g.data_ptr(), g.numel(), code)
+    records = (ctypes.c_int64 * (3 * n))(*flat)
+    nbytes = lib.sparc_grad_norm_workspace_bytes(n)
+    parts = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
+    count = ctypes.c_int64()
+    launch("sparc_grad_norm", lib.sparc_grad_norm, device, n, records, parts.data_ptr(), nbytes, ctypes.byref(count))
+    return records, parts, count.value
+
+
+def _limit(max_norm) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm must be a number >= 0")
+    return max_norm
+
+
+def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
+    """Scales the gradients of `parameters` (one tensor or several; those without a gradient are passed over, a gradient met
+    twice counts once) in place by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them together, and
+    returns the norm before (float32, on the device; nothing synchronises).  float32, bfloat16 and float16 gradients may be
+    mixed; sums in float64.  A norm that is not finite leaves what the formula gives; an infinite max_norm never clips."""
+    max_norm = _limit(max_norm)
+    if torch.is_tensor(parameters):
+        parameters = (parameters,)
+    grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
+    if not grads:
+        return torch.zeros(())
+    device = grads[0].device
+    require_gpu(device)
+    records, parts, count = _norm_of(grads, device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    launch("sparc_grad_scale", lib.sparc_grad_scale, device, len(grads), records, parts.data_ptr(), count, max_norm, norm.data_ptr())
+    return norm
+
+
+def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
+    flat = []
+    for of_one in zip(params, grads, exp_avgs, exp_avg_sqs):
+        n = of_one[0].numel()
+        for t in of_one:
+            if t.dtype != torch.float32 or t.device != device or not t.is_contiguous() or t.numel() != n:
+                raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
+            flat.append(t.data_ptr())
+        flat.append(n)
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+@torch.no_grad()
+def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 0.0, max_grad_norm=None):
+    """Update number `step` (from 1) of torch.optim.Adam on lists of tensors, in place: params, exp_avgs and exp_avg_sqs.
+    With max_grad_norm the gradients enter as clip_grad_norm_(..., max_grad_norm) would leave them, but are only read
+    (once for the norm, once by the update); returns their norm then, None otherwise."""
+    params = list(params)
+    if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs)):
+        raise ValueError("as many gradients and moments as parameters")
+    if not params:
+        return None if max_grad_norm is None else torch.zeros(())
+    device = params[0].device
+    require_gpu(device)
+    records = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
+    rates = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
+    if max_grad_norm is None:
+        _adam_launches(records, len(params), rates, device)
+        return None
+    max_grad_norm = _limit(max_grad_norm)
+    _, parts, count = _norm_of(grads, device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, len(params), records, *rates, parts.data_ptr(), count,
+           max_grad_norm, norm.data_ptr())
+    return norm
+
+
+def _adam_launches(records, n, rates, device):
+    size = ctypes.sizeof(AdamTensor)
+    for a in range(0, n, MAX_TENSORS):
+        launch("sparc_adam_step", lib.sparc_adam_step, device, min(MAX_TENSORS, n - a), ctypes.byref(records, a * size), *rates)
+
+
 class Adam(torch.optim.Optimizer):
-    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0):
+    """max_grad_norm: clip the gradients of all groups together on their way into the update (they themselves stay as
+    they are); grad_norm is then their norm in the latest step, a float32 scalar on the device."""
+
+    grad_norm = None
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+                 max_grad_norm=None):
         if lr < 0 or eps < 0 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1 or weight_decay < 0:
             raise ValueError("invalid Adam hyper-parameter")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        if max_grad_norm is not None:
+            max_grad_norm = _limit(max_grad_norm)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:   # a state written before there was a max_grad_norm
+            group.setdefault("max_grad_norm", self.defaults.get("max_grad_norm"))
+
+    def _clip_at(self):
+        limits = {group.get("max_grad_norm") for group in self.param_groups}
+        if len(limits) > 1:
+            raise ValueError("one max_grad_norm for all parameter groups: the norm is taken over all of them")
+        limit = limits.pop()
+        return None if limit is None else _limit(limit)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -24,12 +149,14 @@ class Adam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        max_norm = self._clip_at()
+        work = []
         for group in self.param_groups:
             live = [p for p in group["params"] if p.grad is not None]
             if not live:
                 continue
             group["step"] = group.get("step", 0) + 1
-            recs = []
+            grads, ms, vs = [], [], []
             for p in live:
                 if p.dtype != torch.float32 or p.grad.dtype != torch.float32 or not p.is_cuda or p.grad.is_sparse:
                     raise RuntimeError("sparc_amd.optim.Adam updates dense float32 parameters on an MI355X")
@@ -39,16 +166,25 @@ class Adam(torch.optim.Optimizer):
                 if not st:
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
-                recs.append((p, g, st["exp_avg"], st["exp_avg_sq"]))
+                grads.append(p.grad if p.grad.is_contiguous() else p.grad.contiguous())
+                ms.append(st["exp_avg"])
+                vs.append(st["exp_avg_sq"])
+            work.append((group, live, grads, ms, vs))
+        if not work:
+            return loss
+        if max_norm is not None:
+            device = work[0][1][0].device
+            require_gpu(device)
+            _, parts, count = _norm_of([g for w in work for g in w[2]], device)
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
+        for group, live, grads, ms, vs in work:
             dev = live[0].device
-            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-            with torch.cuda.device(dev):
-                for a in range(0, len(recs), MAX_TENSORS):
-                    part = recs[a:a + MAX_TENSORS]
-                    arr = (AdamTensor * len(part))(*[AdamTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel())
-                                                     for p, g, m, v in part])
-                    check(lib.sparc_adam_step(len(part), arr, float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]),
-                                              float(group["eps"]), float(group["weight_decay"]), int(group["step"]), stream),
-                          "sparc_adam_step")
+            records = _adam_records(live, grads, ms, vs, dev)
+            rates = (float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
+                     float(group["weight_decay"]), int(group["step"]))
+            if max_norm is not None:
+                launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, dev, len(live), records, *rates, parts.data_ptr(),
+                       count, max_norm, self.grad_norm.data_ptr())
+            else:
+                _adam_launches(records, len(live), rates, dev)
         return loss

@@ -155,6 +155,22 @@ class LayerwiseReducer:
         return done
 
 
+def reported_parameters(net) -> List[torch.nn.Parameter]:
+    """The parameters a LayerwiseReducer is told of: the MLP's, without a table in front of it."""
+    own = getattr(net, "mlp_parameters", None)
+    return own() if own is not None else list(net.parameters())
+
+
+def reduce_gradients(net, reducer: LayerwiseReducer, group=None):
+    """Average the gradients of one backward: the layers the backward reported through the reducer, what it did not
+    report (a node table; everything, for a model that reports no layers) in one bucket."""
+    done = reducer.finish()
+    known = {id(p) for p in reported_parameters(net)} if done else set()
+    rest = [p for p in net.parameters() if id(p) not in known]
+    if rest:
+        all_reduce_mean_gradients(rest, group)
+
+
 class ShardedSpectralTrainer:
     """Data-parallel SpectralNet steps over this rank's shard of cluster batches.  net / criterion can be
     injected (anything with forward_pair(x2, x1, top_idx=) and __call__(batch, Y, is_normalized=)); by
@@ -162,13 +178,13 @@ class ShardedSpectralTrainer:
 
     def __init__(self, architecture: dict, input_dim: int, device, lr: float = 1e-3, orth_mode: str = "reference",
                  group=None, seed: Optional[int] = 0, net=None, criterion=None, fused_adam: bool = True,
-                 hip_graph: bool = False, reduce_in_a_world_of_one: bool = False):
+                 hip_graph: bool = False, reduce_in_a_world_of_one: bool = False, max_grad_norm=None, node_table=None):
         self.device = torch.device(device)
         if seed is not None:
             torch.manual_seed(seed)  # identical initial weights on every rank
         if net is None:
             from .SpectralTrainer import SpectralNetModel
-            net = SpectralNetModel(architecture, input_dim, self.device, orth_mode=orth_mode).to(self.device)
+            net = SpectralNetModel(architecture, input_dim, self.device, orth_mode=orth_mode, node_table=node_table).to(self.device)
         if criterion is None:
             from .SpectralTrainer import SpectralNetLoss
             criterion = SpectralNetLoss()
@@ -189,14 +205,17 @@ class ShardedSpectralTrainer:
             self.optimizer = torch.optim.Adam(self.net.parameters(), lr=self.lr, fused=True, capturable=True)
         elif fused_adam and self.device.type == "cuda":
             from .optim import Adam
-            self.optimizer = Adam(self.net.parameters(), lr=lr)
+            self.optimizer = Adam(self.net.parameters(), lr=lr, max_grad_norm=max_grad_norm)
         else:
             self.optimizer = torch.optim.Adam(self.net.parameters(), lr=lr)
+        self.max_grad_norm = max_grad_norm
+        # (the package's Adam clips on the way into its update; torch's is handed clipped gradients)
+        self.clip_first = max_grad_norm is not None and "max_grad_norm" not in self.optimizer.defaults
         self._graphed = None
         self.criterion = criterion
         self.reducer = None
         if self.distributed:
-            self.attach_reducer(LayerwiseReducer(self.params, group))
+            self.attach_reducer(LayerwiseReducer(reported_parameters(self.net), group))
         self.features = []
         self.batches = []
 
@@ -209,7 +228,8 @@ class ShardedSpectralTrainer:
             self.net.grad_ready_hook = reducer   # (called as hook(layer, dW, db); its destination() lets the backward write into the buckets)
 
     def add_batch(self, features: torch.Tensor, batch) -> int:
-        self.features.append(features.to(self.device, dtype=torch.float32).contiguous())
+        tokens = getattr(self.net, "node_table", None) is not None
+        self.features.append(features.to(self.device, dtype=features.dtype if tokens else torch.float32).contiguous())
         self.batches.append(batch)
         return len(self.batches) - 1
 
@@ -222,7 +242,7 @@ class ShardedSpectralTrainer:
             if self._graphed is None:
                 from .stepgraph import GraphedSteps
                 self._graphed = GraphedSteps(self.net, self.criterion, self.optimizer, self.features, self.batches,
-                                             self.k, self.device)
+                                             self.k, self.device, max_grad_norm=self.max_grad_norm)
             return self._graphed.step(pid, pid_2, top_idx)
         net = self.net
         net.train()
@@ -230,8 +250,11 @@ class ShardedSpectralTrainer:
         Y = net.forward_pair(self.features[pid_2], self.features[pid], top_idx=top_idx)
         loss = self.criterion(self.batches[pid], Y, is_normalized=True)
         loss.backward(gradient=LapLoss.unit_gradient(loss))
-        if self.distributed and self.reducer.finish() == 0:
-            all_reduce_mean_gradients(self.params, self.group)   # no layer reported: one bucket, one collective
+        if self.distributed:
+            reduce_gradients(net, self.reducer, self.group)
+        if self.clip_first:
+            from .optim import clip_grad_norm_
+            clip_grad_norm_(self.params, self.max_grad_norm)
         self.optimizer.step()
         return loss.detach()
 

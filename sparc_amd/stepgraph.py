@@ -21,6 +21,7 @@ import torch
 
 from .graph import Workspace
 from .ops import LapLoss
+from .optim import clip_grad_norm_
 
 
 class GraphedSteps:
@@ -30,9 +31,10 @@ class GraphedSteps:
     RING = 8   # pinned staging buffers for the permutation heads: the host may run this many steps ahead
     MAX_GRAPHS = 64   # pairs captured at most; a pair met after that runs eagerly every time
 
-    def __init__(self, net, criterion, optimizer, features, batches, k: int, device):
+    def __init__(self, net, criterion, optimizer, features, batches, k: int, device, max_grad_norm=None):
         self.net, self.criterion, self.optimizer = net, criterion, optimizer
         self.features, self.batches, self.k = features, batches, int(k)
+        self.max_grad_norm = max_grad_norm
         self.device = torch.device(device)
         self.top_idx = torch.zeros(self.k, dtype=torch.int32, device=self.device)
         # the orthonormalisation matrix of the last step outlives the step (validation and predict use it,
@@ -50,6 +52,8 @@ class GraphedSteps:
         Y = self.net.forward_pair(self.features[pid_2], self.features[pid], top_idx=self.top_idx)
         loss = self.criterion(self.batches[pid], Y, is_normalized=True)
         loss.backward(gradient=LapLoss.unit_gradient(loss))
+        if self.max_grad_norm is not None:
+            clip_grad_norm_(self.net.parameters(), self.max_grad_norm)
         self.optimizer.step()
         self.orth.copy_(self.net.orthonorm_weights.detach())
         return loss.detach()
