@@ -454,8 +454,8 @@ int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr
  * trainers take an optional max_grad_norm.  N = sqrt(sum over all tensors of the sum of squares), coefficient
  * c = min(1, max_norm / (N + 1e-6)); a norm that is not finite gives what this formula gives, max_norm = infinity gives 1.
  * tensors: a HOST array of records of device pointers, elements dense in memory, in any order, at any element alignment.
- *   sparc_grad_norm          the sums of squares (float64) as at most 1024 partial sums: parts[0 .. *n_parts), n_parts a
- *                            HOST word written before the call returns; parts: the query's bytes, 8-byte aligned.
+ *   sparc_grad_norm          the sums of squares (float64) as partial sums: parts[0 .. *n_parts), n_parts a HOST
+ *                            word written before the call returns; parts: the query's bytes, 8-byte aligned.
  *   sparc_grad_scale         g <- c g, rounded to nearest, in place, and *norm_out = N (one device float)
  *   sparc_adam_step_clipped  sparc_adam_step on c g (the gradients themselves stay), any number of tensors, and *norm_out
  * The two consumers add the partial sums up themselves, in a fixed order. */

@@ -13,7 +13,9 @@ namespace {
 
 constexpr int BLOCK = 256;
 constexpr int BLOCK_BYTES = 16384;   // of one tensor per workgroup and turn: four 16-byte loads in flight per thread
-constexpr int PARTS = 1024;          // partial sums of one launch: four workgroups per CU
+constexpr int NORM_THREADS = 1024, NORM_BYTES = 65536;   // the same of the norm's pass, which has a partial sum per workgroup
+constexpr int PARTS = 512;           // partial sums of one launch: two workgroups per CU
+constexpr int MOST_BLOCKS = 2048;    // workgroups of a launch that writes: eight per CU
 constexpr int ADAM_ELEMS = 1024;     // elements of one tensor per workgroup and turn of the Adam step
 constexpr int ADAM_MOST = 48;        // tensors per launch of the Adam step
 
@@ -47,41 +49,48 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 template <int DT>
 __device__ __forceinline__ double squares(const void* p, const int64_t n, const int64_t e0) {
     typedef typename Elem<DT>::type T;
-    constexpr int VE = 16 / sizeof(T), TURNS = BLOCK_BYTES / (BLOCK * 16);
+    constexpr int VE = 16 / sizeof(T), TURNS = NORM_BYTES / (NORM_THREADS * 16);
     const T* g = static_cast<const T*>(p);
     double s = 0.0;
-    if (e0 + BLOCK_BYTES / static_cast<int>(sizeof(T)) <= n) {
-        Vec<DT, VE> v[TURNS];
+    Vec<DT, VE> v[TURNS];
 #pragma unroll
-        for (int k = 0; k < TURNS; ++k) v[k].load(g + e0 + (k * BLOCK + threadIdx.x) * VE);
+    for (int k = 0; k < TURNS; ++k) {
+        const int64_t e = e0 + (k * NORM_THREADS + threadIdx.x) * VE;
+        if (e + VE <= n) {
+            v[k].load(g + e);
+        } else {   // the tensor's last vector, and behind it
 #pragma unroll
-        for (int k = 0; k < TURNS; ++k)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const double x = v[k].get(i);
-                s = fma(x, x, s);
-            }
-    } else {
-        for (int64_t i = e0 + threadIdx.x; i < n; i += BLOCK) {
-            const double x = Elem<DT>::up(g[i]);
-            s = fma(x, x, s);
+            for (int i = 0; i < VE; ++i) v[k].set(i, e + i < n ? Elem<DT>::up(g[e + i]) : 0.f);
         }
     }
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            const double x = v[k].get(i);
+            s = fma(x, x, s);
+        }
     return s;
 }
 
-__global__ __launch_bounds__(BLOCK) void grad_squares_kernel(const GradArgs a, const int blocks, double* parts) {
-    __shared__ double lds[BLOCK / 64];
+__global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(const GradArgs a, const int blocks, double* parts) {
+    __shared__ double lds[NORM_THREADS / 64];
     double s = 0.0;
     for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
         const int t = tensor_of(a, b);
         const int64_t k = b - a.first_block[t];
-        if (a.dtype[t] == SPARC_F32) s += squares<SPARC_F32>(a.p[t], a.n[t], k * (BLOCK_BYTES / 4));
-        else if (a.dtype[t] == SPARC_BF16) s += squares<SPARC_BF16>(a.p[t], a.n[t], k * (BLOCK_BYTES / 2));
-        else s += squares<SPARC_F16>(a.p[t], a.n[t], k * (BLOCK_BYTES / 2));
+        if (a.dtype[t] == SPARC_F32) s += squares<SPARC_F32>(a.p[t], a.n[t], k * (NORM_BYTES / 4));
+        else if (a.dtype[t] == SPARC_BF16) s += squares<SPARC_BF16>(a.p[t], a.n[t], k * (NORM_BYTES / 2));
+        else s += squares<SPARC_F16>(a.p[t], a.n[t], k * (NORM_BYTES / 2));
     }
-    s = block_sum(s, lds);
-    if (threadIdx.x == 0) parts[blockIdx.x] = s;
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = lds[0];
+        for (int w = 1; w < NORM_THREADS / 64; ++w) s += lds[w];
+        parts[blockIdx.x] = s;
+    }
 }
 
 // parts[0] = the sum of parts[0 .. n): for lists that took more than one launch.
@@ -117,18 +126,22 @@ __device__ __forceinline__ void scale_block(void* p, const int64_t n, const int6
     typedef typename Elem<DT>::type T;
     constexpr int VE = 16 / sizeof(T), TURNS = BLOCK_BYTES / (BLOCK * 16);
     T* g = static_cast<T*>(p);
-    if (e0 + BLOCK_BYTES / static_cast<int>(sizeof(T)) <= n) {
-        Vec<DT, VE> v[TURNS];
+    Vec<DT, VE> v[TURNS];
 #pragma unroll
-        for (int k = 0; k < TURNS; ++k) v[k].load(g + e0 + (k * BLOCK + threadIdx.x) * VE);
+    for (int k = 0; k < TURNS; ++k) {
+        const int64_t e = e0 + (k * BLOCK + threadIdx.x) * VE;
+        if (e + VE <= n) v[k].load(g + e);
+    }
 #pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
+    for (int k = 0; k < TURNS; ++k) {
+        const int64_t e = e0 + (k * BLOCK + threadIdx.x) * VE;
+        if (e + VE <= n) {
 #pragma unroll
             for (int i = 0; i < VE; ++i) v[k].set(i, v[k].get(i) * coef);
-            v[k].store(g + e0 + (k * BLOCK + threadIdx.x) * VE);
+            v[k].store(g + e);
+        } else {
+            for (int64_t i = e; i < n; ++i) g[i] = Elem<DT>::down(Elem<DT>::up(g[i]) * coef);
         }
-    } else {
-        for (int64_t i = e0 + threadIdx.x; i < n; i += BLOCK) g[i] = Elem<DT>::down(Elem<DT>::up(g[i]) * coef);
     }
 }
 
@@ -201,14 +214,14 @@ bool grads_ok(const int64_t n_tensors, const sparc_grad_tensor_t* t) {
 }
 
 // The first `count` tensors of t as kernel arguments; returns their number of blocks (below 2^30: SPARC_GRAD_MAX_ELEMS).
-int64_t fill(GradArgs& a, const sparc_grad_tensor_t* t, const int count) {
+int64_t fill(GradArgs& a, const sparc_grad_tensor_t* t, const int count, const int block_bytes) {
     int64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
         a.p[i] = t[i].p;
         a.n[i] = t[i].n;
         a.dtype[i] = static_cast<uint8_t>(t[i].dtype);
         a.first_block[i] = static_cast<int32_t>(blocks);
-        const int64_t per = BLOCK_BYTES / (t[i].dtype == SPARC_F32 ? 4 : 2);
+        const int64_t per = block_bytes / (t[i].dtype == SPARC_F32 ? 4 : 2);
         blocks += (t[i].n + per - 1) / per;
     }
     a.first_block[count] = static_cast<int32_t>(blocks);
@@ -233,10 +246,10 @@ extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* ten
     for (int64_t from = 0; from < n_tensors; from += SPARC_GRAD_MAX_TENSORS) {
         GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
-        const int64_t blocks = fill(a, tensors + from, count);
+        const int64_t blocks = fill(a, tensors + from, count, NORM_BYTES);
         if (blocks == 0) continue;
         const int grid = static_cast<int>(blocks < PARTS ? blocks : PARTS);
-        hipLaunchKernelGGL(grad_squares_kernel, dim3(grid), dim3(BLOCK), 0, stream, a, static_cast<int>(blocks), parts + total);
+        hipLaunchKernelGGL(grad_squares_kernel, dim3(grid), dim3(NORM_THREADS), 0, stream, a, static_cast<int>(blocks), parts + total);
         SPARC_CHECK_LAUNCH();
         total += grid;
         ++launches;
@@ -257,9 +270,9 @@ extern "C" int sparc_grad_scale(int64_t n_tensors, const sparc_grad_tensor_t* te
     for (int64_t from = 0; from < n_tensors || from == 0; from += SPARC_GRAD_MAX_TENSORS) {
         GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
-        const int64_t blocks = fill(a, tensors + from, count);
+        const int64_t blocks = fill(a, tensors + from, count, BLOCK_BYTES);
         if (blocks == 0 && !c.norm_out) continue;
-        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < 2 * PARTS ? blocks : 2 * PARTS);
+        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
         hipLaunchKernelGGL(grad_scale_kernel, dim3(grid), dim3(BLOCK), 0, stream, a, static_cast<int>(blocks), c);
         SPARC_CHECK_LAUNCH();
         c.norm_out = nullptr;
@@ -298,7 +311,7 @@ extern "C" int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tenso
         a.eps = static_cast<float>(eps);
         a.weight_decay = static_cast<float>(weight_decay);
         if (blocks == 0 && !c.norm_out) continue;
-        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < 2 * PARTS ? blocks : 2 * PARTS);
+        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
         hipLaunchKernelGGL(adam_clip_kernel, dim3(grid), dim3(BLOCK), 0, stream, a, static_cast<int>(blocks), c);
         SPARC_CHECK_LAUNCH();
         c.norm_out = nullptr;

@@ -44,14 +44,16 @@ def _padding(padding_idx, rows: int) -> int:
 
 def _lookup(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
     dev = table.device
-    require_gpu(dev)
+    if not table.is_cuda:
+        require_gpu(dev)
     ids = _tokens(ids, dev)
     ld = _rows_of(table, "table")
     rows, dim = table.shape
-    out = torch.empty(*ids.shape, dim, dtype=table.dtype, device=dev)
-    if out.numel():
-        launch("sparc_embedding_fwd", lib.sparc_embedding_fwd, dev, ids.numel(), rows, dim, DTYPES[table.dtype], ids.data_ptr(),
-               _ID_DTYPES[ids.dtype], table.data_ptr() or out.data_ptr(), ld, scale, out.data_ptr(), dim)
+    out = table.new_empty((*ids.shape, dim))
+    n = ids.numel()
+    if n and dim:
+        launch("sparc_embedding_fwd", lib.sparc_embedding_fwd, dev, n, rows, dim, DTYPES[table.dtype], ids.data_ptr(),
+               _ID_DTYPES[ids.dtype], table.data_ptr(), ld, scale, out.data_ptr(), dim)
     return out
 
 
@@ -60,7 +62,8 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
     shape of ids and one more dimension, dim).  float32 sums, rounded once.  Rows without a place, and row padding_idx,
     are zero; places whose token is no row are left out."""
     dev = grad.device
-    require_gpu(dev)
+    if not grad.is_cuda:
+        require_gpu(dev)
     ids = _tokens(ids, dev)
     rows = int(rows)
     if rows < 0 or grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
@@ -104,7 +107,8 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     or float16 with contiguous rows (any row stride).  The product is rounded once.  A token that is no row of the table
     gives a row of NaN (nothing is read, nothing synchronises) and no gradient.  padding_idx: this row is read as any
     other and gets no gradient.  Differentiable once, with respect to the table."""
-    _padding(padding_idx, table.shape[0])
+    if padding_idx is not None:
+        _padding(padding_idx, table.shape[0])
     if table.requires_grad and torch.is_grad_enabled():
         return EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
     return _lookup(ids, table, float(scale))

@@ -164,14 +164,20 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def launch(what: str, fn, device, *args) -> None:
-    """fn(*args, stream): an entry point of the library on `device` (made current where it is not) and its current stream."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    """fn(*args, stream): an entry point of the library on `device` (made current where it is not) and its current stream
+    (asked for as a number: a torch.cuda.Stream object costs 2 us, half as much as the launch)."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, what)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
 class Workspace:

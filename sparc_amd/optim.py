@@ -6,6 +6,7 @@ torch's own."""
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -18,8 +19,6 @@ MAX_TENSORS = 32
 
 def _dense(t: torch.Tensor) -> bool:
     """Every element once in numel() consecutive places, in any order of the dimensions."""
-    if t.is_contiguous():
-        return True
     at = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
         if stride != at:
@@ -29,22 +28,25 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _norm_of(grads, device):
-    """(list records for the C calls, partial sums of the squares on the device, how many)."""
-    n = len(grads)
+    """(records for the C calls: keep the array while they run, partial sums of the squares on the device, how many)."""
     flat = []
+    code_of = DTYPES.get
     for g in grads:
-        if g.device != device:
-            raise ValueError("the gradients of one norm live on one device")
-        code = DTYPES.get(g.dtype)
-        if code is None or g.is_sparse or not _dense(g):
-            raise ValueError("gradients must be dense float32, bfloat16 or float16 tensors")
+        code = code_of(g.dtype)
+        if code is None or g.device != device or g.is_sparse or not (g.is_contiguous() or _dense(g)):
+            raise ValueError("the gradients of one norm are dense float32, bfloat16 or float16 tensors on one device")
         flat += (g.data_ptr(), g.numel(), code)
-    records = (ctypes.c_int64 * (3 * n))(*flat)
+    records = array("q", flat)
+    n = len(grads)
     nbytes = lib.sparc_grad_norm_workspace_bytes(n)
-    parts = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
+    parts = torch.empty(nbytes >> 3, dtype=torch.float64, device=device)
     count = ctypes.c_int64()
-    launch("sparc_grad_norm", lib.sparc_grad_norm, device, n, records, parts.data_ptr(), nbytes, ctypes.byref(count))
+    launch("sparc_grad_norm", lib.sparc_grad_norm, device, n, _address(records), parts.data_ptr(), nbytes, ctypes.byref(count))
     return records, parts, count.value
+
+
+def _address(records) -> int:
+    return records.buffer_info()[0]
 
 
 def _limit(max_norm) -> float:
@@ -62,27 +64,32 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     max_norm = _limit(max_norm)
     if torch.is_tensor(parameters):
         parameters = (parameters,)
-    grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if len(set(map(id, grads))) < len(grads):
+        grads = list({id(g): g for g in grads}.values())
     if not grads:
         return torch.zeros(())
     device = grads[0].device
-    require_gpu(device)
+    if not grads[0].is_cuda:
+        require_gpu(device)
     records, parts, count = _norm_of(grads, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    launch("sparc_grad_scale", lib.sparc_grad_scale, device, len(grads), records, parts.data_ptr(), count, max_norm, norm.data_ptr())
+    launch("sparc_grad_scale", lib.sparc_grad_scale, device, len(grads), _address(records), parts.data_ptr(), count, max_norm,
+           norm.data_ptr())
     return norm
 
 
 def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
     flat = []
+    f32 = torch.float32
     for of_one in zip(params, grads, exp_avgs, exp_avg_sqs):
         n = of_one[0].numel()
         for t in of_one:
-            if t.dtype != torch.float32 or t.device != device or not t.is_contiguous() or t.numel() != n:
+            if t.dtype is not f32 or t.numel() != n or t.device != device or not t.is_contiguous():
                 raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
             flat.append(t.data_ptr())
         flat.append(n)
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return array("q", flat)
 
 
 @torch.no_grad()
@@ -97,7 +104,8 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     if not params:
         return None if max_grad_norm is None else torch.zeros(())
     device = params[0].device
-    require_gpu(device)
+    if not params[0].is_cuda:
+        require_gpu(device)
     records = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
     rates = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
     if max_grad_norm is None:
@@ -106,15 +114,15 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     max_grad_norm = _limit(max_grad_norm)
     _, parts, count = _norm_of(grads, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, len(params), records, *rates, parts.data_ptr(), count,
-           max_grad_norm, norm.data_ptr())
+    launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, len(params), _address(records), *rates, parts.data_ptr(),
+           count, max_grad_norm, norm.data_ptr())
     return norm
 
 
 def _adam_launches(records, n, rates, device):
     size = ctypes.sizeof(AdamTensor)
     for a in range(0, n, MAX_TENSORS):
-        launch("sparc_adam_step", lib.sparc_adam_step, device, min(MAX_TENSORS, n - a), ctypes.byref(records, a * size), *rates)
+        launch("sparc_adam_step", lib.sparc_adam_step, device, min(MAX_TENSORS, n - a), _address(records) + a * size, *rates)
 
 
 class Adam(torch.optim.Optimizer):
@@ -183,8 +191,8 @@ class Adam(torch.optim.Optimizer):
             rates = (float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                      float(group["weight_decay"]), int(group["step"]))
             if max_norm is not None:
-                launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, dev, len(live), records, *rates, parts.data_ptr(),
-                       count, max_norm, self.grad_norm.data_ptr())
+                launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, dev, len(live), _address(records), *rates,
+                       parts.data_ptr(), count, max_norm, self.grad_norm.data_ptr())
             else:
                 _adam_launches(records, len(live), rates, dev)
         return loss
