@@ -3,25 +3,29 @@
 //     out[i, :] = round(scale * table[ids[i], :])
 //     dT[v, :]  = round(scale * sum over i with ids[i] = v of g[i, :])         (rows without a token: 0)
 //
-// Gradient.  Four launches, no atomics on values, every sum in one fixed order:
-//   tile_counts    a workgroup per tile of TILE tokens sorts their places by bucket (a bucket is 2^shift consecutive
-//                  rows), stable, and writes where each bucket starts inside the tile;
-//   bucket_rows    a workgroup per bucket walks its part of every tile in order and sorts it by row, stable: the places
-//                  of every row in ascending order (`place`) and where each row's places end (`row_end`), a CSR matrix
-//                  whose product with g is the gradient;
-//   row_sums       the product.  Work is cut along the merged list of (places of row 0, row 0 done, places of row 1, ...)
-//                  so that a worker has `per` items whatever the rows hold: long rows are cut, empty rows cost the
-//                  store of their zeros and no separate fill.  A row of at most LONG_ROW places belongs to the worker
-//                  that meets its first; a longer one leaves one partial sum per worker
+// Gradient.  No atomics on values, every sum in one fixed order:
+//   digit_counts, digit_scatter   a stable radix sort of the tokens, one or more digits of the row number: a workgroup per
+//                  tile of tokens counts the tile's digits, then ranks its tokens (ballots inside a wave, counters in LDS
+//                  between waves, the other tiles' counts before it) and scatters {row, place}.  However often one
+//                  token occurs, every tile is the same work;
+//   row_sums       adds up.  Work is cut along the merged list of (places of row 0, row 0 done, places of row 1, ...) so that
+//                  a worker has `per` items whatever the rows hold: long rows are cut, empty rows cost the store of their
+//                  zeros and no separate fill.  A row of at most LONG_ROW places belongs to the worker that meets its
+//                  first; a longer one leaves one partial sum per worker,
 //   join_rows      which are added in order (float64) here.  Usually nothing to do.
+// Few tokens take one launch instead (few_tokens).
 #include <type_traits>
 
 #include "elem.h"
 
 namespace {
 
-constexpr int TILE = 2048;         // tokens per workgroup of tile_counts
-constexpr int MAX_BUCKETS = 2048;  // counters per wave of tile_counts
+constexpr int SORT_WAVES = 8;
+constexpr int SORT_BLOCK = 64 * SORT_WAVES;
+constexpr int UP_FRONT = 8;                    // tokens a lane of a sorting workgroup holds
+constexpr int CHUNK = SORT_BLOCK * UP_FRONT;   // tokens a sorting workgroup ranks at once
+constexpr int MOST_TILES = 128;                // every tile reads all tiles' counts
+constexpr int MOST_BITS = 11;                  // of a digit
 constexpr int WAVES = 4;
 constexpr int BLOCK = 64 * WAVES;
 constexpr int LONG_ROW = 64;
@@ -93,24 +97,22 @@ __global__ __launch_bounds__(BLOCK) void lookup_kernel(const LookupArgs a, const
 
 // ---- gradient ------------------------------------------------------------------------------------------------
 
-// Everything the launches share.  tiles x buckets is bounded by n / TILE x MAX_BUCKETS: as large as the tokens.
+// Everything the launches share.
 struct GradArgs {
     const void* ids;
     const void* g;
     void* out;
     int64_t n, rows, ldg, padding;
-    int64_t tiles, tile;       // number of tiles, tokens of a tile
-    int64_t workers;
-    int buckets, shift;
+    int64_t tile;              // tokens of a tile, a multiple of CHUNK
+    int tiles;
     int dim, wide_ids;
     int per;                   // items of a worker
     float scale;
-    uint32_t* tile_start;      // [tiles][buckets + 1]: where a bucket starts inside a tile
-    uint2* sorted;             // [n] {place, row inside the bucket}, by bucket inside a tile
-    uint2* flat;               // [n] the same, by bucket
-    uint32_t* place;           // [n] places, by row
-    uint32_t* row_end;         // [rows]
-    uint32_t* long_rows;       // [1 + 3 * most]: count, then {row, first worker, last worker}
+    uint32_t* counts;          // [tiles][1 << bits]: digits of a tile
+    uint2* sorted;             // [n] {row, place}; the last pass leaves the result here
+    uint2* other;              // [n] the same, between passes
+    uint32_t* kept;            // one word: tokens that are rows and not padding
+    uint32_t* long_rows;       // [1 + 2 * most]: count, then {row, last worker}
     float* part;               // [2 workers][dim]
 };
 
@@ -122,247 +124,160 @@ __device__ __forceinline__ int rank_among_equals(const uint32_t key, const int b
         same &= ((key >> b) & 1u) ? ones : ~ones;
     }
     *all = same;
-    const uint64_t below = same & ((1ull << (threadIdx.x & 63)) - 1ull);
-    return __popcll(below);
+    return __popcll(same & ((1ull << (threadIdx.x & 63)) - 1ull));
 }
 
-// Exclusive prefix sums over counters cnt[w * stride + k] in LDS, w < waves, k < stride (a multiple of 4, 16-byte
-// aligned), key by key and inside a key wave by wave; every counter becomes its start.  All threads; tot: a word per wave of
-// the workgroup.  Returns the total.
-__device__ uint32_t scan_counters(uint32_t* cnt, const int stride, const int waves, uint32_t* tot) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all_waves = blockDim.x >> 6;
-    const int quads = stride >> 2, each = (quads + blockDim.x - 1) / blockDim.x;
-    const int q0 = min(tid * each, quads), q1 = min(q0 + each, quads);
-    uint4* c4 = reinterpret_cast<uint4*>(cnt);
-    uint32_t mine = 0;
-    for (int q = q0; q < q1; ++q)
-        for (int w = 0; w < waves; ++w) {
-            const uint4 c = c4[w * quads + q];
-            mine += c.x + c.y + c.z + c.w;
-        }
-    uint32_t upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t other = __shfl_up(upto, off);
-        if (lane >= off) upto += other;
-    }
-    if (lane == 63) tot[wave] = upto;
-    __syncthreads();
-    uint32_t base = upto - mine, total = 0;
-    for (int w = 0; w < all_waves; ++w) {
-        if (w < wave) base += tot[w];
-        total += tot[w];
-    }
-    for (int q = q0; q < q1; ++q) {
-        uint4 key = make_uint4(0, 0, 0, 0);   // places of the quad's keys in all waves
-        for (int w = 0; w < waves; ++w) {
-            const uint4 c = c4[w * quads + q];
-            key.x += c.x; key.y += c.y; key.z += c.z; key.w += c.w;
-        }
-        uint4 at = make_uint4(base, base + key.x, base + key.x + key.y, base + key.x + key.y + key.z);
-        base = at.w + key.w;
-        for (int w = 0; w < waves; ++w) {
-            const uint4 c = c4[w * quads + q];
-            c4[w * quads + q] = at;
-            at.x += c.x; at.y += c.y; at.z += c.z; at.w += c.w;
-        }
-    }
-    __syncthreads();
-    return total;
-}
-
-constexpr int UP_FRONT = 8;   // tokens a lane of tile_counts loads at once: a wave's share of a tile
-
-__global__ __launch_bounds__(BLOCK) void tile_counts(const GradArgs a, const int bits, const int stride) {
-    extern __shared__ __align__(16) uint32_t cnt[];   // [WAVES][stride]
-    __shared__ uint32_t tot[WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t t = blockIdx.x, first = t * a.tile;
-    const int64_t per_wave = a.tile / WAVES;
-    const int64_t lo = min(first + wave * per_wave, a.n), hi = min(first + (wave + 1) * per_wave, a.n);
-    uint32_t* mine = cnt + wave * stride;
-    if (t == 0 && threadIdx.x == 0) a.long_rows[0] = 0;
-    int64_t id[UP_FRONT];
-    auto tokens = [&](const int64_t i0) {   // -1: none, or one without a gradient
+// The next UP_FRONT {row, place} of this lane, places i0 + 64 k + lane below hi; row = ~0: none.
+__device__ __forceinline__ void take(const GradArgs& a, const bool first, const uint2* in, const int64_t i0, const int64_t hi, uint2* e) {
+    const int lane = threadIdx.x & 63;
+    if (first) {
+        int64_t id[UP_FRONT];
 #pragma unroll
         for (int k = 0; k < UP_FRONT; ++k) {
             const int64_t i = i0 + k * 64 + lane;
             id[k] = i < hi ? token(a.ids, a.wide_ids, i) : -1;
         }
 #pragma unroll
-        for (int k = 0; k < UP_FRONT; ++k)
-            if (id[k] >= a.rows || id[k] == a.padding) id[k] = -1;
-    };
-    tokens(lo);
-    for (int i = threadIdx.x; i < WAVES * stride; i += BLOCK) cnt[i] = 0;
-    __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 64 * UP_FRONT) {
-        if (i0 > lo) tokens(i0);
-#pragma unroll
-        for (int k = 0; k < UP_FRONT; ++k)
-            if (id[k] >= 0) atomicAdd(mine + (id[k] >> a.shift), 1u);
-    }
-    __syncthreads();
-    const uint32_t total = scan_counters(cnt, stride, WAVES, tot);
-    uint32_t* starts = a.tile_start + t * (a.buckets + 1);
-    for (int b = threadIdx.x; b < a.buckets; b += BLOCK) starts[b] = cnt[b];
-    if (threadIdx.x == 0) starts[a.buckets] = total;
-    __syncthreads();   // (wave 0 moves its counters, which are the bucket starts, on)
-    for (int64_t i0 = lo; i0 < hi; i0 += 64 * UP_FRONT) {
-        if (hi - lo > 64 * UP_FRONT) tokens(i0);
+        for (int k = 0; k < UP_FRONT; ++k) {
+            const bool ok = id[k] >= 0 && id[k] < a.rows && id[k] != a.padding;
+            e[k] = make_uint2(ok ? static_cast<uint32_t>(id[k]) : ~0u, static_cast<uint32_t>(i0 + k * 64 + lane));
+        }
+    } else {
 #pragma unroll
         for (int k = 0; k < UP_FRONT; ++k) {
-            const bool ok = id[k] >= 0;
-            const uint32_t b = ok ? static_cast<uint32_t>(id[k] >> a.shift) : 0u;
+            const int64_t i = i0 + k * 64 + lane;
+            e[k] = i < hi ? in[i] : make_uint2(~0u, 0u);
+        }
+    }
+}
+
+// Digits of the tokens of a tile: digit = (row >> shift) & (1 << bits) - 1.
+__global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, const uint2* in, const int shift, const int bits) {
+    __shared__ uint32_t cnt[1 << MOST_BITS];
+    const bool first = in == nullptr;
+    const int digits = 1 << bits;
+    const int64_t n = first ? a.n : *a.kept;
+    const int64_t lo = blockIdx.x * a.tile, hi = min(lo + a.tile, n);
+    for (int i = threadIdx.x; i < digits; i += SORT_BLOCK) cnt[i] = 0;
+    __syncthreads();
+    for (int64_t c = lo; c < hi; c += CHUNK) {
+        uint2 e[UP_FRONT];
+        take(a, first, in, c + (threadIdx.x >> 6) * (64 * UP_FRONT), hi, e);
+#pragma unroll
+        for (int k = 0; k < UP_FRONT; ++k)
+            if (e[k].x != ~0u) atomicAdd(cnt + ((e[k].x >> shift) & (digits - 1)), 1u);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < digits; i += SORT_BLOCK) a.counts[static_cast<int64_t>(blockIdx.x) * digits + i] = cnt[i];
+}
+
+__global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, const uint2* in, uint2* out, const int shift, const int bits) {
+    extern __shared__ __align__(16) uint32_t lds[];   // base [digits], total [digits], cnt uint16 [SORT_WAVES][digits]
+    __shared__ uint32_t sums[SORT_WAVES];
+    const bool first = in == nullptr;
+    const int digits = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t *base = lds, *total = lds + digits;
+    uint16_t* cnt = reinterpret_cast<uint16_t*>(total + digits);
+    const int64_t n = first ? a.n : *a.kept;
+    const int64_t lo = blockIdx.x * a.tile, hi = min(lo + a.tile, n);
+    if (lo >= hi && blockIdx.x > 0) return;
+    uint2 e[UP_FRONT];
+    take(a, first, in, lo + wave * (64 * UP_FRONT), hi, e);   // (under way while the counts are added up)
+    // base[d]: tokens of smaller digits in all tiles, and of digit d in the tiles before this one
+    for (int d = tid; d < digits; d += SORT_BLOCK) base[d] = total[d] = 0;
+    __syncthreads();
+    const int each = (digits + SORT_BLOCK - 1) / SORT_BLOCK;      // digits of a thread: `each` in a row, of every `parts`-th tile
+    const int columns = digits / each, parts = SORT_BLOCK / columns;
+    const int d0 = (tid % columns) * each;
+    for (int k = 0; k < each; ++k) {
+        uint32_t before = 0, all = 0;
+#pragma unroll 8
+        for (int t = tid / columns; t < a.tiles; t += parts) {
+            const uint32_t c = a.counts[static_cast<int64_t>(t) * digits + d0 + k];
+            all += c;
+            before += t < static_cast<int>(blockIdx.x) ? c : 0u;
+        }
+        atomicAdd(base + d0 + k, before);
+        atomicAdd(total + d0 + k, all);
+    }
+    __syncthreads();
+    uint32_t mine = 0;
+    if (tid < columns)
+        for (int k = 0; k < each; ++k) mine += total[d0 + k];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t below = __shfl_up(upto, off);
+        if (lane >= off) upto += below;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    uint32_t smaller = upto - mine, kept = 0;
+    for (int w = 0; w < SORT_WAVES; ++w) {
+        if (w < wave) smaller += sums[w];
+        kept += sums[w];
+    }
+    if (tid < columns)
+        for (int k = 0; k < each; ++k) {
+            base[d0 + k] += smaller;
+            smaller += total[d0 + k];
+        }
+    if (first && blockIdx.x == 0 && tid == 0) {
+        *a.kept = kept;
+        a.long_rows[0] = 0;
+    }
+    for (int64_t c = lo; c < hi; c += CHUNK) {
+        if (c > lo) take(a, first, in, c + wave * (64 * UP_FRONT), hi, e);
+        uint32_t* words = reinterpret_cast<uint32_t*>(cnt);
+        for (int i = tid; i < SORT_WAVES * digits / 2; i += SORT_BLOCK) words[i] = 0;
+        __syncthreads();
+        uint16_t* own = cnt + wave * digits;
+        uint32_t at[UP_FRONT];   // rank among the wave's tokens of the digit
+#pragma unroll
+        for (int k = 0; k < UP_FRONT; ++k) {
+            const bool ok = e[k].x != ~0u;
+            const uint32_t d = ok ? (e[k].x >> shift) & (digits - 1) : 0u;
             uint64_t same;
-            const int r = rank_among_equals(b, bits, __ballot(ok), &same);
+            const int r = rank_among_equals(d, bits, __ballot(ok), &same);
             if (ok) {
-                const uint32_t at = mine[b];
-                a.sorted[first + at + r] = make_uint2(static_cast<uint32_t>(i0 + k * 64 + lane),
-                                                      static_cast<uint32_t>(id[k] - (static_cast<int64_t>(b) << a.shift)));
-                if (r == 0) mine[b] = at + __popcll(same);
+                const uint32_t c0 = own[d];
+                at[k] = c0 + r;
+                if (r == 0) own[d] = static_cast<uint16_t>(c0 + __popcll(same));
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the counters as the next turn's lanes find them
         }
+        __syncthreads();
+        for (int d = tid; d < digits; d += SORT_BLOCK) {             // counters become starts inside the chunk
+            uint32_t run = 0;
+#pragma unroll
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                const uint32_t c0 = cnt[w * digits + d];
+                cnt[w * digits + d] = static_cast<uint16_t>(run);
+                run += c0;
+            }
+            total[d] = run;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < UP_FRONT; ++k)
+            if (e[k].x != ~0u) {
+                const uint32_t d = (e[k].x >> shift) & (digits - 1);
+                out[base[d] + own[d] + at[k]] = e[k];
+            }
+        __syncthreads();
+        for (int d = tid; d < digits; d += SORT_BLOCK) base[d] += total[d];
     }
 }
 
-// Frequent tokens make a few buckets large, so a bucket has sixteen waves; they share COUNTERS words of LDS: all for one
-// wave's rows when the bucket is small (one wave then ranks it), a sixteenth each otherwise.  Rows that the counters do
-// not hold at once take further passes over the bucket.
-constexpr int BIG_WAVES = 16;
-constexpr int COUNTERS = 8192;
-constexpr int ONE_WAVE = 512;   // places that one wave ranks alone
-constexpr int RANK_AHEAD = 4;   // places a lane loads at once
-
-__global__ __launch_bounds__(64 * BIG_WAVES) void bucket_rows(const GradArgs a) {
-    extern __shared__ __align__(16) uint32_t lds[];   // counters [COUNTERS], run [tiles], where [tiles]
-    __shared__ uint32_t tot[BIG_WAVES];
-    __shared__ uint32_t before[BIG_WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t b = blockIdx.x;
-    const int64_t row0 = b << a.shift;
-    const int64_t in_bucket = min(static_cast<int64_t>(1) << a.shift, a.rows - row0);
-    const int tiles = static_cast<int>(a.tiles);
-    uint32_t* cnt = lds;
-    uint32_t* run = cnt + COUNTERS;
-    uint32_t* where = run + tiles;
-    // the bucket's part of every tile: running totals, and the places before the bucket (its start in `place`)
-    uint32_t start = 0, total = 0;
-    for (int t0 = 0; t0 < tiles; t0 += 64 * BIG_WAVES) {
-        const int t = t0 + tid;
-        uint32_t lo = 0, len = 0;
-        if (t < tiles) {
-            const uint32_t* starts = a.tile_start + static_cast<int64_t>(t) * (a.buckets + 1) + b;
-            lo = starts[0];
-            len = starts[1] - lo;
-            where[t] = lo;
-        }
-        uint32_t upto = len, low = lo;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t other = __shfl_up(upto, off), o2 = __shfl_xor(low, off);
-            if (lane >= off) upto += other;
-            low += o2;
-        }
-        if (lane == 63) {
-            tot[wave] = upto;
-            before[wave] = low;
-        }
-        __syncthreads();
-        uint32_t base = total;
-#pragma unroll
-        for (int w = 0; w < BIG_WAVES; ++w) {
-            if (w < wave) base += tot[w];
-            total += tot[w];
-            start += before[w];
-        }
-        if (t < tiles) run[t] = base + upto - len;
-        __syncthreads();
-    }
-    const int waves = total <= ONE_WAVE ? 1 : BIG_WAVES;
-    const int slots = static_cast<int>(min(in_bucket, static_cast<int64_t>(COUNTERS / waves)));
-    int row_bits = 0, top = 1;
-    while ((1 << row_bits) < slots) ++row_bits;
-    while (top < tiles) top <<= 1;
-    const uint32_t per_wave = waves == 1 ? total : ((total + 64 * BIG_WAVES - 1) / (64 * BIG_WAVES)) * 64;
-    const uint32_t lo = min(wave * per_wave, total), hi = wave < waves ? min(lo + per_wave, total) : lo;
-    uint2* flat = a.flat + start;   // the bucket's places in order, once they are found in the tiles
-    uint32_t done = start;          // places of the passes before this one
-    for (int64_t r0 = 0; r0 < in_bucket; r0 += slots) {
-        const int count = static_cast<int>(min(in_bucket - r0, static_cast<int64_t>(slots)));
-        const int stride = (count + 3) & ~3;
-        for (int i = tid; i < waves * stride; i += 64 * BIG_WAVES) cnt[i] = 0;
-        __syncthreads();
-        uint32_t* mine = cnt + wave * stride;
-        for (int turn = 0; turn < 2; ++turn) {   // count, then place
-            for (uint32_t j0 = lo; j0 < hi; j0 += 64 * RANK_AHEAD) {
-                uint2 e[RANK_AHEAD];
-                if (turn == 0 && r0 == 0) {
-                    // place j of the bucket lies in the last tile whose run begins at or before j
-                    int t[RANK_AHEAD] = {};
-                    for (int s = top >> 1; s > 0; s >>= 1)
-#pragma unroll
-                        for (int k = 0; k < RANK_AHEAD; ++k)
-                            if (t[k] + s < tiles && run[t[k] + s] <= j0 + k * 64 + lane) t[k] += s;
-#pragma unroll
-                    for (int k = 0; k < RANK_AHEAD; ++k) {
-                        const uint32_t j = j0 + k * 64 + lane;
-                        e[k] = make_uint2(0u, 0xffffffffu);
-                        if (j < hi) e[k] = a.sorted[t[k] * a.tile + where[t[k]] + (j - run[t[k]])];
-                    }
-#pragma unroll
-                    for (int k = 0; k < RANK_AHEAD; ++k) {
-                        const uint32_t j = j0 + k * 64 + lane;
-                        if (j < hi) flat[j] = e[k];   // (read back by this very lane)
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < RANK_AHEAD; ++k) {
-                        const uint32_t j = j0 + k * 64 + lane;
-                        e[k] = j < hi ? flat[j] : make_uint2(0u, 0xffffffffu);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < RANK_AHEAD; ++k) {
-                    const int64_t local = static_cast<int64_t>(e[k].y) - r0;
-                    const bool ok = local >= 0 && local < count;
-                    const uint32_t r = ok ? static_cast<uint32_t>(local) : 0u;
-                    uint64_t same;
-                    const int rank = rank_among_equals(r, row_bits, __ballot(ok), &same);
-                    if (ok) {
-                        const uint32_t at = mine[r];
-                        if (turn == 1) a.place[done + at + rank] = e[k].x;
-                        if (rank == 0) mine[r] = at + __popcll(same);
-                    }
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                }
-            }
-            __syncthreads();
-            if (turn == 0) {
-                const uint32_t all = scan_counters(cnt, stride, waves, tot);
-                // wave 0's counter of the next row is where this row ends
-                for (int k = tid; k < count; k += 64 * BIG_WAVES) a.row_end[row0 + r0 + k] = done + (k + 1 < count ? cnt[k + 1] : all);
-                if (tid == 0) tot[0] = all;
-                __syncthreads();
-            }
-        }
-        done += tot[0];
-        __syncthreads();
-    }
-}
-
-// The point of the merged list with `diag` items before it: the smallest row r whose end item lies at or behind diag,
-// i.e. row_end[r] + r >= diag; diag - r places lie before it.  (Items of row r: its places, then its end.)
-__device__ __forceinline__ int64_t merge_row(const uint32_t* row_end, const int64_t rows, const int64_t diag) {
-    // 64 probes at a time; the answer is in [lo, hi]
-    int64_t lo = 0, hi = min(rows, diag);
+// Places before item `diag` of the merged list: place e is its item e + row of e (the rows before that one have ended).
+__device__ __forceinline__ int64_t merge_place(const uint2* sorted, const int64_t places, const int64_t rows, const int64_t diag) {
+    int64_t lo = max(static_cast<int64_t>(0), diag - rows), hi = min(places, diag);   // the answer is in [lo, hi]
     const int lane = threadIdx.x & 63;
-    while (hi > lo) {
+    while (hi > lo) {                                                                  // 64 probes at a time
         const int64_t width = (hi - lo + 63) >> 6;
-        const int64_t r = lo + lane * width;
-        const bool below = r < hi && static_cast<int64_t>(row_end[r]) + r < diag;
-        const int k = __popcll(__ballot(below));   // probes 0 .. k - 1 are below: the answer lies behind probe k - 1
+        const int64_t e = lo + lane * width;
+        const bool before = e < hi && static_cast<int64_t>(sorted[e].x) + e < diag;
+        const int k = __popcll(__ballot(before));   // probes 0 .. k - 1 are before: the answer lies behind probe k - 1
         if (k == 0) return lo;
         const int64_t new_lo = lo + (k - 1) * width + 1;
         hi = min(hi, lo + k * width);
@@ -372,11 +287,13 @@ __device__ __forceinline__ int64_t merge_row(const uint32_t* row_end, const int6
 }
 
 // Workers are groups of `lanes` lanes (a power of two); lane u of a group owns VE columns of the slice blockIdx.y.
+constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
+
 template <int DT, int VE>
 __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
-    __shared__ uint32_t ends[STAGE + 2];                 // row_end of rows [row0 - 1, row1]
-    __shared__ uint32_t places[STAGE + LONG_ROW];
+    __shared__ uint32_t rows_of[STAGE + 2 * MARGIN];     // the workgroup's places, and their rows, from place `from` on
+    __shared__ uint32_t places[STAGE + 2 * MARGIN];
     __shared__ int64_t edge[2];
     const T* g = static_cast<const T*>(a.g);
     T* out = static_cast<T*>(a.out);
@@ -384,100 +301,118 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     const int lanes = 1 << lanes_log2, in_group = BLOCK >> lanes_log2;
     const int u = tid & (lanes - 1);
     const int64_t first_worker = static_cast<int64_t>(blockIdx.x) * in_group;
-    const int64_t all_places = a.rows > 0 ? a.row_end[a.rows - 1] : 0;
+    const int64_t all_places = *a.kept;
     const int64_t items = all_places + a.rows;
     const int64_t d0 = min(first_worker * a.per, items), d1 = min(d0 + static_cast<int64_t>(in_group) * a.per, items);
     if (d0 >= d1) return;                                // (the whole workgroup)
     if (wave < 2) {
-        const int64_t r = merge_row(a.row_end, a.rows, wave ? d1 : d0);
-        if (lane == 0) edge[wave] = r;
+        const int64_t e = merge_place(a.sorted, all_places, a.rows, wave ? d1 : d0);
+        if (lane == 0) edge[wave] = e;
     }
     __syncthreads();
-    const int64_t row0 = edge[0], row1 = edge[1];        // rows row0 .. row1 - 1 end in this workgroup's items
-    const uint32_t e0 = static_cast<uint32_t>(d0 - row0), e1 = static_cast<uint32_t>(d1 - row1);
-    const int n_ends = static_cast<int>(row1 - row0) + 2;   // ends[k] = row_end[row0 - 1 + k]
-    for (int k = tid; k < n_ends; k += BLOCK) {
-        const int64_t r = row0 - 1 + k;
-        ends[k] = r < 0 ? 0u : r < a.rows ? a.row_end[r] : static_cast<uint32_t>(all_places);
+    const int64_t e_first = edge[0], e_last = edge[1];
+    const int64_t from = max(e_first - MARGIN, static_cast<int64_t>(0)), to = min(e_last + MARGIN, all_places);
+    for (int64_t k = from + tid; k < to; k += BLOCK) {
+        const uint2 s = a.sorted[k];
+        rows_of[k - from] = s.x;
+        places[k - from] = s.y;
     }
-    const uint32_t e_last = min(e1 + LONG_ROW, static_cast<uint32_t>(all_places));
-    for (uint32_t k = e0 + tid; k < e_last; k += BLOCK) places[k - e0] = a.place[k];
     __syncthreads();
     const int64_t worker = first_worker + (tid >> lanes_log2);
     const int64_t w0 = min(worker * a.per, items), w1 = min(w0 + a.per, items);
-    const int col = min((blockIdx.y * lanes + u) * VE, a.dim - VE);
+    const int col = min((static_cast<int>(blockIdx.y) * lanes + u) * VE, a.dim - VE);
     if (w0 >= w1 || (static_cast<int>(blockIdx.y) * lanes + u) * VE >= a.dim) return;   // no barrier below
-    // this worker's two points, as rows relative to row0
-    auto split = [&](const int64_t d) {
-        int lo = 0, hi = static_cast<int>(min(row1 - row0, d - d0));
+    // from here on: places relative to `from`, rows relative to row0
+    const int64_t row0 = d0 - e_first;
+    const int n_staged = static_cast<int>(to - from), i_first = static_cast<int>(e_first - from), i_last = static_cast<int>(e_last - from);
+    auto row_at = [&](const int i) { return static_cast<int>(rows_of[i] - row0); };
+    auto split = [&](const int64_t d) {                  // the first place at or behind item d
+        int lo = i_first, hi = min(i_last, i_first + static_cast<int>(d - d0));
+        const int64_t limit = d - d0 + i_first;          // item of place i: d0 + i - i_first + row_at(i)
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (static_cast<int64_t>(ends[mid + 1]) + row0 + mid < d) lo = mid + 1;
+            if (mid + static_cast<int64_t>(row_at(mid)) < limit) lo = mid + 1;
             else hi = mid;
         }
         return lo;
     };
-    int r = split(w0), r_stop = split(w1);               // rows r .. r_stop - 1 end in [w0, w1)
-    uint32_t e = static_cast<uint32_t>(w0 - row0 - r), e_stop = static_cast<uint32_t>(w1 - row0 - r_stop);
-    bool inside = false;                                 // the first row began in an earlier worker
-    if (e > ends[r]) {                                   // (ends[r]: where row r begins)
-        if (ends[r + 1] - ends[r] <= LONG_ROW) {
-            e = ends[r + 1];                             // an earlier worker has the whole row
-            ++r;
-        } else {
-            inside = true;
+    // Is row r, met at place i, begun before i?  0: no, -1: yes, and longer than LONG_ROW, otherwise its end (> 0)
+    auto cut = [&](const int i, const int r) {
+        if (i == 0 || row_at(i - 1) != r) return 0;      // (i is only 0 where no place lies before)
+        int s_lo = max(i - MARGIN, 0), s_hi = i - 1;     // its first place, as far as MARGIN sees
+        while (s_lo < s_hi) {
+            const int mid = (s_lo + s_hi) >> 1;
+            if (row_at(mid) < r) s_lo = mid + 1;
+            else s_hi = mid;
         }
+        int f_lo = i, f_hi = min(i + MARGIN, n_staged);  // behind its last place
+        while (f_lo < f_hi) {
+            const int mid = (f_lo + f_hi) >> 1;
+            if (row_at(mid) <= r) f_lo = mid + 1;
+            else f_hi = mid;
+        }
+        return f_lo - s_lo > LONG_ROW ? -1 : f_lo;
+    };
+    int i = split(w0), i_stop = split(w1);
+    int r = static_cast<int>(w0 - d0) - (i - i_first), r_stop = static_cast<int>(w1 - d0) - (i_stop - i_first);
+    int c = cut(i, r);
+    bool inside = c < 0;                                 // the first row is a long one that began in an earlier worker
+    if (c > 0) {                                         // an earlier worker has the whole row
+        i = c;
+        ++r;
     }
-    if (row0 + r_stop < a.rows && e_stop > ends[r_stop] && ends[r_stop + 1] - ends[r_stop] <= LONG_ROW) {
-        e_stop = ends[r_stop + 1];                       // the row that is cut here is this worker's
+    c = cut(i_stop, r_stop);
+    const bool goes_on = c < 0;                          // a long row goes on in the next worker
+    if (c > 0) {                                         // the row that is cut here is this worker's
+        i_stop = c;
         ++r_stop;
     }
-    if (r > r_stop || (r == r_stop && e >= e_stop)) return;
+    if (r > r_stop || (r == r_stop && i >= i_stop)) return;
     float acc[VE];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+    for (int k = 0; k < VE; ++k) acc[k] = 0.f;
     auto finish_row = [&]() {
         if (inside) {
             float* p = a.part + (2 * worker) * a.dim + col;
 #pragma unroll
-            for (int i = 0; i < VE; ++i) p[i] = acc[i];
+            for (int k = 0; k < VE; ++k) p[k] = acc[k];
             if (u == 0 && blockIdx.y == 0) {             // the last piece of a long row: announce it
-                const uint32_t k = atomicAdd(a.long_rows, 1u);
-                a.long_rows[1 + 3 * k] = static_cast<uint32_t>(row0 + r);
-                a.long_rows[2 + 3 * k] = static_cast<uint32_t>((row0 + r + ends[r]) / a.per);
-                a.long_rows[3 + 3 * k] = static_cast<uint32_t>(worker);
+                const uint32_t at = atomicAdd(a.long_rows, 1u);
+                a.long_rows[1 + 2 * at] = static_cast<uint32_t>(row0 + r);
+                a.long_rows[2 + 2 * at] = static_cast<uint32_t>(worker);
             }
             inside = false;
         } else {
             Vec<DT, VE> v;
 #pragma unroll
-            for (int i = 0; i < VE; ++i) v.set(i, acc[i] * a.scale);
+            for (int k = 0; k < VE; ++k) v.set(k, acc[k] * a.scale);
             v.store(out + (row0 + r) * a.dim + col);
         }
 #pragma unroll
-        for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+        for (int k = 0; k < VE; ++k) acc[k] = 0.f;
         ++r;
     };
     Vec<DT, VE> ahead[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-        if (e + k < e_stop) ahead[k].load(g + static_cast<int64_t>(places[e + k - e0]) * a.ldg + col);
-    while (e < e_stop) {
+        if (i + k < i_stop) ahead[k].load(g + static_cast<int64_t>(places[i + k]) * a.ldg + col);
+    while (i < i_stop) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            if (e + k >= e_stop) break;
-            while (ends[r + 1] <= e + k) finish_row();
+            if (i + k >= i_stop) break;
+            const int row = row_at(i + k);
+            while (r < row) finish_row();
 #pragma unroll
-            for (int i = 0; i < VE; ++i) acc[i] += ahead[k].get(i);
-            if (e + k + AHEAD < e_stop) ahead[k].load(g + static_cast<int64_t>(places[e + k + AHEAD - e0]) * a.ldg + col);
+            for (int j = 0; j < VE; ++j) acc[j] += ahead[k].get(j);
+            if (i + k + AHEAD < i_stop) ahead[k].load(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
         }
-        e += AHEAD;
+        i += AHEAD;
     }
     while (r < r_stop) finish_row();
-    if (e_stop > ends[r_stop]) {                         // a long row goes on in the next worker
+    if (goes_on) {
         float* p = a.part + (2 * worker + (inside ? 0 : 1)) * a.dim + col;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) p[i] = acc[i];
+        for (int k = 0; k < VE; ++k) p[k] = acc[k];
     }
 }
 
@@ -486,11 +421,25 @@ template <int DT>
 __global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a) {
     typedef typename Elem<DT>::type T;
     __shared__ double sum[WAVES][64];
+    __shared__ int64_t start;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = blockIdx.y * 64 + lane;
     const uint32_t count = a.long_rows[0];
     for (uint32_t k = blockIdx.x; k < count; k += gridDim.x) {
-        const int64_t row = a.long_rows[1 + 3 * k], first = a.long_rows[2 + 3 * k], last = a.long_rows[3 + 3 * k];
+        const int64_t row = a.long_rows[1 + 2 * k], last = a.long_rows[2 + 2 * k];
+        if (wave == 0) {                                 // the row's first place, and with it the worker that began the row
+            int64_t lo = 0, hi = *a.kept;
+            while (hi > lo) {
+                const int64_t width = (hi - lo + 63) >> 6, e = lo + lane * width;
+                const int before = __popcll(__ballot(e < hi && a.sorted[e].x < row));
+                if (before == 0) break;
+                hi = min(hi, lo + before * width);
+                lo += (before - 1) * width + 1;
+            }
+            if (lane == 0) start = lo;
+        }
+        __syncthreads();
+        const int64_t first = (row + start) / a.per;
         const int64_t pieces = last - first + 1, each = (pieces + WAVES - 1) / WAVES;
         const int64_t lo = min(wave * each, pieces), hi = min(lo + each, pieces);
         double s = 0.0;
@@ -671,11 +620,10 @@ __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int 
     }
 }
 
-// Sizes of the workspace's parts, from n, rows and dim alone.
+// Sizes of the launches and of the workspace's parts, from n, rows and dim alone.
 struct Plan {
-    int64_t tile, tiles, workers;
-    int shift, buckets, per, lanes_log2, slices, in_group;
-    size_t bytes;
+    int64_t tile, workers;
+    int tiles, passes, bits, per, lanes_log2, slices, in_group;
 };
 
 int64_t ceil_div(const int64_t a, const int64_t b) { return (a + b - 1) / b; }
@@ -690,15 +638,14 @@ int lanes_for(const int64_t units, int* slices) {
 
 Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     Plan p;
-    p.tile = TILE * ceil_div(n > 0 ? n : 1, static_cast<int64_t>(TILE) * MAX_BUCKETS);   // at most MAX_BUCKETS tiles
-    p.tiles = ceil_div(n, p.tile);
-    // about 256 places in a bucket, no more rows than one wave's counters hold, no more buckets than tile_counts takes
-    int64_t most = ceil_div(n, 256);
-    if (most < ceil_div(rows, COUNTERS)) most = ceil_div(rows, COUNTERS);
-    if (most > MAX_BUCKETS) most = MAX_BUCKETS;
-    p.shift = 0;
-    while (ceil_div(rows, static_cast<int64_t>(1) << p.shift) > most) ++p.shift;
-    p.buckets = static_cast<int>(ceil_div(rows, static_cast<int64_t>(1) << p.shift));
+    p.tile = CHUNK * ceil_div(n > 0 ? n : 1, static_cast<int64_t>(CHUNK) * MOST_TILES);
+    p.tiles = static_cast<int>(ceil_div(n > 0 ? n : 1, p.tile));
+    int bits = 1;
+    while ((static_cast<int64_t>(1) << bits) < rows) ++bits;
+    // wide digits save passes, but every tile reads the counts of all digits of all tiles
+    const int most = p.tiles <= 32 ? MOST_BITS : 8;
+    p.passes = (bits + most - 1) / most;
+    p.bits = (bits + p.passes - 1) / p.passes;
     p.lanes_log2 = lanes_for((dim + ve - 1) / ve, &p.slices);
     p.in_group = BLOCK >> p.lanes_log2;
     // items of a worker: enough workers for every SIMD's wave slots first, up to 64 items then
@@ -716,15 +663,14 @@ int launch_lookup(F&& f, const int dtype, const bool vectors) {
     return vectors ? f(lookup_kernel<SPARC_F16, 8>) : f(lookup_kernel<SPARC_F16, 1>);
 }
 
-GradArgs carve(const Plan& p, const int64_t n, const int64_t rows, const int dim, void* ws, const size_t ws_bytes, bool* ok, size_t* used) {
+GradArgs carve(const Plan& p, const int64_t n, const int dim, void* ws, const size_t ws_bytes, bool* ok, size_t* used) {
     GradArgs a = {};
     WsCarver c(ws, ws_bytes);
-    a.tile_start = c.take<uint32_t>(static_cast<size_t>(p.buckets + 1) * p.tiles);
+    a.counts = c.take<uint32_t>(static_cast<size_t>(p.tiles) << p.bits);
     a.sorted = c.take<uint2>(n);
-    a.flat = c.take<uint2>(n);
-    a.place = c.take<uint32_t>(n);
-    a.row_end = c.take<uint32_t>(rows);
-    a.long_rows = c.take<uint32_t>(1 + 3 * (n / LONG_ROW + 1));
+    a.other = c.take<uint2>(p.passes > 1 ? n : 0);
+    a.kept = c.take<uint32_t>(1);
+    a.long_rows = c.take<uint32_t>(1 + 2 * (n / LONG_ROW + 1));
     a.part = c.take<float>(static_cast<size_t>(2) * p.workers * dim);
     *ok = c.ok();
     *used = c.off;
@@ -773,7 +719,7 @@ extern "C" size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, 
     const Plan p = plan_of(n, rows, static_cast<int>(dim), dim >= ve ? ve : 1);
     bool ok;
     size_t used;
-    carve(p, n, rows, static_cast<int>(dim), nullptr, 0, &ok, &used);
+    carve(p, n, static_cast<int>(dim), nullptr, 0, &ok, &used);
     return used;
 }
 
@@ -791,24 +737,21 @@ int launch_few(const GradArgs& a, const int lanes_log2, const int slices, sparc_
 
 template <int DT, int VE>
 int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
-    int bits = 0;
-    while ((1 << bits) < p.buckets) ++bits;
-    const int stride = (p.buckets + 3) & ~3;
-    if (p.tiles > 0) {
-        hipLaunchKernelGGL(tile_counts, dim3(static_cast<unsigned>(p.tiles)), dim3(BLOCK),
-                           static_cast<size_t>(WAVES) * stride * sizeof(uint32_t), stream, a, bits, stride);
+    const size_t lds = (static_cast<size_t>(1) << p.bits) * (2 * sizeof(uint32_t) + SORT_WAVES * sizeof(uint16_t));
+    const uint2* in = nullptr;   // the ids themselves
+    for (int pass = 0; pass < p.passes; ++pass) {
+        uint2* out = (p.passes - pass) & 1 ? a.sorted : a.other;
+        hipLaunchKernelGGL(digit_counts, dim3(p.tiles), dim3(SORT_BLOCK), 0, stream, a, in, pass * p.bits, p.bits);
         SPARC_CHECK_LAUNCH();
+        hipLaunchKernelGGL(digit_scatter, dim3(p.tiles), dim3(SORT_BLOCK), lds, stream, a, in, out, pass * p.bits, p.bits);
+        SPARC_CHECK_LAUNCH();
+        in = out;
     }
-    hipLaunchKernelGGL(bucket_rows, dim3(static_cast<unsigned>(p.buckets)), dim3(64 * BIG_WAVES),
-                       static_cast<size_t>(COUNTERS + 2 * p.tiles) * sizeof(uint32_t), stream, a);
-    SPARC_CHECK_LAUNCH();
     hipLaunchKernelGGL((row_sums<DT, VE>), dim3(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), p.slices), dim3(BLOCK), 0, stream, a,
                        p.lanes_log2);
     SPARC_CHECK_LAUNCH();
-    if (a.n > LONG_ROW) {
-        hipLaunchKernelGGL((join_rows<DT>), dim3(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64)), dim3(BLOCK), 0, stream, a);
-        SPARC_CHECK_LAUNCH();
-    }
+    hipLaunchKernelGGL((join_rows<DT>), dim3(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64)), dim3(BLOCK), 0, stream, a);
+    SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
 
@@ -836,7 +779,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         p = plan_of(n, rows, static_cast<int>(dim), used_ve);
         bool ok;
         size_t used;
-        a = carve(p, n, rows, static_cast<int>(dim), ws, ws_bytes, &ok, &used);
+        a = carve(p, n, static_cast<int>(dim), ws, ws_bytes, &ok, &used);
         if (!ok) return SPARC_ERR_WS;
         a.per = p.per;
     }
@@ -849,9 +792,6 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
     a.padding = padding_idx;
     a.tiles = p.tiles;
     a.tile = p.tile;
-    a.workers = p.workers;
-    a.buckets = p.buckets;
-    a.shift = p.shift;
     a.dim = static_cast<int>(dim);
     a.wide_ids = ids_64 ? 1 : 0;
     a.scale = static_cast<float>(scale);
