@@ -118,13 +118,17 @@ struct GradArgs {
 
 // Lanes below this one whose key equals mine, among the lanes of `live`; *all: every such lane.
 __device__ __forceinline__ int rank_among_equals(const uint32_t key, const int bits, const uint64_t live, uint64_t* all) {
-    uint64_t same = live;
-    for (int b = 0; b < bits; ++b) {
-        const uint64_t ones = __ballot((key >> b) & 1u);
-        same &= ((key >> b) & 1u) ? ones : ~ones;
+    uint32_t lo = static_cast<uint32_t>(live), hi = static_cast<uint32_t>(live >> 32);
+#pragma unroll
+    for (int b = 0; b < MOST_BITS; ++b) {
+        if (b >= bits) break;
+        const uint32_t mine = 0u - ((key >> b) & 1u);            // all ones where my bit is set
+        const uint64_t ones = __ballot(mine != 0u);
+        lo &= ~(static_cast<uint32_t>(ones) ^ mine);             // the lanes whose bit is mine
+        hi &= ~(static_cast<uint32_t>(ones >> 32) ^ mine);
     }
-    *all = same;
-    return __popcll(same & ((1ull << (threadIdx.x & 63)) - 1ull));
+    *all = static_cast<uint64_t>(hi) << 32 | lo;
+    return __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
 }
 
 // The next UP_FRONT {row, place} of this lane, places i0 + 64 k + lane below hi; row = ~0: none.
@@ -464,38 +468,64 @@ __global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a) {
 // ---- gradient of few tokens: one launch ------------------------------------------------------------------
 
 // Up to FEW tokens a workgroup can look through all of them itself: it owns `per` consecutive rows, writes their zeros,
-// collects the places of its rows in order as keys {row, place}, sorts the keys and adds up the runs.  No workspace, one
-// launch instead of four dependent ones.
-constexpr int FEW = 4096, PLACE_BITS = 12;
-constexpr int FEW_TURNS = FEW / BLOCK;
+// collects the places of its rows as keys {row, place} (in any order), sorts the keys and adds up the runs.  No workspace,
+// one launch instead of six dependent ones.
+constexpr int FEW = 16384, PLACE_BITS = 14;
 constexpr int FEW_BLOCKS = 1024;   // rows are dealt to at most about that many workgroups
 constexpr int FEW_AHEAD = 8;       // gradient rows in flight per worker
+constexpr int FEW_TURNS = 4;       // 16-byte vectors of tokens in flight per thread
+
+template <typename ID>
+__device__ __forceinline__ void collect_rows(const ID* ids, const int n, const int64_t row0, const int in_block, const int64_t padding,
+                                             uint32_t* keys, uint32_t* count) {
+    constexpr int VE = 16 / sizeof(ID);
+    typedef ID mem __attribute__((ext_vector_type(VE), aligned(sizeof(ID))));
+    const int lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 < n; i0 += BLOCK * VE * FEW_TURNS) {
+        mem v[FEW_TURNS];
+#pragma unroll
+        for (int k = 0; k < FEW_TURNS; ++k) {
+            const int i = i0 + (k * BLOCK + static_cast<int>(threadIdx.x)) * VE;
+            if (i + VE <= n) {
+                v[k] = *reinterpret_cast<const mem*>(ids + i);
+            } else {
+#pragma unroll
+                for (int c = 0; c < VE; ++c) v[k][c] = i + c < n ? ids[i + c] : static_cast<ID>(-1);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < FEW_TURNS; ++k)
+#pragma unroll
+            for (int c = 0; c < VE; ++c) {
+                const int64_t id = v[k][c];
+                const bool hit = id >= row0 && id < row0 + in_block && id != padding;
+                const uint64_t hits = __ballot(hit);
+                if (hits == 0) continue;                 // (the whole wave, nearly always)
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(count, static_cast<uint32_t>(__popcll(hits)));
+                at = __builtin_amdgcn_readfirstlane(at);
+                if (hit) {
+                    const int i = i0 + (k * BLOCK + static_cast<int>(threadIdx.x)) * VE + c;
+                    keys[at + __popcll(hits & ((1ull << lane) - 1ull))] = static_cast<uint32_t>(id - row0) << PLACE_BITS | static_cast<uint32_t>(i);
+                }
+            }
+    }
+}
 
 template <int DT, int VE>
 __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t keys[];     // a power of two of them, at least n
-    __shared__ uint32_t found[FEW_TURNS * WAVES];
     __shared__ uint32_t total_found;
     __shared__ float piece[BLOCK * VE];
     __shared__ uint32_t long_runs[FEW / LONG_ROW], n_long;
     const T* g = static_cast<const T*>(a.g);
     T* out = static_cast<T*>(a.out);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x;
     const int n = static_cast<int>(a.n);
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.per;
     const int in_block = static_cast<int>(min(static_cast<int64_t>(a.per), a.rows - row0));
-    uint32_t local[FEW_TURNS];
-#pragma unroll
-    for (int k = 0; k < FEW_TURNS; ++k) {
-        const int i = k * BLOCK + tid;
-        local[k] = 0xffffffffu;
-        if (k * BLOCK < n && i < n) {
-            const int64_t id = token(a.ids, a.wide_ids, i);
-            if (id >= row0 && id < row0 + in_block && id != a.padding) local[k] = static_cast<uint32_t>(id - row0);
-        }
-    }
-    // zeros behind the loads
+    if (tid == 0) n_long = total_found = 0;
     const int lanes = 1 << lanes_log2, workers = BLOCK >> lanes_log2, worker = tid >> lanes_log2;
     const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + (tid & (lanes - 1));
     const bool mine = unit * VE < a.dim;
@@ -510,53 +540,28 @@ __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int 
     } else if (mine) {
         for (int r = worker; r < in_block; r += workers) zero.store(out + (row0 + r) * a.dim + col);
     }
-    // places in order: turn by turn, wave by wave, lane by lane
-#pragma unroll
-    for (int k = 0; k < FEW_TURNS; ++k) {
-        const uint64_t hits = __ballot(local[k] != 0xffffffffu);
-        if (lane == 0) found[k * WAVES + wave] = __popcll(hits);
-    }
-    if (tid == 0) n_long = 0;
     __syncthreads();
-    static_assert(FEW_TURNS * WAVES == 64, "one wave scans the counts");
-    if (wave == 0) {
-        const uint32_t c = found[lane];
-        uint32_t upto = c;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t other = __shfl_up(upto, off);
-            if (lane >= off) upto += other;
-        }
-        found[lane] = upto - c;
-        if (lane == 63) total_found = upto;
-    }
+    if (a.wide_ids) collect_rows(static_cast<const int64_t*>(a.ids), n, row0, in_block, a.padding, keys, &total_found);
+    else collect_rows(static_cast<const int32_t*>(a.ids), n, row0, in_block, a.padding, keys, &total_found);
     __syncthreads();
     const int count = static_cast<int>(total_found);
     if (count == 0) return;                              // (the whole workgroup)
-#pragma unroll
-    for (int k = 0; k < FEW_TURNS; ++k) {
-        const bool hit = local[k] != 0xffffffffu;
-        const uint64_t hits = __ballot(hit);
-        if (hit) keys[found[k * WAVES + wave] + __popcll(hits & ((1ull << lane) - 1ull))] = local[k] << PLACE_BITS | (k * BLOCK + tid);
-    }
     int size = 1;
     while (size < count) size <<= 1;
     for (int i = count + tid; i < size; i += BLOCK) keys[i] = 0xffffffffu;
     __syncthreads();
-    if (in_block > 1) {                                  // (one row: the places are in order)
-        for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                for (int i = tid; i < size / 2; i += BLOCK) {
-                    const int x = ((i & ~(j - 1)) << 1) | (i & (j - 1)), y = x | j;
-                    const uint32_t p = keys[x], q = keys[y];
-                    if ((p > q) == ((x & k) == 0)) {
-                        keys[x] = q;
-                        keys[y] = p;
-                    }
+    for (int k = 2; k <= size; k <<= 1)                  // bitonic: the keys are distinct, so this is the order of the places
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int i = tid; i < size / 2; i += BLOCK) {
+                const int x = ((i & ~(j - 1)) << 1) | (i & (j - 1)), y = x | j;
+                const uint32_t p = keys[x], q = keys[y];
+                if ((p > q) == ((x & k) == 0)) {
+                    keys[x] = q;
+                    keys[y] = p;
                 }
-                __syncthreads();
             }
-    }
+            __syncthreads();
+        }
     __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0): the zeros have left before any wave writes sums over them
     __syncthreads();
     auto same_row = [&](const int i, const uint32_t row) { return i < count && keys[i] >> PLACE_BITS == row; };
@@ -772,7 +777,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         if (ws_bytes < 256 || (reinterpret_cast<uintptr_t>(ws) & 255)) return SPARC_ERR_WS;   // (as for more tokens)
         p.lanes_log2 = lanes_for(ceil_div(dim, used_ve), &p.slices);
         int64_t per = ceil_div(rows, FEW_BLOCKS);
-        const int64_t most = static_cast<int64_t>(1) << (32 - PLACE_BITS - 1);   // keys below the padding's
+        const int64_t most = static_cast<int64_t>(1) << (32 - PLACE_BITS - 1);   // (keys stay below the one that pads the sort)
         if (per > most) per = most;
         a.per = static_cast<int>(per);
     } else {
