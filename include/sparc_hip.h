@@ -488,7 +488,8 @@ int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tensor_t* tensor
  *   sparc_embedding_grad  out[v] = round(scale * sum over ids[i] = v of g[i]) for ALL rows v (dense [rows][dim]; rows
  *                         without a token, and row padding_idx when it is a row, are 0); tokens outside the table are left
  *                         out.  Sums in float32, of long rows joined in float64, in an order fixed by the tokens alone.
- * The gradient needs the query's workspace (256-byte aligned; 0 for sizes that are refused). */
+ * The gradient needs the query's workspace, 256-byte aligned; where the query gives 0 (few tokens; sizes that the call
+ * refuses) none, and ws may be NULL. */
 #define SPARC_EMBEDDING_MAX 2147483647LL      /* tokens, and rows */
 #define SPARC_EMBEDDING_MAX_DIM 1048576LL
 int sparc_embedding_fwd(int64_t n, int64_t rows, int64_t dim, int dtype, const void* ids, int ids_64, const void* table,

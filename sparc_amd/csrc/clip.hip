@@ -15,29 +15,49 @@ constexpr int BLOCK = 256;
 constexpr int BLOCK_BYTES = 16384;   // of one tensor per workgroup and turn: four 16-byte loads in flight per thread
 constexpr int NORM_THREADS = 1024, NORM_BYTES = 65536;   // the same of the norm's pass, which has a partial sum per workgroup
 constexpr int PARTS = 512;           // partial sums of one launch: two workgroups per CU
-constexpr int MOST_BLOCKS = 2048;    // workgroups of a launch that writes: eight per CU
+constexpr int MOST_BLOCKS = 65536;   // workgroups of a launch that writes
 constexpr int ADAM_ELEMS = 1024;     // elements of one tensor per workgroup and turn of the Adam step
-constexpr int ADAM_MOST = 48;        // tensors per launch of the Adam step
+constexpr int ADAM_MOST = 64;        // tensors per launch of the Adam step
+// What the 256 MB Infinity Cache is left to keep from one pass to the next.  Longer lists go by with streaming (nontemporal)
+// accesses, but for their last KEEP_BYTES in the norm's pass, which the scaling, going backwards, finds there.
+constexpr int64_t KEEP_BYTES = SPARC_KEEP_BYTES;
 
 struct GradArgs {
     void* p[SPARC_GRAD_MAX_TENSORS];
-    int64_t n[SPARC_GRAD_MAX_TENSORS];
-    int32_t first_block[SPARC_GRAD_MAX_TENSORS + 1];   // blocks [first_block[i], first_block[i + 1]) belong to tensor i
-    uint8_t dtype[SPARC_GRAD_MAX_TENSORS];
-    int n_tensors;
+    int64_t n_dtype[SPARC_GRAD_MAX_TENSORS];           // elements << 2 | type
+    int32_t first_block[SPARC_GRAD_MAX_TENSORS];       // where tensor i's blocks begin; behind the last tensor: INT32_MAX
+    int blocks, plain_from;                            // blocks from plain_from on are read without streaming
 };
 
-// Index of the tensor that block b belongs to (wave-uniform; tensors without elements own no block).
-template <class A>
-__device__ __forceinline__ int tensor_of(const A& a, const int b) {
-    int lo = 0, hi = a.n_tensors;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.first_block[mid] <= b) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+__device__ __forceinline__ int64_t lane_value(const int64_t v, const int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
+
+// The records of a launch, one or two per lane: a search for a block's tensor is two ballots and no load.
+struct Records {
+    int64_t p[2], n_dtype[2];
+    int32_t first[2];
+    __device__ __forceinline__ Records(const GradArgs& a) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            p[h] = reinterpret_cast<int64_t>(a.p[lane + 64 * h]);
+            n_dtype[h] = a.n_dtype[lane + 64 * h];
+            first[h] = a.first_block[lane + 64 * h];
+        }
+    }
+    // Block b: its tensor, elements and type, and which of the tensor's blocks it is (all uniform).
+    __device__ __forceinline__ void find(const int b, void** base, int64_t* n, int* dtype, int64_t* k) const {
+        const int t = __popcll(__ballot(first[0] <= b)) + __popcll(__ballot(first[1] <= b)) - 1;
+        const int h = t >> 6, lane = t & 63;
+        *base = reinterpret_cast<void*>(lane_value(h ? p[1] : p[0], lane));
+        const int64_t nd = lane_value(h ? n_dtype[1] : n_dtype[0], lane);
+        *n = nd >> 2;
+        *dtype = static_cast<int>(nd) & 3;
+        *k = b - __builtin_amdgcn_readlane(h ? first[1] : first[0], lane);
+    }
+};
 
 __device__ __forceinline__ double block_sum(double v, double* lds) {
     v = wave_sum(v);
@@ -46,43 +66,60 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
     return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-template <int DT>
-__device__ __forceinline__ double squares(const void* p, const int64_t n, const int64_t e0) {
+template <int DT, bool STREAM>
+__device__ __forceinline__ double squares(const void* p, const int64_t n, const int64_t k) {
     typedef typename Elem<DT>::type T;
     constexpr int VE = 16 / sizeof(T), TURNS = NORM_BYTES / (NORM_THREADS * 16);
-    const T* g = static_cast<const T*>(p);
+    const int64_t e0 = k * (NORM_BYTES / static_cast<int>(sizeof(T)));
+    const T* g = static_cast<const T*>(p) + e0 + threadIdx.x * VE;
     double s = 0.0;
-    Vec<DT, VE> v[TURNS];
-#pragma unroll
-    for (int k = 0; k < TURNS; ++k) {
-        const int64_t e = e0 + (k * NORM_THREADS + threadIdx.x) * VE;
-        if (e + VE <= n) {
-            v[k].load(g + e);
-        } else {   // the tensor's last vector, and behind it
-#pragma unroll
-            for (int i = 0; i < VE; ++i) v[k].set(i, e + i < n ? Elem<DT>::up(g[e + i]) : 0.f);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < TURNS; ++k)
+    auto add = [&s](const Vec<DT, VE>& v) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-            const double x = v[k].get(i);
+            const double x = v.get(i);
             s = fma(x, x, s);
         }
+    };
+    if (e0 + NORM_BYTES / static_cast<int>(sizeof(T)) <= n) {
+        Vec<DT, VE> v[TURNS];
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j) v[j].template load<STREAM>(g + j * NORM_THREADS * VE);
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j) add(v[j]);
+    } else {   // the tensor's end
+        const int64_t left = n - e0 - static_cast<int64_t>(threadIdx.x) * VE;
+        int j = 0;
+#pragma unroll 2
+        for (; j + VE <= left; j += NORM_THREADS * VE) {
+            Vec<DT, VE> v;
+            v.load(g + j);
+            add(v);
+        }
+        for (; j < left; ++j) {   // (less than a vector, of one thread)
+            const double x = Elem<DT>::up(g[j]);
+            s = fma(x, x, s);
+        }
+    }
     return s;
 }
 
-__global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(const GradArgs a, const int blocks, double* parts) {
+template <bool STREAM>
+__device__ __forceinline__ double squares_of_block(const Records& records, const int b) {
+    void* p;
+    int64_t n, k;
+    int dtype;
+    records.find(b, &p, &n, &dtype, &k);
+    return dtype == SPARC_F32 ? squares<SPARC_F32, STREAM>(p, n, k)
+           : dtype == SPARC_BF16 ? squares<SPARC_BF16, STREAM>(p, n, k) : squares<SPARC_F16, STREAM>(p, n, k);
+}
+
+__global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(const GradArgs a, double* parts) {
     __shared__ double lds[NORM_THREADS / 64];
+    const Records records(a);
     double s = 0.0;
-    for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
-        const int t = tensor_of(a, b);
-        const int64_t k = b - a.first_block[t];
-        if (a.dtype[t] == SPARC_F32) s += squares<SPARC_F32>(a.p[t], a.n[t], k * (NORM_BYTES / 4));
-        else if (a.dtype[t] == SPARC_BF16) s += squares<SPARC_BF16>(a.p[t], a.n[t], k * (NORM_BYTES / 2));
-        else s += squares<SPARC_F16>(a.p[t], a.n[t], k * (NORM_BYTES / 2));
-    }
+    int b = blockIdx.x;
+    for (; b < a.plain_from; b += gridDim.x) s += squares_of_block<true>(records, b);
+    for (; b < a.blocks; b += gridDim.x) s += squares_of_block<false>(records, b);
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -109,58 +146,86 @@ struct Clip {
     int n_parts;
 };
 
-// The coefficient, in every thread.  A norm that is not finite gives what the formula gives: 0 for an infinite one (so
-// infinite gradients become NaN), NaN for NaN; an infinite max_norm never clips.
-__device__ __forceinline__ float clip_coef(const Clip& c, double* lds) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < c.n_parts; i += BLOCK) s += c.parts[i];
-    s = block_sum(s, lds);
-    const double norm = sqrt(s);
-    if (c.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *c.norm_out = static_cast<float>(norm);
-    const double coef = isinf(c.max_norm) ? 1.0 : c.max_norm / (norm + 1e-6);
-    return coef >= 1.0 ? 1.f : static_cast<float>(coef);
-}
+// The coefficient, in every thread; computed where it is first asked for, behind the loads that do not need it.  A norm that
+// is not finite gives what the formula gives: 0 for an infinite one (so infinite gradients become NaN), NaN for NaN; an
+// infinite max_norm never clips.
+struct Coefficient {
+    const Clip& c;
+    double* lds;
+    float value;
+    bool known;
+    __device__ __forceinline__ Coefficient(const Clip& clip, double* scratch) : c(clip), lds(scratch), value(0.f), known(false) {}
+    __device__ __forceinline__ float get() {   // by the whole workgroup
+        if (!known) {
+            double s = 0.0;
+            for (int i = threadIdx.x; i < c.n_parts; i += BLOCK) s += c.parts[i];
+            const double norm = sqrt(block_sum(s, lds));
+            if (c.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *c.norm_out = static_cast<float>(norm);
+            const double coef = isinf(c.max_norm) ? 1.0 : c.max_norm / (norm + 1e-6);
+            value = coef >= 1.0 ? 1.f : static_cast<float>(coef);
+            known = true;
+        }
+        return value;
+    }
+};
 
-template <int DT>
-__device__ __forceinline__ void scale_block(void* p, const int64_t n, const int64_t e0, const float coef) {
+template <int DT, bool STREAM>
+__device__ __forceinline__ void scale_block(void* p, const int64_t n, const int64_t k, Coefficient& c) {
     typedef typename Elem<DT>::type T;
     constexpr int VE = 16 / sizeof(T), TURNS = BLOCK_BYTES / (BLOCK * 16);
-    T* g = static_cast<T*>(p);
-    Vec<DT, VE> v[TURNS];
+    const int64_t e0 = k * (BLOCK_BYTES / static_cast<int>(sizeof(T)));
+    T* g = static_cast<T*>(p) + e0 + threadIdx.x * VE;
+    auto scaled = [](Vec<DT, VE>& v, const float coef) {
 #pragma unroll
-    for (int k = 0; k < TURNS; ++k) {
-        const int64_t e = e0 + (k * BLOCK + threadIdx.x) * VE;
-        if (e + VE <= n) v[k].load(g + e);
-    }
+        for (int i = 0; i < VE; ++i) v.set(i, v.get(i) * coef);
+    };
+    if (e0 + BLOCK_BYTES / static_cast<int>(sizeof(T)) <= n) {
+        Vec<DT, VE> v[TURNS];
 #pragma unroll
-    for (int k = 0; k < TURNS; ++k) {
-        const int64_t e = e0 + (k * BLOCK + threadIdx.x) * VE;
-        if (e + VE <= n) {
+        for (int j = 0; j < TURNS; ++j) v[j].template load<STREAM>(g + j * BLOCK * VE);
+        const float coef = c.get();
 #pragma unroll
-            for (int i = 0; i < VE; ++i) v[k].set(i, v[k].get(i) * coef);
-            v[k].store(g + e);
-        } else {
-            for (int64_t i = e; i < n; ++i) g[i] = Elem<DT>::down(Elem<DT>::up(g[i]) * coef);
+        for (int j = 0; j < TURNS; ++j) {
+            scaled(v[j], coef);
+            v[j].template store<STREAM>(g + j * BLOCK * VE);
         }
+    } else {
+        const int64_t left = n - e0 - static_cast<int64_t>(threadIdx.x) * VE;
+        const float coef = c.get();
+        int j = 0;
+#pragma unroll 2
+        for (; j + VE <= left; j += BLOCK * VE) {
+            Vec<DT, VE> v;
+            v.load(g + j);
+            scaled(v, coef);
+            v.store(g + j);
+        }
+        for (; j < left; ++j) g[j] = Elem<DT>::down(Elem<DT>::up(g[j]) * coef);
     }
 }
 
-__global__ __launch_bounds__(BLOCK) void grad_scale_kernel(const GradArgs a, const int blocks, const Clip c) {
+// From the last block to the first: the norm's pass left the last ones in the cache.
+template <bool STREAM>
+__global__ __launch_bounds__(BLOCK) void grad_scale_kernel(const GradArgs a, const Clip clip) {
     __shared__ double lds[BLOCK / 64];
-    const float coef = clip_coef(c, lds);
-    for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
-        const int t = tensor_of(a, b);
-        const int64_t k = b - a.first_block[t];
-        if (a.dtype[t] == SPARC_F32) scale_block<SPARC_F32>(a.p[t], a.n[t], k * (BLOCK_BYTES / 4), coef);
-        else if (a.dtype[t] == SPARC_BF16) scale_block<SPARC_BF16>(a.p[t], a.n[t], k * (BLOCK_BYTES / 2), coef);
-        else scale_block<SPARC_F16>(a.p[t], a.n[t], k * (BLOCK_BYTES / 2), coef);
+    const Records records(a);
+    Coefficient c(clip, lds);
+    for (int b = a.blocks - 1 - static_cast<int>(blockIdx.x); b >= 0; b -= gridDim.x) {
+        void* p;
+        int64_t n, k;
+        int dtype;
+        records.find(b, &p, &n, &dtype, &k);
+        if (dtype == SPARC_F32) scale_block<SPARC_F32, STREAM>(p, n, k, c);
+        else if (dtype == SPARC_BF16) scale_block<SPARC_BF16, STREAM>(p, n, k, c);
+        else scale_block<SPARC_F16, STREAM>(p, n, k, c);
     }
+    c.get();   // (a list without elements has a norm too)
 }
 
 struct AdamClipArgs {
     sparc_adam_tensor_t t[ADAM_MOST];
-    int32_t first_block[ADAM_MOST + 1];
-    int n_tensors;
+    int32_t first_block[ADAM_MOST];   // where tensor i's blocks begin; behind the last tensor: INT32_MAX
+    int blocks;
     float step_size, bc2_rsqrt, beta2, one_minus_beta1, one_minus_beta2, eps, weight_decay;
 };
 
@@ -173,37 +238,51 @@ __device__ __forceinline__ void adam_one(float& p, const float g0, float& m, flo
     p -= a.step_size * (m / (sqrtf(v) * a.bc2_rsqrt + a.eps));
 }
 
-__global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, const int blocks, const Clip c) {
+template <bool STREAM>
+__global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, const Clip clip) {
     __shared__ double lds[BLOCK / 64];
     typedef Vec<SPARC_F32, 4> V4;
-    const float coef = clip_coef(c, lds);
-    for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
-        const int ti = tensor_of(a, b);
-        const sparc_adam_tensor_t t = a.t[ti];
-        const int64_t e = (static_cast<int64_t>(b) - a.first_block[ti]) * ADAM_ELEMS + threadIdx.x * 4;
-        if (e + 4 <= t.n) {
-            V4 p, g, m, v;
-            p.load(t.p + e);
-            g.load(t.g + e);
-            m.load(t.m + e);
-            v.load(t.v + e);
+    const int lane = threadIdx.x & 63;
+    const sparc_adam_tensor_t mine = a.t[lane];   // (ADAM_MOST lanes)
+    const int32_t first = a.first_block[lane];
+    static_assert(ADAM_MOST == 64, "a record per lane");
+    Coefficient c(clip, lds);
+    for (int b = blockIdx.x; b < a.blocks; b += gridDim.x) {
+        const int of = __popcll(__ballot(first <= b)) - 1;
+        float* tp = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.p), of));
+        const float* tg = reinterpret_cast<const float*>(lane_value(reinterpret_cast<int64_t>(mine.g), of));
+        float* tm = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.m), of));
+        float* tv = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.v), of));
+        const int64_t n = lane_value(mine.n, of);
+        const int64_t e = static_cast<int64_t>(b - __builtin_amdgcn_readlane(first, of)) * ADAM_ELEMS + threadIdx.x * 4;
+        const bool whole = e + 4 <= n;
+        V4 p, g, m, v;
+        if (whole) {
+            g.load<STREAM>(tg + e);
+            p.load<STREAM>(tp + e);
+            m.load<STREAM>(tm + e);
+            v.load<STREAM>(tv + e);
+        }
+        const float coef = c.get();
+        if (whole) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float pi = p.v[i], mi = m.v[i], vi = v.v[i];
                 adam_one(pi, g.v[i], mi, vi, a, coef);
                 p.v[i] = pi; m.v[i] = mi; v.v[i] = vi;
             }
-            p.store(t.p + e);
-            m.store(t.m + e);
-            v.store(t.v + e);
+            p.store<STREAM>(tp + e);
+            m.store<STREAM>(tm + e);
+            v.store<STREAM>(tv + e);
         } else {
-            for (int64_t i = e; i < t.n; ++i) {
-                float p = t.p[i], m = t.m[i], v = t.v[i];
-                adam_one(p, t.g[i], m, v, a, coef);
-                t.p[i] = p; t.m[i] = m; t.v[i] = v;
+            for (int64_t i = e; i < n; ++i) {
+                float pi = tp[i], mi = tm[i], vi = tv[i];
+                adam_one(pi, tg[i], mi, vi, a, coef);
+                tp[i] = pi; tm[i] = mi; tv[i] = vi;
             }
         }
     }
+    c.get();   // (a list without elements has a norm too)
 }
 
 bool grads_ok(const int64_t n_tensors, const sparc_grad_tensor_t* t) {
@@ -213,20 +292,25 @@ bool grads_ok(const int64_t n_tensors, const sparc_grad_tensor_t* t) {
     return true;
 }
 
-// The first `count` tensors of t as kernel arguments; returns their number of blocks (below 2^30: SPARC_GRAD_MAX_ELEMS).
-int64_t fill(GradArgs& a, const sparc_grad_tensor_t* t, const int count, const int block_bytes) {
-    int64_t blocks = 0;
-    for (int i = 0; i < count; ++i) {
-        a.p[i] = t[i].p;
-        a.n[i] = t[i].n;
-        a.dtype[i] = static_cast<uint8_t>(t[i].dtype);
-        a.first_block[i] = static_cast<int32_t>(blocks);
-        const int64_t per = block_bytes / (t[i].dtype == SPARC_F32 ? 4 : 2);
-        blocks += (t[i].n + per - 1) / per;
+int64_t bytes_of(const sparc_grad_tensor_t& t) { return t.n * (t.dtype == SPARC_F32 ? 4 : 2); }
+
+// The first `count` tensors of t as kernel arguments.  Their number of blocks stays below 2^30 (SPARC_GRAD_MAX_ELEMS).
+// left: bytes of the list from t on.
+void fill(GradArgs& a, const sparc_grad_tensor_t* t, const int count, const int block_bytes, const int64_t left) {
+    int64_t blocks = 0, bytes = 0;
+    for (int i = 0; i < SPARC_GRAD_MAX_TENSORS; ++i) {
+        const bool real = i < count;
+        a.p[i] = real ? t[i].p : nullptr;
+        a.n_dtype[i] = real ? t[i].n << 2 | t[i].dtype : 0;
+        a.first_block[i] = real ? static_cast<int32_t>(blocks) : INT32_MAX;
+        if (!real) continue;
+        bytes += bytes_of(t[i]);
+        blocks += (bytes_of(t[i]) + block_bytes - 1) / block_bytes;
     }
-    a.first_block[count] = static_cast<int32_t>(blocks);
-    a.n_tensors = count;
-    return blocks;
+    a.blocks = static_cast<int>(blocks);
+    const int64_t keep = KEEP_BYTES - (left - bytes);   // of these tensors' bytes
+    const int64_t plain = keep <= 0 ? 0 : keep / block_bytes;
+    a.plain_from = static_cast<int>(keep >= bytes || plain >= blocks ? 0 : blocks - plain);
 }
 
 }  // namespace
@@ -241,15 +325,17 @@ extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* ten
                                int64_t* n_parts, sparc_stream_t stream) {
     if (!parts || !n_parts || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
     if (parts_bytes < sparc_grad_norm_workspace_bytes(n_tensors) || (reinterpret_cast<uintptr_t>(parts) & 7)) return SPARC_ERR_WS;
-    int64_t total = 0;
+    int64_t total = 0, left = 0;
     int launches = 0;
+    for (int64_t i = 0; i < n_tensors; ++i) left += bytes_of(tensors[i]);
     for (int64_t from = 0; from < n_tensors; from += SPARC_GRAD_MAX_TENSORS) {
         GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
-        const int64_t blocks = fill(a, tensors + from, count, NORM_BYTES);
-        if (blocks == 0) continue;
-        const int grid = static_cast<int>(blocks < PARTS ? blocks : PARTS);
-        hipLaunchKernelGGL(grad_squares_kernel, dim3(grid), dim3(NORM_THREADS), 0, stream, a, static_cast<int>(blocks), parts + total);
+        fill(a, tensors + from, count, NORM_BYTES, left);
+        for (int i = 0; i < count; ++i) left -= bytes_of(tensors[from + i]);
+        if (a.blocks == 0) continue;
+        const int grid = a.blocks < PARTS ? a.blocks : PARTS;
+        hipLaunchKernelGGL(grad_squares_kernel, dim3(grid), dim3(NORM_THREADS), 0, stream, a, parts + total);
         SPARC_CHECK_LAUNCH();
         total += grid;
         ++launches;
@@ -267,13 +353,18 @@ extern "C" int sparc_grad_scale(int64_t n_tensors, const sparc_grad_tensor_t* te
                                 double max_norm, float* norm_out, sparc_stream_t stream) {
     if (!parts || !norm_out || n_parts < 0 || n_parts > PARTS || !(max_norm >= 0.0) || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
     Clip c = {parts, norm_out, max_norm, static_cast<int>(n_parts)};
-    for (int64_t from = 0; from < n_tensors || from == 0; from += SPARC_GRAD_MAX_TENSORS) {
+    int64_t left = 0;
+    const int64_t launches = n_tensors ? (n_tensors + SPARC_GRAD_MAX_TENSORS - 1) / SPARC_GRAD_MAX_TENSORS : 1;
+    for (int64_t i = launches - 1; i >= 0; --i) {   // backwards, as inside a launch
+        const int64_t from = i * SPARC_GRAD_MAX_TENSORS;
         GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
-        const int64_t blocks = fill(a, tensors + from, count, BLOCK_BYTES);
-        if (blocks == 0 && !c.norm_out) continue;
-        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(grid), dim3(BLOCK), 0, stream, a, static_cast<int>(blocks), c);
+        for (int k = 0; k < count; ++k) left += bytes_of(tensors[from + k]);
+        fill(a, tensors + from, count, BLOCK_BYTES, left);
+        if (a.blocks == 0 && !c.norm_out) continue;
+        const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
+        if (a.plain_from > 0) hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
+        else hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
         SPARC_CHECK_LAUNCH();
         c.norm_out = nullptr;
     }
@@ -286,23 +377,24 @@ extern "C" int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tenso
     if (n_tensors < 0 || (n_tensors > 0 && !tensors) || step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) ||
         !(eps >= 0.0) || !parts || !norm_out || n_parts < 0 || n_parts > PARTS || !(max_norm >= 0.0))
         return SPARC_ERR_ARG;
+    int64_t all = 0;
     for (int64_t i = 0; i < n_tensors; ++i) {
         const sparc_adam_tensor_t& t = tensors[i];
         if (t.n < 0 || t.n > SPARC_GRAD_MAX_ELEMS || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v))) return SPARC_ERR_ARG;
+        all += t.n;
     }
     const double bc1 = 1.0 - pow(beta1, static_cast<double>(step)), bc2 = 1.0 - pow(beta2, static_cast<double>(step));
     Clip c = {parts, norm_out, max_norm, static_cast<int>(n_parts)};
     for (int64_t from = 0; from < n_tensors || from == 0; from += ADAM_MOST) {
         AdamClipArgs a;
-        const int count = static_cast<int>(n_tensors - from < ADAM_MOST ? n_tensors - from : ADAM_MOST);
-        int64_t blocks = 0;
-        for (int i = 0; i < count; ++i) {
-            a.t[i] = tensors[from + i];
-            a.first_block[i] = static_cast<int32_t>(blocks);
+        int64_t blocks = 0;   // below 2^30
+        for (int i = 0; i < ADAM_MOST; ++i) {
+            const bool real = from + i < n_tensors;
+            a.t[i] = real ? tensors[from + i] : sparc_adam_tensor_t{};
+            a.first_block[i] = real ? static_cast<int32_t>(blocks) : INT32_MAX;
             blocks += (a.t[i].n + ADAM_ELEMS - 1) / ADAM_ELEMS;
         }
-        a.first_block[count] = static_cast<int32_t>(blocks);
-        a.n_tensors = count;
+        a.blocks = static_cast<int>(blocks);
         a.step_size = static_cast<float>(lr / bc1);
         a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
         a.beta2 = static_cast<float>(beta2);
@@ -312,7 +404,8 @@ extern "C" int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tenso
         a.weight_decay = static_cast<float>(weight_decay);
         if (blocks == 0 && !c.norm_out) continue;
         const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
-        hipLaunchKernelGGL(adam_clip_kernel, dim3(grid), dim3(BLOCK), 0, stream, a, static_cast<int>(blocks), c);
+        if (16 * all > KEEP_BYTES) hipLaunchKernelGGL(adam_clip_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
+        else hipLaunchKernelGGL(adam_clip_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
         SPARC_CHECK_LAUNCH();
         c.norm_out = nullptr;
     }

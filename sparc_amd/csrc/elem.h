@@ -4,7 +4,8 @@
 #pragma once
 #include "common.h"
 
-typedef uint32_t sparc_u4 __attribute__((ext_vector_type(4)));
+// What the 256 MB Infinity Cache is left to keep from one pass over the data to the next.
+constexpr int64_t SPARC_KEEP_BYTES = 192000000;
 
 template <int DT>
 struct Elem;
@@ -33,8 +34,17 @@ struct Vec {
     typedef typename Elem<DT>::type T;
     typedef T mem __attribute__((ext_vector_type(VE), aligned(sizeof(T))));
     mem v;
-    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const mem*>(p); }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<mem*>(p) = v; }
+    // STREAM: nontemporal.  A template parameter, because the compiler merges two branches that differ in nothing else.
+    template <bool STREAM = false>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (STREAM) v = __builtin_nontemporal_load(reinterpret_cast<const mem*>(p));
+        else v = *reinterpret_cast<const mem*>(p);
+    }
+    template <bool STREAM = false>
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<mem*>(p));
+        else *reinterpret_cast<mem*>(p) = v;
+    }
     __device__ __forceinline__ float get(const int i) const { return Elem<DT>::up(v[i]); }
     __device__ __forceinline__ void set(const int i, const float x) { v[i] = Elem<DT>::down(x); }
 };
@@ -42,8 +52,16 @@ template <int DT>
 struct Vec<DT, 1> {
     typedef typename Elem<DT>::type T;
     T v;
-    __device__ __forceinline__ void load(const T* p) { v = *p; }
-    __device__ __forceinline__ void store(T* p) const { *p = v; }
+    template <bool STREAM = false>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (STREAM) v = __builtin_nontemporal_load(p);
+        else v = *p;
+    }
+    template <bool STREAM = false>
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+        else *p = v;
+    }
     __device__ __forceinline__ float get(int) const { return Elem<DT>::up(v); }
     __device__ __forceinline__ void set(int, const float x) { v = Elem<DT>::down(x); }
 };

@@ -18,6 +18,12 @@
 
 #include "elem.h"
 
+#ifndef V_RS
+#define V_RS SPARC_KEEP_BYTES
+#endif
+#ifndef V_PER
+#define V_PER 64
+#endif
 namespace {
 
 constexpr int SORT_WAVES = 8;
@@ -58,7 +64,7 @@ __device__ __forceinline__ int64_t token(const void* ids, const int wide, const 
 // the row: it overlaps the one before it and both write the same values.
 constexpr int TURNS = 4;
 
-template <int DT, int VE>
+template <int DT, int VE, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void lookup_kernel(const LookupArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     const T* table = static_cast<const T*>(a.table);
@@ -91,7 +97,7 @@ __global__ __launch_bounds__(BLOCK) void lookup_kernel(const LookupArgs a, const
 #pragma unroll
             for (int i = 0; i < VE; ++i) v[k].set(i, __builtin_nanf(""));
         }
-        v[k].store(out + row * a.ldo + col);
+        v[k].template store<STREAM>(out + row * a.ldo + col);
     }
 }
 
@@ -180,6 +186,7 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
     __shared__ uint32_t sums[SORT_WAVES];
     const bool first = in == nullptr;
     const int digits = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(4 * SORT_BLOCK >= 1 << MOST_BITS, "a thread has four digits");
     uint32_t *base = lds, *total = lds + digits;
     uint16_t* cnt = reinterpret_cast<uint16_t*>(total + digits);
     const int64_t n = first ? a.n : *a.kept;
@@ -190,25 +197,29 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
     // base[d]: tokens of smaller digits in all tiles, and of digit d in the tiles before this one
     for (int d = tid; d < digits; d += SORT_BLOCK) base[d] = total[d] = 0;
     __syncthreads();
-    const int each = (digits + SORT_BLOCK - 1) / SORT_BLOCK;      // digits of a thread: `each` in a row, of every `parts`-th tile
-    const int columns = digits / each, parts = SORT_BLOCK / columns;
-    const int d0 = (tid % columns) * each;
-    for (int k = 0; k < each; ++k) {
-        uint32_t before = 0, all = 0;
-#pragma unroll 8
-        for (int t = tid / columns; t < a.tiles; t += parts) {
-            const uint32_t c = a.counts[static_cast<int64_t>(t) * digits + d0 + k];
-            all += c;
-            before += t < static_cast<int>(blockIdx.x) ? c : 0u;
-        }
-        atomicAdd(base + d0 + k, before);
-        atomicAdd(total + d0 + k, all);
+    const int columns = digits >> 2, parts = SORT_BLOCK / columns;   // four digits of every `parts`-th tile to a thread
+    const int column = tid & (columns - 1);
+    uint4 before = make_uint4(0, 0, 0, 0), all = before;
+    const uint4* counts = reinterpret_cast<const uint4*>(a.counts) + column;
+#pragma unroll 16
+    for (int t = tid / columns; t < a.tiles; t += parts) {
+        const uint4 c = counts[t * columns];
+        const bool earlier = t < static_cast<int>(blockIdx.x);
+        all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
+        before.x += earlier ? c.x : 0u; before.y += earlier ? c.y : 0u; before.z += earlier ? c.z : 0u; before.w += earlier ? c.w : 0u;
+    }
+    const uint32_t before4[4] = {before.x, before.y, before.z, before.w}, all4[4] = {all.x, all.y, all.z, all.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        atomicAdd(base + 4 * column + k, before4[k]);
+        atomicAdd(total + 4 * column + k, all4[k]);
     }
     __syncthreads();
-    uint32_t mine = 0;
+    uint32_t mine[4] = {}, sum = 0;
     if (tid < columns)
-        for (int k = 0; k < each; ++k) mine += total[d0 + k];
-    uint32_t upto = mine;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += mine[k] = total[4 * column + k];
+    uint32_t upto = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const uint32_t below = __shfl_up(upto, off);
@@ -216,15 +227,17 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
     }
     if (lane == 63) sums[wave] = upto;
     __syncthreads();
-    uint32_t smaller = upto - mine, kept = 0;
+    uint32_t smaller = upto - sum, kept = 0;
+#pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) {
         if (w < wave) smaller += sums[w];
         kept += sums[w];
     }
     if (tid < columns)
-        for (int k = 0; k < each; ++k) {
-            base[d0 + k] += smaller;
-            smaller += total[d0 + k];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            base[4 * column + k] += smaller;
+            smaller += mine[k];
         }
     if (first && blockIdx.x == 0 && tid == 0) {
         *a.kept = kept;
@@ -293,7 +306,7 @@ __device__ __forceinline__ int64_t merge_place(const uint2* sorted, const int64_
 // Workers are groups of `lanes` lanes (a power of two); lane u of a group owns VE columns of the slice blockIdx.y.
 constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
 
-template <int DT, int VE>
+template <int DT, int VE, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     __shared__ uint32_t rows_of[STAGE + 2 * MARGIN];     // the workgroup's places, and their rows, from place `from` on
@@ -390,7 +403,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
             Vec<DT, VE> v;
 #pragma unroll
             for (int k = 0; k < VE; ++k) v.set(k, acc[k] * a.scale);
-            v.store(out + (row0 + r) * a.dim + col);
+            v.template store<STREAM>(out + (row0 + r) * a.dim + col);
         }
 #pragma unroll
         for (int k = 0; k < VE; ++k) acc[k] = 0.f;
@@ -645,7 +658,7 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     Plan p;
     p.tile = CHUNK * ceil_div(n > 0 ? n : 1, static_cast<int64_t>(CHUNK) * MOST_TILES);
     p.tiles = static_cast<int>(ceil_div(n > 0 ? n : 1, p.tile));
-    int bits = 1;
+    int bits = 2;
     while ((static_cast<int64_t>(1) << bits) < rows) ++bits;
     // wide digits save passes, but every tile reads the counts of all digits of all tiles
     const int most = p.tiles <= 32 ? MOST_BITS : 8;
@@ -655,17 +668,33 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     p.in_group = BLOCK >> p.lanes_log2;
     // items of a worker: enough workers for every SIMD's wave slots first, up to 64 items then
     const int64_t wanted = ceil_div(n + rows, static_cast<int64_t>(8192) * 64 >> p.lanes_log2);
-    p.per = static_cast<int>(wanted < 4 ? 4 : wanted > 64 ? 64 : wanted);
+    p.per = static_cast<int>(wanted < 4 ? 4 : wanted > V_PER ? V_PER : wanted);
     if (static_cast<int64_t>(p.per) * p.in_group > STAGE) p.per = STAGE / p.in_group;
     p.workers = ceil_div(n + rows, p.per);
     return p;
 }
 
+template <int DT, int VE>
+int launch_lookup(const LookupArgs& a, sparc_stream_t stream) {
+    int slices;
+    const int lanes_log2 = lanes_for(ceil_div(a.dim, VE), &slices);
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.n, static_cast<int64_t>(BLOCK >> lanes_log2) * TURNS)), static_cast<unsigned>(slices));
+    if (a.n * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > SPARC_KEEP_BYTES)
+        hipLaunchKernelGGL((lookup_kernel<DT, VE, true>), grid, dim3(BLOCK), 0, stream, a, lanes_log2);
+    else
+        hipLaunchKernelGGL((lookup_kernel<DT, VE, false>), grid, dim3(BLOCK), 0, stream, a, lanes_log2);
+    SPARC_CHECK_LAUNCH();
+    return SPARC_OK;
+}
+
+// f(type, width): the element type and the elements of a vector as integral constants.
 template <typename F>
-int launch_lookup(F&& f, const int dtype, const bool vectors) {
-    if (dtype == SPARC_F32) return vectors ? f(lookup_kernel<SPARC_F32, 4>) : f(lookup_kernel<SPARC_F32, 1>);
-    if (dtype == SPARC_BF16) return vectors ? f(lookup_kernel<SPARC_BF16, 8>) : f(lookup_kernel<SPARC_BF16, 1>);
-    return vectors ? f(lookup_kernel<SPARC_F16, 8>) : f(lookup_kernel<SPARC_F16, 1>);
+int dispatch(const int dtype, const int64_t dim, F&& f) {
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    if (dtype == SPARC_F32) return dim >= 4 ? f(integral_constant<int, SPARC_F32>(), integral_constant<int, 4>()) : f(integral_constant<int, SPARC_F32>(), one);
+    if (dtype == SPARC_BF16) return dim >= 8 ? f(integral_constant<int, SPARC_BF16>(), integral_constant<int, 8>()) : f(integral_constant<int, SPARC_BF16>(), one);
+    return dim >= 8 ? f(integral_constant<int, SPARC_F16>(), integral_constant<int, 8>()) : f(integral_constant<int, SPARC_F16>(), one);
 }
 
 GradArgs carve(const Plan& p, const int64_t n, const int dim, void* ws, const size_t ws_bytes, bool* ok, size_t* used) {
@@ -692,8 +721,6 @@ extern "C" int sparc_embedding_fwd(int64_t n, int64_t rows, int64_t dim, int dty
         return SPARC_ERR_ARG;
     if (n > SPARC_EMBEDDING_MAX || rows > SPARC_EMBEDDING_MAX || dim > SPARC_EMBEDDING_MAX_DIM) return SPARC_ERR_SIZE;
     if (n == 0 || dim == 0) return SPARC_OK;
-    const int ve = elements_of_16_bytes(dtype);
-    const bool vectors = dim >= ve;
     LookupArgs a;
     a.ids = ids;
     a.table = table;
@@ -705,21 +732,14 @@ extern "C" int sparc_embedding_fwd(int64_t n, int64_t rows, int64_t dim, int dty
     a.dim = static_cast<int>(dim);
     a.wide_ids = ids_64 ? 1 : 0;
     a.scale = static_cast<float>(scale);
-    int slices;
-    const int lanes_log2 = lanes_for(vectors ? ceil_div(dim, ve) : dim, &slices);
-    const int64_t blocks = ceil_div(n, static_cast<int64_t>(BLOCK >> lanes_log2) * TURNS);   // at most 2^27
-    return launch_lookup([&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(slices)), dim3(BLOCK), 0, stream, a, lanes_log2);
-        SPARC_CHECK_LAUNCH();
-        return SPARC_OK;
-    }, dtype, vectors);
+    return dispatch(dtype, dim, [&](auto type, auto width) { return launch_lookup<decltype(type)::value, decltype(width)::value>(a, stream); });
 }
 
 extern "C" size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t dim, int dtype) {
     if (n < 0 || rows < 0 || dim < 0 || n > SPARC_EMBEDDING_MAX || rows > SPARC_EMBEDDING_MAX || dim > SPARC_EMBEDDING_MAX_DIM ||
         dtype < SPARC_F32 || dtype > SPARC_F16)
         return 0;
-    if (n <= FEW) return 256;   // (few_tokens has none)
+    if (n <= FEW) return 0;
     const int ve = elements_of_16_bytes(dtype);
     const Plan p = plan_of(n, rows, static_cast<int>(dim), dim >= ve ? ve : 1);
     bool ok;
@@ -752,8 +772,11 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
         SPARC_CHECK_LAUNCH();
         in = out;
     }
-    hipLaunchKernelGGL((row_sums<DT, VE>), dim3(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), p.slices), dim3(BLOCK), 0, stream, a,
-                       p.lanes_log2);
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), p.slices);
+    if (a.rows * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > V_RS)
+        hipLaunchKernelGGL((row_sums<DT, VE, true>), grid, dim3(BLOCK), 0, stream, a, p.lanes_log2);
+    else
+        hipLaunchKernelGGL((row_sums<DT, VE, false>), grid, dim3(BLOCK), 0, stream, a, p.lanes_log2);
     SPARC_CHECK_LAUNCH();
     hipLaunchKernelGGL((join_rows<DT>), dim3(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64)), dim3(BLOCK), 0, stream, a);
     SPARC_CHECK_LAUNCH();
@@ -765,7 +788,7 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
 extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dtype, const void* ids, int ids_64, const void* g,
                                     int64_t ldg, double scale, int64_t padding_idx, void* out, void* ws, size_t ws_bytes,
                                     sparc_stream_t stream) {
-    if (n < 0 || rows < 0 || dim < 0 || dtype < SPARC_F32 || dtype > SPARC_F16 || ldg < dim || !out || !ws || (n > 0 && (!ids || !g)))
+    if (n < 0 || rows < 0 || dim < 0 || dtype < SPARC_F32 || dtype > SPARC_F16 || ldg < dim || !out || (n > 0 && (!ids || !g)))
         return SPARC_ERR_ARG;
     if (n > SPARC_EMBEDDING_MAX || rows > SPARC_EMBEDDING_MAX || dim > SPARC_EMBEDDING_MAX_DIM) return SPARC_ERR_SIZE;
     if (rows == 0 || dim == 0) return SPARC_OK;
@@ -774,7 +797,6 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
     Plan p = {};
     const bool few = n <= FEW;
     if (few) {
-        if (ws_bytes < 256 || (reinterpret_cast<uintptr_t>(ws) & 255)) return SPARC_ERR_WS;   // (as for more tokens)
         p.lanes_log2 = lanes_for(ceil_div(dim, used_ve), &p.slices);
         int64_t per = ceil_div(rows, FEW_BLOCKS);
         const int64_t most = static_cast<int64_t>(1) << (32 - PLACE_BITS - 1);   // (keys stay below the one that pads the sort)
@@ -785,7 +807,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         bool ok;
         size_t used;
         a = carve(p, n, static_cast<int>(dim), ws, ws_bytes, &ok, &used);
-        if (!ok) return SPARC_ERR_WS;
+        if (!ws || !ok) return SPARC_ERR_WS;
         a.per = p.per;
     }
     a.ids = ids;
@@ -800,13 +822,8 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
     a.dim = static_cast<int>(dim);
     a.wide_ids = ids_64 ? 1 : 0;
     a.scale = static_cast<float>(scale);
-    auto run = [&](auto type, auto width) {
+    return dispatch(dtype, dim, [&](auto type, auto width) {
         constexpr int DT = decltype(type)::value, VE = decltype(width)::value;
         return few ? launch_few<DT, VE>(a, p.lanes_log2, p.slices, stream) : launch_grad<DT, VE>(a, p, stream);
-    };
-    using std::integral_constant;
-    const integral_constant<int, 1> one;
-    if (dtype == SPARC_F32) return used_ve > 1 ? run(integral_constant<int, SPARC_F32>(), integral_constant<int, 4>()) : run(integral_constant<int, SPARC_F32>(), one);
-    if (dtype == SPARC_BF16) return used_ve > 1 ? run(integral_constant<int, SPARC_BF16>(), integral_constant<int, 8>()) : run(integral_constant<int, SPARC_BF16>(), one);
-    return used_ve > 1 ? run(integral_constant<int, SPARC_F16>(), integral_constant<int, 8>()) : run(integral_constant<int, SPARC_F16>(), one);
+    });
 }

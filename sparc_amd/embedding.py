@@ -74,14 +74,17 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
         g = g.contiguous()
     ld = _rows_of(g, "grad")
     pad = _padding(padding_idx, rows)
-    out = torch.empty(rows, dim, dtype=g.dtype, device=dev)
-    if out.numel():
-        n = ids.numel()
-        nbytes = lib.sparc_embedding_grad_workspace_bytes(n, rows, dim, DTYPES[g.dtype])
-        ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=dev)   # of this call alone: streams and graphs share nothing
-        at = ws.data_ptr()
-        launch("sparc_embedding_grad", lib.sparc_embedding_grad, dev, n, rows, dim, DTYPES[g.dtype], ids.data_ptr(),
-               _ID_DTYPES[ids.dtype], g.data_ptr(), ld, scale, pad, out.data_ptr(), at + (-at) % 256, nbytes)
+    out = g.new_empty((rows, dim))
+    if rows and dim:
+        n, code = ids.numel(), DTYPES[g.dtype]
+        nbytes = lib.sparc_embedding_grad_workspace_bytes(n, rows, dim, code)
+        at = None
+        if nbytes:
+            ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=dev)   # of this call alone: streams and graphs share nothing
+            at = ws.data_ptr()
+            at += (-at) % 256
+        launch("sparc_embedding_grad", lib.sparc_embedding_grad, dev, n, rows, dim, code, ids.data_ptr(), _ID_DTYPES[ids.dtype],
+               g.data_ptr(), ld, scale, pad, out.data_ptr(), at, nbytes)
     return out
 
 

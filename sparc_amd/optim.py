@@ -6,6 +6,7 @@ torch's own."""
 from __future__ import annotations
 
 import ctypes
+import operator
 from array import array
 
 import torch
@@ -27,22 +28,35 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _norm_of(grads, device):
-    """(records for the C calls: keep the array while they run, partial sums of the squares on the device, how many)."""
-    flat = []
-    code_of = DTYPES.get
-    for g in grads:
-        code = code_of(g.dtype)
-        if code is None or g.device != device or g.is_sparse or not (g.is_contiguous() or _dense(g)):
-            raise ValueError("the gradients of one norm are dense float32, bfloat16 or float16 tensors on one device")
-        flat += (g.data_ptr(), g.numel(), code)
-    records = array("q", flat)
-    n = len(grads)
+_type_of, _is_sparse = operator.attrgetter("dtype"), operator.attrgetter("is_sparse")
+_device_of, _address_of, _size_of = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
+_is_contiguous = torch.Tensor.is_contiguous
+
+
+def _grad_records(grads, device):
+    """The list as the C calls take it (an array of {address, elements, type}: keep it while they run)."""
+    types = list(map(_type_of, grads))
+    if any(map(_is_sparse, grads)) or set(map(_device_of, grads)) != {device.index} or not DTYPES.keys() >= set(types) \
+            or not (all(map(_is_contiguous, grads)) or all(map(_dense, grads))):
+        raise ValueError("the gradients of one norm are dense float32, bfloat16 or float16 tensors on one device")
+    return _records(list(map(_address_of, grads)), list(map(_size_of, grads)), [DTYPES[t] for t in types])
+
+
+def _records(*columns):
+    """One int64 array of the columns' entries, record by record."""
+    out = array("q", bytes(8 * len(columns) * len(columns[0])))
+    for i, column in enumerate(columns):
+        out[i::len(columns)] = array("q", column)
+    return out
+
+
+def _norm_of(records, n, device):
+    """(partial sums of the squares on the device, how many) of n records."""
     nbytes = lib.sparc_grad_norm_workspace_bytes(n)
     parts = torch.empty(nbytes >> 3, dtype=torch.float64, device=device)
     count = ctypes.c_int64()
     launch("sparc_grad_norm", lib.sparc_grad_norm, device, n, _address(records), parts.data_ptr(), nbytes, ctypes.byref(count))
-    return records, parts, count.value
+    return parts, count.value
 
 
 def _address(records) -> int:
@@ -72,7 +86,8 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     device = grads[0].device
     if not grads[0].is_cuda:
         require_gpu(device)
-    records, parts, count = _norm_of(grads, device)
+    records = _grad_records(grads, device)
+    parts, count = _norm_of(records, len(grads), device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     launch("sparc_grad_scale", lib.sparc_grad_scale, device, len(grads), _address(records), parts.data_ptr(), count, max_norm,
            norm.data_ptr())
@@ -80,16 +95,15 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 
 
 def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
-    flat = []
-    f32 = torch.float32
-    for of_one in zip(params, grads, exp_avgs, exp_avg_sqs):
-        n = of_one[0].numel()
-        for t in of_one:
-            if t.dtype is not f32 or t.numel() != n or t.device != device or not t.is_contiguous():
-                raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
-            flat.append(t.data_ptr())
-        flat.append(n)
-    return array("q", flat)
+    """(records of the update, records of the gradients)."""
+    n = len(params)
+    every = [*params, *grads, *exp_avgs, *exp_avg_sqs]
+    sizes = list(map(_size_of, every))
+    if set(map(_type_of, every)) != {torch.float32} or any(map(_is_sparse, every)) or set(map(_device_of, every)) != {device.index} \
+            or not all(map(_is_contiguous, every)) or sizes != sizes[:n] * 4:
+        raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
+    at = list(map(_address_of, every))
+    return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), _records(at[n:2 * n], sizes[:n], [0] * n)
 
 
 @torch.no_grad()
@@ -106,13 +120,13 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     device = params[0].device
     if not params[0].is_cuda:
         require_gpu(device)
-    records = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
+    records, of_grads = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
     rates = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
     if max_grad_norm is None:
         _adam_launches(records, len(params), rates, device)
         return None
     max_grad_norm = _limit(max_grad_norm)
-    _, parts, count = _norm_of(grads, device)
+    parts, count = _norm_of(of_grads, len(params), device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, len(params), _address(records), *rates, parts.data_ptr(),
            count, max_grad_norm, norm.data_ptr())
@@ -183,11 +197,12 @@ class Adam(torch.optim.Optimizer):
         if max_norm is not None:
             device = work[0][1][0].device
             require_gpu(device)
-            _, parts, count = _norm_of([g for w in work for g in w[2]], device)
+            grads = [g for w in work for g in w[2]]
+            parts, count = _norm_of(_grad_records(grads, device), len(grads), device)
             self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
         for group, live, grads, ms, vs in work:
             dev = live[0].device
-            records = _adam_records(live, grads, ms, vs, dev)
+            records, _ = _adam_records(live, grads, ms, vs, dev)
             rates = (float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                      float(group["weight_decay"]), int(group["step"]))
             if max_norm is not None:

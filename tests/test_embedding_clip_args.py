@@ -17,25 +17,26 @@ def test_embedding_arguments():
     for bad in (dict(n=1 << 31), dict(rows=1 << 31), dict(dim=(1 << 20) + 1, ld=1 << 21, ldo=1 << 21)):
         assert fwd(**bad) == -4, bad
     assert fwd(n=0) == 0 and fwd(dim=0, ld=0, ldo=0) == 0                    # nothing to do, nothing launched
-    grad = lambda n=4, rows=5, dim=8, dtype=0, ids=P, g=P, ldg=8, out=P, ws=P, nbytes=1 << 40: lib.sparc_embedding_grad(  # noqa: E731
+    grad = lambda n=20000, rows=5, dim=8, dtype=0, ids=P, g=P, ldg=8, out=P, ws=P, nbytes=1 << 40: lib.sparc_embedding_grad(  # noqa: E731
         n, rows, dim, dtype, ids, 0, g, ldg, 1.0, -1, out, ws, nbytes, None)
     for bad in (dict(n=-1), dict(rows=-1), dict(dim=-1), dict(dtype=3), dict(ids=None), dict(g=None), dict(out=None),
-                dict(ws=None), dict(ldg=7)):
+                dict(ldg=7)):
         assert grad(**bad) == -1, bad
     for bad in (dict(n=1 << 31), dict(rows=1 << 31), dict(dim=(1 << 20) + 1, ldg=1 << 21)):
         assert grad(**bad) == -4, bad
-    assert grad(nbytes=16) == -2 and grad(ws=P + 8) == -2
+    assert grad(nbytes=16) == -2 and grad(ws=P + 8) == -2 and grad(ws=None) == -2
     assert grad(rows=0) == 0 and grad(dim=0, ldg=0) == 0
     assert lib.sparc_embedding_grad_workspace_bytes(1 << 31, 5, 8, 0) == 0
     assert lib.sparc_embedding_grad_workspace_bytes(4, 5, 8, 7) == 0
-    assert lib.sparc_embedding_grad_workspace_bytes(0, 5, 8, 0) > 0
+    assert lib.sparc_embedding_grad_workspace_bytes(16384, 5, 8, 0) == 0        # one launch, without scratch
+    assert lib.sparc_embedding_grad_workspace_bytes(16385, 5, 8, 0) > 0
 
 
 def test_gradient_workspace_stays_near_its_operands():
     """A few words per token and row, and partial sums: never a multiple of the gradient for sizes that occur."""
     from sparc_amd._lib import lib
-    for n, rows, dim, dtype, size in ((2437, 2708, 64, 0, 4), (48979, 2449029, 64, 0, 4), (262147, 50021, 512, 1, 2), (1, 1, 1, 0, 4),
-                                      (2_000_000_000, 1000, 1, 2, 2), (1000, 2_000_000_000, 1, 2, 2)):
+    for n, rows, dim, dtype, size in ((20437, 2708, 64, 0, 4), (48979, 2449029, 64, 0, 4), (262147, 50021, 512, 1, 2), (16385, 1, 1, 0, 4),
+                                      (2_000_000_000, 1000, 1, 2, 2), (17000, 2_000_000_000, 1, 2, 2)):
         nbytes = lib.sparc_embedding_grad_workspace_bytes(n, rows, dim, dtype)
         assert 0 < nbytes <= 64 * (n + rows) + 4 * (n + rows) * dim * size + (1 << 26), (n, rows, dim)
 
