@@ -18,11 +18,8 @@
 
 #include "elem.h"
 
-#ifndef V_RS
-#define V_RS SPARC_KEEP_BYTES
-#endif
-#ifndef V_PER
-#define V_PER 64
+#ifndef V_FILL
+#define V_FILL 4
 #endif
 namespace {
 
@@ -122,8 +119,8 @@ struct GradArgs {
     float* part;               // [2 workers][dim]
 };
 
-// Lanes below this one whose key equals mine, among the lanes of `live`; *all: every such lane.
-__device__ __forceinline__ int rank_among_equals(const uint32_t key, const int bits, const uint64_t live, uint64_t* all) {
+// The lanes of `live` whose key equals mine.
+__device__ __forceinline__ uint64_t equals(const uint32_t key, const int bits, const uint64_t live) {
     uint32_t lo = static_cast<uint32_t>(live), hi = static_cast<uint32_t>(live >> 32);
 #pragma unroll
     for (int b = 0; b < MOST_BITS; ++b) {
@@ -133,8 +130,36 @@ __device__ __forceinline__ int rank_among_equals(const uint32_t key, const int b
         lo &= ~(static_cast<uint32_t>(ones) ^ mine);             // the lanes whose bit is mine
         hi &= ~(static_cast<uint32_t>(ones >> 32) ^ mine);
     }
-    *all = static_cast<uint64_t>(hi) << 32 | lo;
-    return __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// Zeros that a launch of the sort writes with workgroups of its own behind the sorting ones: the sort waits on memory
+// latency and leaves the bandwidth idle.
+struct Zeros {
+    uint16_t* p;
+    int64_t count;         // of uint16
+    bool streaming;
+};
+constexpr int ZERO_CHUNK = SORT_BLOCK * 8 * 8;   // uint16 of a workgroup: eight 16-byte stores per thread
+
+__device__ __forceinline__ void write_zeros(const Zeros& z, const int64_t chunk) {
+    typedef uint16_t mem __attribute__((ext_vector_type(8), aligned(2)));
+    const mem zero = {};
+    const int64_t from = chunk * ZERO_CHUNK + threadIdx.x * 8;
+    if ((chunk + 1) * ZERO_CHUNK <= z.count) {
+        if (z.streaming) {
+#pragma unroll 8
+            for (int k = 0; k < 8; ++k) __builtin_nontemporal_store(zero, reinterpret_cast<mem*>(z.p + from + k * SORT_BLOCK * 8));
+        } else {
+            for (int k = 0; k < 8; ++k) *reinterpret_cast<mem*>(z.p + from + k * SORT_BLOCK * 8) = zero;
+        }
+        return;
+    }
+    for (int64_t i = from; i < z.count; i += SORT_BLOCK * 8) {
+        if (i + 8 <= z.count) *reinterpret_cast<mem*>(z.p + i) = zero;
+        else
+            for (int64_t k = i; k < z.count; ++k) z.p[k] = 0;
+    }
 }
 
 // The next UP_FRONT {row, place} of this lane, places i0 + 64 k + lane below hi; row = ~0: none.
@@ -162,8 +187,9 @@ __device__ __forceinline__ void take(const GradArgs& a, const bool first, const 
 }
 
 // Digits of the tokens of a tile: digit = (row >> shift) & (1 << bits) - 1.
-__global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, const uint2* in, const int shift, const int bits) {
+__global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, const Zeros z, const uint2* in, const int shift, const int bits) {
     __shared__ uint32_t cnt[1 << MOST_BITS];
+    if (static_cast<int>(blockIdx.x) >= a.tiles) return write_zeros(z, blockIdx.x - a.tiles);
     const bool first = in == nullptr;
     const int digits = 1 << bits;
     const int64_t n = first ? a.n : *a.kept;
@@ -181,9 +207,10 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, con
     for (int i = threadIdx.x; i < digits; i += SORT_BLOCK) a.counts[static_cast<int64_t>(blockIdx.x) * digits + i] = cnt[i];
 }
 
-__global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, const uint2* in, uint2* out, const int shift, const int bits) {
+__global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, const Zeros z, const uint2* in, uint2* out, const int shift, const int bits) {
     extern __shared__ __align__(16) uint32_t lds[];   // base [digits], total [digits], cnt uint16 [SORT_WAVES][digits]
     __shared__ uint32_t sums[SORT_WAVES];
+    if (static_cast<int>(blockIdx.x) >= a.tiles) return write_zeros(z, blockIdx.x - a.tiles);
     const bool first = in == nullptr;
     const int digits = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     static_assert(4 * SORT_BLOCK >= 1 << MOST_BITS, "a thread has four digits");
@@ -201,12 +228,21 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
     const int column = tid & (columns - 1);
     uint4 before = make_uint4(0, 0, 0, 0), all = before;
     const uint4* counts = reinterpret_cast<const uint4*>(a.counts) + column;
-#pragma unroll 16
-    for (int t = tid / columns; t < a.tiles; t += parts) {
-        const uint4 c = counts[t * columns];
-        const bool earlier = t < static_cast<int>(blockIdx.x);
-        all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
-        before.x += earlier ? c.x : 0u; before.y += earlier ? c.y : 0u; before.z += earlier ? c.z : 0u; before.w += earlier ? c.w : 0u;
+    constexpr int LOADS = 8;   // in flight
+    for (int t0 = tid / columns; t0 < a.tiles; t0 += LOADS * parts) {
+        uint4 c[LOADS];
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) {
+            const int t = t0 + k * parts;
+            c[k] = t < a.tiles ? counts[t * columns] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) {
+            const bool earlier = t0 + k * parts < static_cast<int>(blockIdx.x);
+            all.x += c[k].x; all.y += c[k].y; all.z += c[k].z; all.w += c[k].w;
+            before.x += earlier ? c[k].x : 0u; before.y += earlier ? c[k].y : 0u;
+            before.z += earlier ? c[k].z : 0u; before.w += earlier ? c[k].w : 0u;
+        }
     }
     const uint32_t before4[4] = {before.x, before.y, before.z, before.w}, all4[4] = {all.x, all.y, all.z, all.w};
 #pragma unroll
@@ -249,17 +285,21 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
         for (int i = tid; i < SORT_WAVES * digits / 2; i += SORT_BLOCK) words[i] = 0;
         __syncthreads();
         uint16_t* own = cnt + wave * digits;
-        uint32_t at[UP_FRONT];   // rank among the wave's tokens of the digit
+        uint64_t same[UP_FRONT];
+        uint32_t digit[UP_FRONT], at[UP_FRONT];   // at: rank among the wave's tokens of the digit
 #pragma unroll
         for (int k = 0; k < UP_FRONT; ++k) {
             const bool ok = e[k].x != ~0u;
-            const uint32_t d = ok ? (e[k].x >> shift) & (digits - 1) : 0u;
-            uint64_t same;
-            const int r = rank_among_equals(d, bits, __ballot(ok), &same);
-            if (ok) {
-                const uint32_t c0 = own[d];
+            digit[k] = ok ? (e[k].x >> shift) & (digits - 1) : 0u;
+            same[k] = equals(digit[k], bits, __ballot(ok));
+        }
+#pragma unroll
+        for (int k = 0; k < UP_FRONT; ++k) {
+            const int r = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(same[k] >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(same[k]), 0u));
+            if (e[k].x != ~0u) {
+                const uint32_t c0 = own[digit[k]];
                 at[k] = c0 + r;
-                if (r == 0) own[d] = static_cast<uint16_t>(c0 + __popcll(same));
+                if (r == 0) own[digit[k]] = static_cast<uint16_t>(c0 + __popcll(same[k]));
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the counters as the next turn's lanes find them
         }
@@ -277,10 +317,7 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < UP_FRONT; ++k)
-            if (e[k].x != ~0u) {
-                const uint32_t d = (e[k].x >> shift) & (digits - 1);
-                out[base[d] + own[d] + at[k]] = e[k];
-            }
+            if (e[k].x != ~0u) out[base[digit[k]] + own[digit[k]] + at[k]] = e[k];
         __syncthreads();
         for (int d = tid; d < digits; d += SORT_BLOCK) base[d] += total[d];
     }
@@ -304,30 +341,36 @@ __device__ __forceinline__ int64_t merge_place(const uint2* sorted, const int64_
 }
 
 // Workers are groups of `lanes` lanes (a power of two); lane u of a group owns VE columns of the slice blockIdx.y.
+// FILLED: the table holds zeros already (written beside the sort) and a worker's items are places alone, the rows without
+// any cost nothing.
 constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
 
-template <int DT, int VE, bool STREAM>
+template <int DT, int VE, bool FILLED, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
-    __shared__ uint32_t rows_of[STAGE + 2 * MARGIN];     // the workgroup's places, and their rows, from place `from` on
-    __shared__ uint32_t places[STAGE + 2 * MARGIN];
+    extern __shared__ __align__(16) uint32_t staged[];   // the workgroup's places from place `from` on: their rows, then they
     __shared__ int64_t edge[2];
     const T* g = static_cast<const T*>(a.g);
     T* out = static_cast<T*>(a.out);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lanes = 1 << lanes_log2, in_group = BLOCK >> lanes_log2;
     const int u = tid & (lanes - 1);
+    uint32_t *rows_of = staged, *places = staged + (in_group * a.per + 2 * MARGIN);
     const int64_t first_worker = static_cast<int64_t>(blockIdx.x) * in_group;
     const int64_t all_places = *a.kept;
-    const int64_t items = all_places + a.rows;
+    const int64_t items = FILLED ? all_places : all_places + a.rows;
     const int64_t d0 = min(first_worker * a.per, items), d1 = min(d0 + static_cast<int64_t>(in_group) * a.per, items);
     if (d0 >= d1) return;                                // (the whole workgroup)
-    if (wave < 2) {
-        const int64_t e = merge_place(a.sorted, all_places, a.rows, wave ? d1 : d0);
-        if (lane == 0) edge[wave] = e;
+    int64_t e_first = d0, e_last = d1;
+    if constexpr (!FILLED) {
+        if (wave < 2) {
+            const int64_t e = merge_place(a.sorted, all_places, a.rows, wave ? d1 : d0);
+            if (lane == 0) edge[wave] = e;
+        }
+        __syncthreads();
+        e_first = edge[0];
+        e_last = edge[1];
     }
-    __syncthreads();
-    const int64_t e_first = edge[0], e_last = edge[1];
     const int64_t from = max(e_first - MARGIN, static_cast<int64_t>(0)), to = min(e_last + MARGIN, all_places);
     for (int64_t k = from + tid; k < to; k += BLOCK) {
         const uint2 s = a.sorted[k];
@@ -340,10 +383,11 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     const int col = min((static_cast<int>(blockIdx.y) * lanes + u) * VE, a.dim - VE);
     if (w0 >= w1 || (static_cast<int>(blockIdx.y) * lanes + u) * VE >= a.dim) return;   // no barrier below
     // from here on: places relative to `from`, rows relative to row0
-    const int64_t row0 = d0 - e_first;
+    const int64_t row0 = FILLED ? 0 : d0 - e_first;
     const int n_staged = static_cast<int>(to - from), i_first = static_cast<int>(e_first - from), i_last = static_cast<int>(e_last - from);
     auto row_at = [&](const int i) { return static_cast<int>(rows_of[i] - row0); };
     auto split = [&](const int64_t d) {                  // the first place at or behind item d
+        if constexpr (FILLED) return i_first + static_cast<int>(d - d0);
         int lo = i_first, hi = min(i_last, i_first + static_cast<int>(d - d0));
         const int64_t limit = d - d0 + i_first;          // item of place i: d0 + i - i_first + row_at(i)
         while (lo < hi) {
@@ -371,7 +415,15 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
         return f_lo - s_lo > LONG_ROW ? -1 : f_lo;
     };
     int i = split(w0), i_stop = split(w1);
-    int r = static_cast<int>(w0 - d0) - (i - i_first), r_stop = static_cast<int>(w1 - d0) - (i_stop - i_first);
+    // the rows that this worker finishes: r .. r_stop - 1 (FILLED: the row at hand, and the one at the end)
+    int r, r_stop;
+    if constexpr (FILLED) {
+        r = row_at(i);
+        r_stop = i_stop < n_staged ? row_at(i_stop) : -1;
+    } else {
+        r = static_cast<int>(w0 - d0) - (i - i_first);
+        r_stop = static_cast<int>(w1 - d0) - (i_stop - i_first);
+    }
     int c = cut(i, r);
     bool inside = c < 0;                                 // the first row is a long one that began in an earlier worker
     if (c > 0) {                                         // an earlier worker has the whole row
@@ -384,7 +436,8 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
         i_stop = c;
         ++r_stop;
     }
-    if (r > r_stop || (r == r_stop && i >= i_stop)) return;
+    if (FILLED ? i >= i_stop : r > r_stop || (r == r_stop && i >= i_stop)) return;
+    if constexpr (FILLED) r = row_at(i);
     float acc[VE];
 #pragma unroll
     for (int k = 0; k < VE; ++k) acc[k] = 0.f;
@@ -418,14 +471,23 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
         for (int k = 0; k < AHEAD; ++k) {
             if (i + k >= i_stop) break;
             const int row = row_at(i + k);
-            while (r < row) finish_row();
+            if constexpr (FILLED) {
+                if (r != row) finish_row();
+                r = row;
+            } else {
+                while (r < row) finish_row();
+            }
 #pragma unroll
             for (int j = 0; j < VE; ++j) acc[j] += ahead[k].get(j);
             if (i + k + AHEAD < i_stop) ahead[k].load(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
         }
         i += AHEAD;
     }
-    while (r < r_stop) finish_row();
+    if constexpr (FILLED) {
+        if (!goes_on) finish_row();
+    } else {
+        while (r < r_stop) finish_row();
+    }
     if (goes_on) {
         float* p = a.part + (2 * worker + (inside ? 0 : 1)) * a.dim + col;
 #pragma unroll
@@ -435,7 +497,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
 
 // Long rows: slice blockIdx.y of 64 columns, a lane per column; the waves take a quarter of the pieces each.
 template <int DT>
-__global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a) {
+__global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a, const bool filled) {
     typedef typename Elem<DT>::type T;
     __shared__ double sum[WAVES][64];
     __shared__ int64_t start;
@@ -456,7 +518,7 @@ __global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a) {
             if (lane == 0) start = lo;
         }
         __syncthreads();
-        const int64_t first = (row + start) / a.per;
+        const int64_t first = (filled ? start : row + start) / a.per;
         const int64_t pieces = last - first + 1, each = (pieces + WAVES - 1) / WAVES;
         const int64_t lo = min(wave * each, pieces), hi = min(lo + each, pieces);
         double s = 0.0;
@@ -642,6 +704,7 @@ __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int 
 struct Plan {
     int64_t tile, workers;
     int tiles, passes, bits, per, lanes_log2, slices, in_group;
+    bool filled;
 };
 
 int64_t ceil_div(const int64_t a, const int64_t b) { return (a + b - 1) / b; }
@@ -666,11 +729,14 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     p.bits = (bits + p.passes - 1) / p.passes;
     p.lanes_log2 = lanes_for((dim + ve - 1) / ve, &p.slices);
     p.in_group = BLOCK >> p.lanes_log2;
+    // zeros beside the sort where most rows have no token: they are written twice where they have one
+    p.filled = rows >= V_FILL * n;
     // items of a worker: enough workers for every SIMD's wave slots first, up to 64 items then
-    const int64_t wanted = ceil_div(n + rows, static_cast<int64_t>(8192) * 64 >> p.lanes_log2);
-    p.per = static_cast<int>(wanted < 4 ? 4 : wanted > V_PER ? V_PER : wanted);
+    const int64_t items = p.filled ? n : n + rows;
+    const int64_t wanted = ceil_div(items, static_cast<int64_t>(8192) * 64 >> p.lanes_log2);
+    p.per = static_cast<int>(wanted < 4 ? 4 : wanted > 64 ? 64 : wanted);
     if (static_cast<int64_t>(p.per) * p.in_group > STAGE) p.per = STAGE / p.in_group;
-    p.workers = ceil_div(n + rows, p.per);
+    p.workers = ceil_div(items, p.per);
     return p;
 }
 
@@ -750,35 +816,57 @@ extern "C" size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, 
 
 namespace {
 
-template <int DT, int VE>
-int launch_few(const GradArgs& a, const int lanes_log2, const int slices, sparc_stream_t stream) {
-    size_t keys = 1;
-    while (keys < static_cast<size_t>(a.n)) keys <<= 1;
-    hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(static_cast<unsigned>(ceil_div(a.rows, a.per)), static_cast<unsigned>(slices)), dim3(BLOCK),
-                       keys * sizeof(uint32_t), stream, a, lanes_log2);
+template <int DT, int VE, bool FILLED>
+int launch_sums(const GradArgs& a, const Plan& p, const bool streaming, sparc_stream_t stream) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), static_cast<unsigned>(p.slices));
+    const size_t lds = static_cast<size_t>(p.per * p.in_group + 2 * MARGIN) * 2 * sizeof(uint32_t);
+    if (streaming) hipLaunchKernelGGL((row_sums<DT, VE, FILLED, true>), grid, dim3(BLOCK), lds, stream, a, p.lanes_log2);
+    else hipLaunchKernelGGL((row_sums<DT, VE, FILLED, false>), grid, dim3(BLOCK), lds, stream, a, p.lanes_log2);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
 
 template <int DT, int VE>
 int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
+    const int64_t half_words = a.rows * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) / 2;
+    const bool streaming = 2 * half_words > SPARC_KEEP_BYTES;
     const size_t lds = (static_cast<size_t>(1) << p.bits) * (2 * sizeof(uint32_t) + SORT_WAVES * sizeof(uint16_t));
+    // the zeros are dealt to the launches of the sort
+    const int64_t chunks = p.filled ? ceil_div(half_words, ZERO_CHUNK) : 0, each = ceil_div(chunks, 2 * p.passes);
+    int64_t dealt = 0;
+    Zeros z = {};
+    auto grid = [&]() {
+        const int64_t mine = each < chunks - dealt ? each : chunks - dealt;
+        z.p = static_cast<uint16_t*>(a.out) + dealt * ZERO_CHUNK;
+        z.count = half_words - dealt * ZERO_CHUNK < mine * ZERO_CHUNK ? half_words - dealt * ZERO_CHUNK : mine * ZERO_CHUNK;
+        z.streaming = streaming;
+        dealt += mine;
+        return dim3(static_cast<unsigned>(p.tiles + mine));
+    };
     const uint2* in = nullptr;   // the ids themselves
     for (int pass = 0; pass < p.passes; ++pass) {
         uint2* out = (p.passes - pass) & 1 ? a.sorted : a.other;
-        hipLaunchKernelGGL(digit_counts, dim3(p.tiles), dim3(SORT_BLOCK), 0, stream, a, in, pass * p.bits, p.bits);
+        const dim3 counting = grid();
+        hipLaunchKernelGGL(digit_counts, counting, dim3(SORT_BLOCK), 0, stream, a, z, in, pass * p.bits, p.bits);
         SPARC_CHECK_LAUNCH();
-        hipLaunchKernelGGL(digit_scatter, dim3(p.tiles), dim3(SORT_BLOCK), lds, stream, a, in, out, pass * p.bits, p.bits);
+        const dim3 scattering = grid();
+        hipLaunchKernelGGL(digit_scatter, scattering, dim3(SORT_BLOCK), lds, stream, a, z, in, out, pass * p.bits, p.bits);
         SPARC_CHECK_LAUNCH();
         in = out;
     }
-    const dim3 grid(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), p.slices);
-    if (a.rows * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > V_RS)
-        hipLaunchKernelGGL((row_sums<DT, VE, true>), grid, dim3(BLOCK), 0, stream, a, p.lanes_log2);
-    else
-        hipLaunchKernelGGL((row_sums<DT, VE, false>), grid, dim3(BLOCK), 0, stream, a, p.lanes_log2);
+    const int rc = p.filled ? launch_sums<DT, VE, true>(a, p, false, stream) : launch_sums<DT, VE, false>(a, p, streaming, stream);
+    if (rc != SPARC_OK) return rc;
+    hipLaunchKernelGGL((join_rows<DT>), dim3(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64)), dim3(BLOCK), 0, stream, a, p.filled);
     SPARC_CHECK_LAUNCH();
-    hipLaunchKernelGGL((join_rows<DT>), dim3(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64)), dim3(BLOCK), 0, stream, a);
+    return SPARC_OK;
+}
+
+template <int DT, int VE>
+int launch_few(const GradArgs& a, const int lanes_log2, const int slices, sparc_stream_t stream) {
+    size_t keys = 1;
+    while (keys < static_cast<size_t>(a.n)) keys <<= 1;
+    hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(static_cast<unsigned>(ceil_div(a.rows, a.per)), static_cast<unsigned>(slices)), dim3(BLOCK),
+                       keys * sizeof(uint32_t), stream, a, lanes_log2);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
