@@ -18,9 +18,6 @@
 
 #include "elem.h"
 
-#ifndef V_FILL
-#define V_FILL 4
-#endif
 namespace {
 
 constexpr int SORT_WAVES = 8;
@@ -33,8 +30,8 @@ constexpr int WAVES = 4;
 constexpr int BLOCK = 64 * WAVES;
 constexpr int LONG_ROW = 64;
 constexpr int STAGE = 4096;        // items of a workgroup of row_sums at most
-constexpr int AHEAD = 4;           // gradient rows in flight per worker
-constexpr int JOIN_GRID = 256;
+constexpr int AHEAD = 8;           // gradient rows in flight per worker
+constexpr int JOIN_GRID = 128;
 
 template <int DT>
 struct Width {
@@ -345,7 +342,7 @@ __device__ __forceinline__ int64_t merge_place(const uint2* sorted, const int64_
 // any cost nothing.
 constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
 
-template <int DT, int VE, bool FILLED, bool STREAM>
+template <int DT, int VE, bool FILLED, bool STREAM, bool STREAM_G>
 __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t staged[];   // the workgroup's places from place `from` on: their rows, then they
@@ -465,7 +462,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     Vec<DT, VE> ahead[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-        if (i + k < i_stop) ahead[k].load(g + static_cast<int64_t>(places[i + k]) * a.ldg + col);
+        if (i + k < i_stop) ahead[k].template load<STREAM_G>(g + static_cast<int64_t>(places[i + k]) * a.ldg + col);
     while (i < i_stop) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
@@ -479,7 +476,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
             }
 #pragma unroll
             for (int j = 0; j < VE; ++j) acc[j] += ahead[k].get(j);
-            if (i + k + AHEAD < i_stop) ahead[k].load(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
+            if (i + k + AHEAD < i_stop) ahead[k].template load<STREAM_G>(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
         }
         i += AHEAD;
     }
@@ -495,15 +492,18 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     }
 }
 
-// Long rows: slice blockIdx.y of 64 columns, a lane per column; the waves take a quarter of the pieces each.
-template <int DT>
-__global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a, const bool filled) {
+// Long rows: slice blockIdx.y of 64 columns, VE (four, or one where a row has fewer) columns to a lane.  The pieces of a
+// row are dealt to the groups of 16 lanes, which have JOIN_AHEAD of them in flight; the groups' sums meet in their order.
+constexpr int JOIN_WAVES = 8, JOIN_GROUPS = JOIN_WAVES * 4, JOIN_AHEAD = 8;
+
+template <int DT, int VE>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a, const bool filled) {
     typedef typename Elem<DT>::type T;
-    __shared__ double sum[WAVES][64];
+    __shared__ double sum[JOIN_GROUPS][64];
     __shared__ int64_t start;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = blockIdx.y * 64 + lane;
     const uint32_t count = a.long_rows[0];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 4;
+    const int base = blockIdx.y * 64, unit = base + (lane & 15) * VE, col = max(min(unit, a.dim - VE), 0);
     for (uint32_t k = blockIdx.x; k < count; k += gridDim.x) {
         const int64_t row = a.long_rows[1 + 2 * k], last = a.long_rows[2 + 2 * k];
         if (wave == 0) {                                 // the row's first place, and with it the worker that began the row
@@ -519,22 +519,35 @@ __global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a, const bool 
         }
         __syncthreads();
         const int64_t first = (filled ? start : row + start) / a.per;
-        const int64_t pieces = last - first + 1, each = (pieces + WAVES - 1) / WAVES;
-        const int64_t lo = min(wave * each, pieces), hi = min(lo + each, pieces);
-        double s = 0.0;
-        if (col < a.dim) {
-            const float* part = a.part + 2 * first * a.dim + col;
-            if (wave == 0) s = part[a.dim];              // the first worker's piece begins the row: its second slot
-#pragma unroll 8
-            for (int64_t p = max(lo, static_cast<int64_t>(1)); p < hi; ++p) s += part[2 * p * a.dim];
-        }
-        sum[wave][lane] = s;
-        __syncthreads();
-        if (wave == 0 && col < a.dim) {
-            s = sum[0][lane];
+        const int64_t pieces = last - first + 1;
+        // the first worker's piece begins the row: its second slot
+        const float* part = a.part + 2 * first * a.dim + col;
+        double s[VE] = {};
+        if (unit < a.dim) {
+            for (int64_t p0 = group; p0 < pieces; p0 += JOIN_GROUPS * JOIN_AHEAD) {
+                Vec<SPARC_F32, VE> v[JOIN_AHEAD];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) s += sum[w][lane];
-            static_cast<T*>(a.out)[row * a.dim + col] = Elem<DT>::down(static_cast<float>(s) * a.scale);
+                for (int j = 0; j < JOIN_AHEAD; ++j) {
+                    const int64_t p = p0 + j * JOIN_GROUPS;
+                    if (p < pieces) v[j].load(part + (2 * p + (p == 0 ? 1 : 0)) * a.dim);
+                }
+#pragma unroll
+                for (int j = 0; j < JOIN_AHEAD; ++j)
+                    if (p0 + j * JOIN_GROUPS < pieces)
+#pragma unroll
+                        for (int c = 0; c < VE; ++c) s[c] += v[j].get(c);
+            }
+#pragma unroll
+            for (int c = 0; c < VE; ++c)
+                if (col + c >= base) sum[group][col + c - base] = s[c];
+        }
+        __syncthreads();
+        const int mine = base + threadIdx.x;
+        if (threadIdx.x < 64 && mine < a.dim && (VE > 1 || threadIdx.x < 16)) {
+            double all = 0.0;
+#pragma unroll
+            for (int w = 0; w < JOIN_GROUPS; ++w) all += sum[w][threadIdx.x];
+            static_cast<T*>(a.out)[row * a.dim + mine] = Elem<DT>::down(static_cast<float>(all) * a.scale);
         }
         __syncthreads();
     }
@@ -546,7 +559,9 @@ __global__ __launch_bounds__(BLOCK) void join_rows(const GradArgs a, const bool 
 // collects the places of its rows as keys {row, place} (in any order), sorts the keys and adds up the runs.  No workspace,
 // one launch instead of six dependent ones.
 constexpr int FEW = 16384, PLACE_BITS = 14;
-constexpr int FEW_BLOCKS = 1024;   // rows are dealt to at most about that many workgroups
+constexpr int64_t FEW_BYTES = 4 << 20;   // of gradient: one workgroup adds it up alone where all tokens are the same
+constexpr int FEW_THREADS = 512;
+constexpr int FEW_BLOCKS = 512;   // rows are dealt to at most about that many workgroups
 constexpr int FEW_AHEAD = 8;       // gradient rows in flight per worker
 constexpr int FEW_TURNS = 4;       // 16-byte vectors of tokens in flight per thread
 
@@ -556,11 +571,11 @@ __device__ __forceinline__ void collect_rows(const ID* ids, const int n, const i
     constexpr int VE = 16 / sizeof(ID);
     typedef ID mem __attribute__((ext_vector_type(VE), aligned(sizeof(ID))));
     const int lane = threadIdx.x & 63;
-    for (int i0 = 0; i0 < n; i0 += BLOCK * VE * FEW_TURNS) {
+    for (int i0 = 0; i0 < n; i0 += FEW_THREADS * VE * FEW_TURNS) {
         mem v[FEW_TURNS];
 #pragma unroll
         for (int k = 0; k < FEW_TURNS; ++k) {
-            const int i = i0 + (k * BLOCK + static_cast<int>(threadIdx.x)) * VE;
+            const int i = i0 + (k * FEW_THREADS + static_cast<int>(threadIdx.x)) * VE;
             if (i + VE <= n) {
                 v[k] = *reinterpret_cast<const mem*>(ids + i);
             } else {
@@ -580,7 +595,7 @@ __device__ __forceinline__ void collect_rows(const ID* ids, const int n, const i
                 if (lane == 0) at = atomicAdd(count, static_cast<uint32_t>(__popcll(hits)));
                 at = __builtin_amdgcn_readfirstlane(at);
                 if (hit) {
-                    const int i = i0 + (k * BLOCK + static_cast<int>(threadIdx.x)) * VE + c;
+                    const int i = i0 + (k * FEW_THREADS + static_cast<int>(threadIdx.x)) * VE + c;
                     keys[at + __popcll(hits & ((1ull << lane) - 1ull))] = static_cast<uint32_t>(id - row0) << PLACE_BITS | static_cast<uint32_t>(i);
                 }
             }
@@ -588,11 +603,11 @@ __device__ __forceinline__ void collect_rows(const ID* ids, const int n, const i
 }
 
 template <int DT, int VE>
-__global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int lanes_log2) {
+__global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t keys[];     // a power of two of them, at least n
     __shared__ uint32_t total_found;
-    __shared__ float piece[BLOCK * VE];
+    __shared__ float piece[FEW_THREADS * VE];
     __shared__ uint32_t long_runs[FEW / LONG_ROW], n_long;
     const T* g = static_cast<const T*>(a.g);
     T* out = static_cast<T*>(a.out);
@@ -601,7 +616,7 @@ __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int 
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.per;
     const int in_block = static_cast<int>(min(static_cast<int64_t>(a.per), a.rows - row0));
     if (tid == 0) n_long = total_found = 0;
-    const int lanes = 1 << lanes_log2, workers = BLOCK >> lanes_log2, worker = tid >> lanes_log2;
+    const int lanes = 1 << lanes_log2, workers = FEW_THREADS >> lanes_log2, worker = tid >> lanes_log2;
     const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + (tid & (lanes - 1));
     const bool mine = unit * VE < a.dim;
     const int col = mine ? min(unit * VE, a.dim - VE) : 0;
@@ -611,7 +626,7 @@ __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int 
     if (gridDim.y == 1) {
         T* block = out + row0 * a.dim;                   // the rows are one stretch of memory
         const int64_t len = static_cast<int64_t>(in_block) * a.dim;
-        for (int64_t e = static_cast<int64_t>(tid) * VE; e < len; e += BLOCK * VE) zero.store(block + min(e, len - VE));
+        for (int64_t e = static_cast<int64_t>(tid) * VE; e < len; e += FEW_THREADS * VE) zero.store(block + min(e, len - VE));
     } else if (mine) {
         for (int r = worker; r < in_block; r += workers) zero.store(out + (row0 + r) * a.dim + col);
     }
@@ -623,11 +638,11 @@ __global__ __launch_bounds__(BLOCK) void few_tokens(const GradArgs a, const int 
     if (count == 0) return;                              // (the whole workgroup)
     int size = 1;
     while (size < count) size <<= 1;
-    for (int i = count + tid; i < size; i += BLOCK) keys[i] = 0xffffffffu;
+    for (int i = count + tid; i < size; i += FEW_THREADS) keys[i] = 0xffffffffu;
     __syncthreads();
     for (int k = 2; k <= size; k <<= 1)                  // bitonic: the keys are distinct, so this is the order of the places
         for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = tid; i < size / 2; i += BLOCK) {
+            for (int i = tid; i < size / 2; i += FEW_THREADS) {
                 const int x = ((i & ~(j - 1)) << 1) | (i & (j - 1)), y = x | j;
                 const uint32_t p = keys[x], q = keys[y];
                 if ((p > q) == ((x & k) == 0)) {
@@ -730,11 +745,12 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     p.lanes_log2 = lanes_for((dim + ve - 1) / ve, &p.slices);
     p.in_group = BLOCK >> p.lanes_log2;
     // zeros beside the sort where most rows have no token: they are written twice where they have one
-    p.filled = rows >= V_FILL * n;
+    p.filled = rows >= 4 * n;
     // items of a worker: enough workers for every SIMD's wave slots first, up to 64 items then
     const int64_t items = p.filled ? n : n + rows;
     const int64_t wanted = ceil_div(items, static_cast<int64_t>(8192) * 64 >> p.lanes_log2);
-    p.per = static_cast<int>(wanted < 4 ? 4 : wanted > 64 ? 64 : wanted);
+    const int least = p.filled ? 8 : 4;
+    p.per = static_cast<int>(wanted < least ? least : wanted > 64 ? 64 : wanted);
     if (static_cast<int64_t>(p.per) * p.in_group > STAGE) p.per = STAGE / p.in_group;
     p.workers = ceil_div(items, p.per);
     return p;
@@ -777,6 +793,10 @@ GradArgs carve(const Plan& p, const int64_t n, const int dim, void* ws, const si
     return a;
 }
 
+bool few_enough(const int64_t n, const int64_t dim, const int dtype) {
+    return n <= FEW && n * dim * (dtype == SPARC_F32 ? 4 : 2) <= FEW_BYTES;
+}
+
 int elements_of_16_bytes(const int dtype) { return dtype == SPARC_F32 ? 4 : 8; }
 
 }  // namespace
@@ -805,7 +825,7 @@ extern "C" size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, 
     if (n < 0 || rows < 0 || dim < 0 || n > SPARC_EMBEDDING_MAX || rows > SPARC_EMBEDDING_MAX || dim > SPARC_EMBEDDING_MAX_DIM ||
         dtype < SPARC_F32 || dtype > SPARC_F16)
         return 0;
-    if (n <= FEW) return 0;
+    if (few_enough(n, dim, dtype)) return 0;
     const int ve = elements_of_16_bytes(dtype);
     const Plan p = plan_of(n, rows, static_cast<int>(dim), dim >= ve ? ve : 1);
     bool ok;
@@ -820,8 +840,10 @@ template <int DT, int VE, bool FILLED>
 int launch_sums(const GradArgs& a, const Plan& p, const bool streaming, sparc_stream_t stream) {
     const dim3 grid(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), static_cast<unsigned>(p.slices));
     const size_t lds = static_cast<size_t>(p.per * p.in_group + 2 * MARGIN) * 2 * sizeof(uint32_t);
-    if (streaming) hipLaunchKernelGGL((row_sums<DT, VE, FILLED, true>), grid, dim3(BLOCK), lds, stream, a, p.lanes_log2);
-    else hipLaunchKernelGGL((row_sums<DT, VE, FILLED, false>), grid, dim3(BLOCK), lds, stream, a, p.lanes_log2);
+    const bool streaming_g = a.n * a.ldg * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > SPARC_KEEP_BYTES;
+    auto sums = streaming ? (streaming_g ? row_sums<DT, VE, FILLED, true, true> : row_sums<DT, VE, FILLED, true, false>)
+                          : (streaming_g ? row_sums<DT, VE, FILLED, false, true> : row_sums<DT, VE, FILLED, false, false>);
+    hipLaunchKernelGGL(sums, grid, dim3(BLOCK), lds, stream, a, p.lanes_log2);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
@@ -856,7 +878,9 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
     }
     const int rc = p.filled ? launch_sums<DT, VE, true>(a, p, false, stream) : launch_sums<DT, VE, false>(a, p, streaming, stream);
     if (rc != SPARC_OK) return rc;
-    hipLaunchKernelGGL((join_rows<DT>), dim3(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64)), dim3(BLOCK), 0, stream, a, p.filled);
+    const dim3 joining(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64));
+    if (a.dim >= 4) hipLaunchKernelGGL((join_rows<DT, 4>), joining, dim3(64 * JOIN_WAVES), 0, stream, a, p.filled);
+    else hipLaunchKernelGGL((join_rows<DT, 1>), joining, dim3(64 * JOIN_WAVES), 0, stream, a, p.filled);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
@@ -865,7 +889,7 @@ template <int DT, int VE>
 int launch_few(const GradArgs& a, const int lanes_log2, const int slices, sparc_stream_t stream) {
     size_t keys = 1;
     while (keys < static_cast<size_t>(a.n)) keys <<= 1;
-    hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(static_cast<unsigned>(ceil_div(a.rows, a.per)), static_cast<unsigned>(slices)), dim3(BLOCK),
+    hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(static_cast<unsigned>(ceil_div(a.rows, a.per)), static_cast<unsigned>(slices)), dim3(FEW_THREADS),
                        keys * sizeof(uint32_t), stream, a, lanes_log2);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
@@ -883,7 +907,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
     const int ve = elements_of_16_bytes(dtype), used_ve = dim >= ve ? ve : 1;
     GradArgs a = {};
     Plan p = {};
-    const bool few = n <= FEW;
+    const bool few = few_enough(n, dim, dtype);
     if (few) {
         p.lanes_log2 = lanes_for(ceil_div(dim, used_ve), &p.slices);
         int64_t per = ceil_div(rows, FEW_BLOCKS);
