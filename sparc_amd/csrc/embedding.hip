@@ -31,7 +31,7 @@ constexpr int BLOCK = 64 * WAVES;
 constexpr int LONG_ROW = 64;
 constexpr int STAGE = 4096;        // items of a workgroup of row_sums at most
 constexpr int AHEAD = 8;           // gradient rows in flight per worker
-constexpr int JOIN_GRID = 128;
+constexpr int JOIN_GRID = 256;
 
 template <int DT>
 struct Width {
@@ -113,6 +113,7 @@ struct GradArgs {
     uint2* other;              // [n] the same, between passes
     uint32_t* kept;            // one word: tokens that are rows and not padding
     uint32_t* long_rows;       // [1 + 2 * most]: count, then {row, last worker}
+    uint32_t* begins;          // [workers]: 1 where a worker begins the long row that goes on in the next, 0 where it is inside
     float* part;               // [2 workers][dim]
 };
 
@@ -486,6 +487,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
         while (r < r_stop) finish_row();
     }
     if (goes_on) {
+        if (u == 0 && blockIdx.y == 0) a.begins[worker] = inside ? 0u : 1u;
         float* p = a.part + (2 * worker + (inside ? 0 : 1)) * a.dim + col;
 #pragma unroll
         for (int k = 0; k < VE; ++k) p[k] = acc[k];
@@ -494,31 +496,37 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
 
 // Long rows: slice blockIdx.y of 64 columns, VE (four, or one where a row has fewer) columns to a lane.  The pieces of a
 // row are dealt to the groups of 16 lanes, which have JOIN_AHEAD of them in flight; the groups' sums meet in their order.
-constexpr int JOIN_WAVES = 8, JOIN_GROUPS = JOIN_WAVES * 4, JOIN_AHEAD = 8;
+constexpr int JOIN_WAVES = 4, JOIN_GROUPS = JOIN_WAVES * 4, JOIN_AHEAD = 8;
 
 template <int DT, int VE>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a, const bool filled) {
     typedef typename Elem<DT>::type T;
     __shared__ double sum[JOIN_GROUPS][64];
-    __shared__ int64_t start;
+    __shared__ int64_t begun;
     const uint32_t count = a.long_rows[0];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 4;
     const int base = blockIdx.y * 64, unit = base + (lane & 15) * VE, col = max(min(unit, a.dim - VE), 0);
     for (uint32_t k = blockIdx.x; k < count; k += gridDim.x) {
         const int64_t row = a.long_rows[1 + 2 * k], last = a.long_rows[2 + 2 * k];
-        if (wave == 0) {                                 // the row's first place, and with it the worker that began the row
-            int64_t lo = 0, hi = *a.kept;
-            while (hi > lo) {
-                const int64_t width = (hi - lo + 63) >> 6, e = lo + lane * width;
-                const int before = __popcll(__ballot(e < hi && a.sorted[e].x < row));
-                if (before == 0) break;
-                hi = min(hi, lo + before * width);
-                lo += (before - 1) * width + 1;
+        if (wave == 0) {                                 // the worker that began the row: near by, or found by the row's first place
+            const int64_t before = last - 1 - lane;
+            const uint64_t found = __ballot(before >= 0 && a.begins[max(before, static_cast<int64_t>(0))] == 1u);
+            int64_t worker = last - __ffsll(static_cast<unsigned long long>(found));
+            if (found == 0) {
+                int64_t lo = 0, hi = *a.kept;
+                while (hi > lo) {
+                    const int64_t width = (hi - lo + 63) >> 6, e = lo + lane * width;
+                    const int smaller = __popcll(__ballot(e < hi && a.sorted[e].x < row));
+                    if (smaller == 0) break;
+                    hi = min(hi, lo + smaller * width);
+                    lo += (smaller - 1) * width + 1;
+                }
+                worker = (filled ? lo : row + lo) / a.per;
             }
-            if (lane == 0) start = lo;
+            if (lane == 0) begun = worker;
         }
         __syncthreads();
-        const int64_t first = (filled ? start : row + start) / a.per;
+        const int64_t first = begun;
         const int64_t pieces = last - first + 1;
         // the first worker's piece begins the row: its second slot
         const float* part = a.part + 2 * first * a.dim + col;
@@ -660,7 +668,7 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
             Vec<DT, VE> v[FEW_AHEAD];
 #pragma unroll
             for (int k = 0; k < FEW_AHEAD; ++k)
-                if (i + k < to) v[k].load(g + static_cast<int64_t>(keys[i + k] & (FEW - 1)) * a.ldg + col);
+                if (i + k < to) v[k].load(g + static_cast<int64_t>(keys[i + k] & ((1 << PLACE_BITS) - 1)) * a.ldg + col);
 #pragma unroll
             for (int k = 0; k < FEW_AHEAD; ++k)
                 if (i + k < to)
@@ -787,6 +795,7 @@ GradArgs carve(const Plan& p, const int64_t n, const int dim, void* ws, const si
     a.other = c.take<uint2>(p.passes > 1 ? n : 0);
     a.kept = c.take<uint32_t>(1);
     a.long_rows = c.take<uint32_t>(1 + 2 * (n / LONG_ROW + 1));
+    a.begins = c.take<uint32_t>(p.workers);
     a.part = c.take<float>(static_cast<size_t>(2) * p.workers * dim);
     *ok = c.ok();
     *used = c.off;
