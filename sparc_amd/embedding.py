@@ -29,9 +29,12 @@ def _rows_of(t: torch.Tensor, what: str) -> int:
     """Row stride of a matrix whose rows are contiguous."""
     if t.dtype not in DTYPES:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"{what} must be a matrix with contiguous rows that do not overlap")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    if t.dim() == 2:
+        rows, dim = t.shape
+        ld, step = t.stride()
+        if (ld >= dim or rows <= 1) and (step == 1 or dim <= 1):
+            return ld if ld > dim else max(dim, 1)
+    raise ValueError(f"{what} must be a matrix with contiguous rows that do not overlap")
 
 
 def _padding(padding_idx, rows: int) -> int:

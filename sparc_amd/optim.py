@@ -28,16 +28,24 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-_type_of, _is_sparse = operator.attrgetter("dtype"), operator.attrgetter("is_sparse")
+_type_of = operator.attrgetter("dtype")
 _device_of, _address_of, _size_of = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
 _is_contiguous = torch.Tensor.is_contiguous
+
+
+def _dense_on(tensors, device, dense=None) -> bool:
+    """All on the device, and contiguous or, with dense, at least passing it."""
+    try:
+        ok = set(map(_device_of, tensors)) == {device.index}
+        return ok and (all(map(_is_contiguous, tensors)) or (dense is not None and all(map(dense, tensors))))
+    except RuntimeError:   # a sparse tensor has no strides to ask for
+        return False
 
 
 def _grad_records(grads, device):
     """The list as the C calls take it (an array of {address, elements, type}: keep it while they run)."""
     types = list(map(_type_of, grads))
-    if any(map(_is_sparse, grads)) or set(map(_device_of, grads)) != {device.index} or not DTYPES.keys() >= set(types) \
-            or not (all(map(_is_contiguous, grads)) or all(map(_dense, grads))):
+    if not _dense_on(grads, device, _dense) or not DTYPES.keys() >= set(types):
         raise ValueError("the gradients of one norm are dense float32, bfloat16 or float16 tensors on one device")
     return _records(list(map(_address_of, grads)), list(map(_size_of, grads)), [DTYPES[t] for t in types])
 
@@ -99,8 +107,7 @@ def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
     n = len(params)
     every = [*params, *grads, *exp_avgs, *exp_avg_sqs]
     sizes = list(map(_size_of, every))
-    if set(map(_type_of, every)) != {torch.float32} or any(map(_is_sparse, every)) or set(map(_device_of, every)) != {device.index} \
-            or not all(map(_is_contiguous, every)) or sizes != sizes[:n] * 4:
+    if set(map(_type_of, every)) != {torch.float32} or not _dense_on(every, device) or sizes != sizes[:n] * 4:
         raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
     at = list(map(_address_of, every))
     return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), _records(at[n:2 * n], sizes[:n], [0] * n)

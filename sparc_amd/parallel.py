@@ -209,8 +209,6 @@ class ShardedSpectralTrainer:
         else:
             self.optimizer = torch.optim.Adam(self.net.parameters(), lr=lr)
         self.max_grad_norm = max_grad_norm
-        # (the package's Adam clips on the way into its update; torch's is handed clipped gradients)
-        self.clip_first = max_grad_norm is not None and "max_grad_norm" not in self.optimizer.defaults
         self._graphed = None
         self.criterion = criterion
         self.reducer = None
@@ -252,7 +250,8 @@ class ShardedSpectralTrainer:
         loss.backward(gradient=LapLoss.unit_gradient(loss))
         if self.distributed:
             reduce_gradients(net, self.reducer, self.group)
-        if self.clip_first:
+        if self.max_grad_norm is not None and "max_grad_norm" not in self.optimizer.defaults:
+            # (the package's Adam clips on the way into its update; another optimiser is handed clipped gradients)
             from .optim import clip_grad_norm_
             clip_grad_norm_(self.params, self.max_grad_norm)
         self.optimizer.step()
