@@ -22,9 +22,9 @@ namespace {
 
 constexpr int SORT_WAVES = 8;
 constexpr int SORT_BLOCK = 64 * SORT_WAVES;
-constexpr int UP_FRONT = 8;                    // tokens a lane of a sorting workgroup holds
+constexpr int UP_FRONT = 4;                    // tokens a lane of a sorting workgroup holds
 constexpr int CHUNK = SORT_BLOCK * UP_FRONT;   // tokens a sorting workgroup ranks at once
-constexpr int MOST_TILES = 128;                // every tile reads all tiles' counts
+constexpr int MOST_TILES = 256;                // every tile reads all tiles' counts
 constexpr int MOST_BITS = 11;                  // of a digit
 constexpr int WAVES = 4;
 constexpr int BLOCK = 64 * WAVES;

@@ -69,14 +69,14 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
         require_gpu(dev)
     ids = _tokens(ids, dev)
     rows = int(rows)
-    if rows < 0 or grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
+    if rows < 0 or grad.shape[:-1] != ids.shape or grad.dim() == 0:
         raise ValueError(f"a gradient of shape {tuple(grad.shape)} does not belong to ids of shape {tuple(ids.shape)}")
     dim = grad.shape[-1]
-    g = grad.detach().reshape(ids.numel(), dim)
+    g = grad if grad.dim() == 2 else grad.reshape(ids.numel(), dim)
     if (dim > 1 and g.stride(1) != 1) or (g.shape[0] > 1 and g.stride(0) < dim):   # an expanded gradient
         g = g.contiguous()
     ld = _rows_of(g, "grad")
-    pad = _padding(padding_idx, rows)
+    pad = -1 if padding_idx is None else _padding(padding_idx, rows)
     out = g.new_empty((rows, dim))
     if rows and dim:
         n, code = ids.numel(), DTYPES[g.dtype]

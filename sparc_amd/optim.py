@@ -113,7 +113,6 @@ def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
     return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), _records(at[n:2 * n], sizes[:n], [0] * n)
 
 
-@torch.no_grad()
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 0.0, max_grad_norm=None):
     """Update number `step` (from 1) of torch.optim.Adam on lists of tensors, in place: params, exp_avgs and exp_avg_sqs.
