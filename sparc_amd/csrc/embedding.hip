@@ -7,11 +7,11 @@
 //   digit_counts, digit_scatter   a stable radix sort of the tokens, one or more digits of the row number: a workgroup per
 //                  tile of tokens counts the tile's digits, then ranks its tokens (ballots inside a wave, counters in LDS
 //                  between waves, the other tiles' counts before it) and scatters {row, place}.  However often one
-//                  token occurs, every tile is the same work;
-//   row_sums       adds up.  Work is cut along the merged list of (places of row 0, row 0 done, places of row 1, ...) so that
-//                  a worker has `per` items whatever the rows hold: long rows are cut, empty rows cost the store of their
-//                  zeros and no separate fill.  A row of at most LONG_ROW places belongs to the worker that meets its
-//                  first; a longer one leaves one partial sum per worker,
+//                  token occurs, every tile is the same work.  The sort waits on latency and leaves the memory idle, so
+//                  further workgroups of its launches write the table's zeros meanwhile;
+//   row_sums       adds up, over the zeros.  A worker has `per` sorted places whatever the rows hold; a row of at most
+//                  LONG_ROW places belongs to the worker that meets its first, a longer one is cut and leaves one partial
+//                  sum per worker,
 //   join_rows      which are added in order (float64) here.  Usually nothing to do.
 // Few tokens take one launch instead (few_tokens).
 #include <type_traits>
@@ -29,14 +29,9 @@ constexpr int MOST_BITS = 11;                  // of a digit
 constexpr int WAVES = 4;
 constexpr int BLOCK = 64 * WAVES;
 constexpr int LONG_ROW = 64;
-constexpr int STAGE = 4096;        // items of a workgroup of row_sums at most
+constexpr int STAGE = 4096;        // places of a workgroup of row_sums at most
 constexpr int AHEAD = 8;           // gradient rows in flight per worker
 constexpr int JOIN_GRID = 256;
-
-template <int DT>
-struct Width {
-    static constexpr int VE = 16 / sizeof(typename Elem<DT>::type);
-};
 
 // ---- lookup ------------------------------------------------------------------------------------------------
 
@@ -106,7 +101,7 @@ struct GradArgs {
     int64_t tile;              // tokens of a tile, a multiple of CHUNK
     int tiles;
     int dim, wide_ids;
-    int per;                   // items of a worker
+    int per;                   // places of a worker (few_tokens: rows of a workgroup)
     float scale;
     uint32_t* counts;          // [tiles][1 << bits]: digits of a tile
     uint2* sorted;             // [n] {row, place}; the last pass leaves the result here
@@ -131,8 +126,7 @@ __device__ __forceinline__ uint64_t equals(const uint32_t key, const int bits, c
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-// Zeros that a launch of the sort writes with workgroups of its own behind the sorting ones: the sort waits on memory
-// latency and leaves the bandwidth idle.
+// Zeros that a launch of the sort writes with workgroups of its own behind the sorting ones.
 struct Zeros {
     uint16_t* p;
     int64_t count;         // of uint16
@@ -321,124 +315,63 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
     }
 }
 
-// Places before item `diag` of the merged list: place e is its item e + row of e (the rows before that one have ended).
-__device__ __forceinline__ int64_t merge_place(const uint2* sorted, const int64_t places, const int64_t rows, const int64_t diag) {
-    int64_t lo = max(static_cast<int64_t>(0), diag - rows), hi = min(places, diag);   // the answer is in [lo, hi]
-    const int lane = threadIdx.x & 63;
-    while (hi > lo) {                                                                  // 64 probes at a time
-        const int64_t width = (hi - lo + 63) >> 6;
-        const int64_t e = lo + lane * width;
-        const bool before = e < hi && static_cast<int64_t>(sorted[e].x) + e < diag;
-        const int k = __popcll(__ballot(before));   // probes 0 .. k - 1 are before: the answer lies behind probe k - 1
-        if (k == 0) return lo;
-        const int64_t new_lo = lo + (k - 1) * width + 1;
-        hi = min(hi, lo + k * width);
-        lo = new_lo;
-    }
-    return lo;
-}
-
 // Workers are groups of `lanes` lanes (a power of two); lane u of a group owns VE columns of the slice blockIdx.y.
-// FILLED: the table holds zeros already (written beside the sort) and a worker's items are places alone, the rows without
-// any cost nothing.
+// STREAM: a gradient that is read once and outgrows the Infinity Cache goes by it.
 constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
 
-template <int DT, int VE, bool FILLED, bool STREAM, bool STREAM_G>
+template <int DT, int VE, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t staged[];   // the workgroup's places from place `from` on: their rows, then they
-    __shared__ int64_t edge[2];
     const T* g = static_cast<const T*>(a.g);
     T* out = static_cast<T*>(a.out);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int lanes = 1 << lanes_log2, in_group = BLOCK >> lanes_log2;
-    const int u = tid & (lanes - 1);
-    uint32_t *rows_of = staged, *places = staged + (in_group * a.per + 2 * MARGIN);
-    const int64_t first_worker = static_cast<int64_t>(blockIdx.x) * in_group;
-    const int64_t all_places = *a.kept;
-    const int64_t items = FILLED ? all_places : all_places + a.rows;
-    const int64_t d0 = min(first_worker * a.per, items), d1 = min(d0 + static_cast<int64_t>(in_group) * a.per, items);
-    if (d0 >= d1) return;                                // (the whole workgroup)
-    int64_t e_first = d0, e_last = d1;
-    if constexpr (!FILLED) {
-        if (wave < 2) {
-            const int64_t e = merge_place(a.sorted, all_places, a.rows, wave ? d1 : d0);
-            if (lane == 0) edge[wave] = e;
-        }
-        __syncthreads();
-        e_first = edge[0];
-        e_last = edge[1];
-    }
-    const int64_t from = max(e_first - MARGIN, static_cast<int64_t>(0)), to = min(e_last + MARGIN, all_places);
+    const int tid = threadIdx.x;
+    const int lanes = 1 << lanes_log2, in_group = BLOCK >> lanes_log2, u = tid & (lanes - 1);
+    uint32_t *row_of = staged, *places = staged + (in_group * a.per + 2 * MARGIN);
+    const int64_t all = *a.kept;
+    const int64_t e0 = min(static_cast<int64_t>(blockIdx.x) * in_group * a.per, all), e1 = min(e0 + in_group * a.per, all);
+    if (e0 >= e1) return;                                // (the whole workgroup)
+    const int64_t from = max(e0 - MARGIN, static_cast<int64_t>(0)), to = min(e1 + MARGIN, all);
     for (int64_t k = from + tid; k < to; k += BLOCK) {
         const uint2 s = a.sorted[k];
-        rows_of[k - from] = s.x;
+        row_of[k - from] = s.x;
         places[k - from] = s.y;
     }
     __syncthreads();
-    const int64_t worker = first_worker + (tid >> lanes_log2);
-    const int64_t w0 = min(worker * a.per, items), w1 = min(w0 + a.per, items);
-    const int col = min((static_cast<int>(blockIdx.y) * lanes + u) * VE, a.dim - VE);
-    if (w0 >= w1 || (static_cast<int>(blockIdx.y) * lanes + u) * VE >= a.dim) return;   // no barrier below
-    // from here on: places relative to `from`, rows relative to row0
-    const int64_t row0 = FILLED ? 0 : d0 - e_first;
-    const int n_staged = static_cast<int>(to - from), i_first = static_cast<int>(e_first - from), i_last = static_cast<int>(e_last - from);
-    auto row_at = [&](const int i) { return static_cast<int>(rows_of[i] - row0); };
-    auto split = [&](const int64_t d) {                  // the first place at or behind item d
-        if constexpr (FILLED) return i_first + static_cast<int>(d - d0);
-        int lo = i_first, hi = min(i_last, i_first + static_cast<int>(d - d0));
-        const int64_t limit = d - d0 + i_first;          // item of place i: d0 + i - i_first + row_at(i)
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (mid + static_cast<int64_t>(row_at(mid)) < limit) lo = mid + 1;
-            else hi = mid;
-        }
-        return lo;
-    };
-    // Is row r, met at place i, begun before i?  0: no, -1: yes, and longer than LONG_ROW, otherwise its end (> 0)
-    auto cut = [&](const int i, const int r) {
-        if (i == 0 || row_at(i - 1) != r) return 0;      // (i is only 0 where no place lies before)
+    const int64_t worker = static_cast<int64_t>(blockIdx.x) * in_group + (tid >> lanes_log2);
+    const int64_t w0 = worker * a.per, w1 = min(w0 + a.per, all);
+    const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + u, col = min(unit * VE, a.dim - VE);
+    if (w0 >= w1 || unit * VE >= a.dim) return;          // no barrier below
+    // from here on: places relative to `from`
+    const int n_staged = static_cast<int>(to - from);
+    // Where does the row that is cut in front of place i end?  0: no row is, -1: it is longer than LONG_ROW, otherwise its end
+    auto cut = [&](const int i) {
+        if (i == 0 || i == n_staged || row_of[i - 1] != row_of[i]) return 0;   // (0 and n_staged only where all places end)
+        const uint32_t r = row_of[i];
         int s_lo = max(i - MARGIN, 0), s_hi = i - 1;     // its first place, as far as MARGIN sees
         while (s_lo < s_hi) {
             const int mid = (s_lo + s_hi) >> 1;
-            if (row_at(mid) < r) s_lo = mid + 1;
+            if (row_of[mid] < r) s_lo = mid + 1;
             else s_hi = mid;
         }
-        int f_lo = i, f_hi = min(i + MARGIN, n_staged);  // behind its last place
+        int f_lo = i + 1, f_hi = min(i + MARGIN, n_staged);   // behind its last place
         while (f_lo < f_hi) {
             const int mid = (f_lo + f_hi) >> 1;
-            if (row_at(mid) <= r) f_lo = mid + 1;
+            if (row_of[mid] <= r) f_lo = mid + 1;
             else f_hi = mid;
         }
         return f_lo - s_lo > LONG_ROW ? -1 : f_lo;
     };
-    int i = split(w0), i_stop = split(w1);
-    // the rows that this worker finishes: r .. r_stop - 1 (FILLED: the row at hand, and the one at the end)
-    int r, r_stop;
-    if constexpr (FILLED) {
-        r = row_at(i);
-        r_stop = i_stop < n_staged ? row_at(i_stop) : -1;
-    } else {
-        r = static_cast<int>(w0 - d0) - (i - i_first);
-        r_stop = static_cast<int>(w1 - d0) - (i_stop - i_first);
-    }
-    int c = cut(i, r);
-    bool inside = c < 0;                                 // the first row is a long one that began in an earlier worker
-    if (c > 0) {                                         // an earlier worker has the whole row
-        i = c;
-        ++r;
-    }
-    c = cut(i_stop, r_stop);
+    int i = static_cast<int>(w0 - from), i_stop = static_cast<int>(w1 - from);
+    int c = cut(i);
+    bool inside = c < 0;                                 // a long row that began in an earlier worker
+    if (c > 0) i = c;                                    // an earlier worker has the whole row
+    c = cut(i_stop);
     const bool goes_on = c < 0;                          // a long row goes on in the next worker
-    if (c > 0) {                                         // the row that is cut here is this worker's
-        i_stop = c;
-        ++r_stop;
-    }
-    if (FILLED ? i >= i_stop : r > r_stop || (r == r_stop && i >= i_stop)) return;
-    if constexpr (FILLED) r = row_at(i);
-    float acc[VE];
-#pragma unroll
-    for (int k = 0; k < VE; ++k) acc[k] = 0.f;
+    if (c > 0) i_stop = c;                               // the row that is cut here is this worker's
+    if (i >= i_stop) return;
+    uint32_t row = row_of[i];
+    float acc[VE] = {};
     auto finish_row = [&]() {
         if (inside) {
             float* p = a.part + (2 * worker) * a.dim + col;
@@ -446,7 +379,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
             for (int k = 0; k < VE; ++k) p[k] = acc[k];
             if (u == 0 && blockIdx.y == 0) {             // the last piece of a long row: announce it
                 const uint32_t at = atomicAdd(a.long_rows, 1u);
-                a.long_rows[1 + 2 * at] = static_cast<uint32_t>(row0 + r);
+                a.long_rows[1 + 2 * at] = row;
                 a.long_rows[2 + 2 * at] = static_cast<uint32_t>(worker);
             }
             inside = false;
@@ -454,39 +387,32 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
             Vec<DT, VE> v;
 #pragma unroll
             for (int k = 0; k < VE; ++k) v.set(k, acc[k] * a.scale);
-            v.template store<STREAM>(out + (row0 + r) * a.dim + col);
+            v.store(out + static_cast<int64_t>(row) * a.dim + col);
         }
 #pragma unroll
         for (int k = 0; k < VE; ++k) acc[k] = 0.f;
-        ++r;
     };
     Vec<DT, VE> ahead[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-        if (i + k < i_stop) ahead[k].template load<STREAM_G>(g + static_cast<int64_t>(places[i + k]) * a.ldg + col);
+        if (i + k < i_stop) ahead[k].template load<STREAM>(g + static_cast<int64_t>(places[i + k]) * a.ldg + col);
     while (i < i_stop) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             if (i + k >= i_stop) break;
-            const int row = row_at(i + k);
-            if constexpr (FILLED) {
-                if (r != row) finish_row();
-                r = row;
-            } else {
-                while (r < row) finish_row();
+            if (row_of[i + k] != row) {
+                finish_row();
+                row = row_of[i + k];
             }
 #pragma unroll
             for (int j = 0; j < VE; ++j) acc[j] += ahead[k].get(j);
-            if (i + k + AHEAD < i_stop) ahead[k].template load<STREAM_G>(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
+            if (i + k + AHEAD < i_stop) ahead[k].template load<STREAM>(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
         }
         i += AHEAD;
     }
-    if constexpr (FILLED) {
-        if (!goes_on) finish_row();
+    if (!goes_on) {
+        finish_row();
     } else {
-        while (r < r_stop) finish_row();
-    }
-    if (goes_on) {
         if (u == 0 && blockIdx.y == 0) a.begins[worker] = inside ? 0u : 1u;
         float* p = a.part + (2 * worker + (inside ? 0 : 1)) * a.dim + col;
 #pragma unroll
@@ -499,7 +425,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
 constexpr int JOIN_WAVES = 4, JOIN_GROUPS = JOIN_WAVES * 4, JOIN_AHEAD = 8;
 
 template <int DT, int VE>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a, const bool filled) {
+__global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
     typedef typename Elem<DT>::type T;
     __shared__ double sum[JOIN_GROUPS][64];
     __shared__ int64_t begun;
@@ -521,7 +447,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a, c
                     hi = min(hi, lo + smaller * width);
                     lo += (smaller - 1) * width + 1;
                 }
-                worker = (filled ? lo : row + lo) / a.per;
+                worker = lo / a.per;
             }
             if (lane == 0) begun = worker;
         }
@@ -727,7 +653,6 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
 struct Plan {
     int64_t tile, workers;
     int tiles, passes, bits, per, lanes_log2, slices, in_group;
-    bool filled;
 };
 
 int64_t ceil_div(const int64_t a, const int64_t b) { return (a + b - 1) / b; }
@@ -752,15 +677,11 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     p.bits = (bits + p.passes - 1) / p.passes;
     p.lanes_log2 = lanes_for((dim + ve - 1) / ve, &p.slices);
     p.in_group = BLOCK >> p.lanes_log2;
-    // zeros beside the sort where most rows have no token: they are written twice where they have one
-    p.filled = rows >= 4 * n;
-    // items of a worker: enough workers for every SIMD's wave slots first, up to 64 items then
-    const int64_t items = p.filled ? n : n + rows;
-    const int64_t wanted = ceil_div(items, static_cast<int64_t>(8192) * 64 >> p.lanes_log2);
-    const int least = p.filled ? 8 : 4;
-    p.per = static_cast<int>(wanted < least ? least : wanted > 64 ? 64 : wanted);
+    // places of a worker: enough workers for every SIMD's wave slots first, up to 64 places then
+    const int64_t wanted = ceil_div(n, static_cast<int64_t>(8192) * 64 >> p.lanes_log2);
+    p.per = static_cast<int>(wanted < 8 ? 8 : wanted > 64 ? 64 : wanted);
     if (static_cast<int64_t>(p.per) * p.in_group > STAGE) p.per = STAGE / p.in_group;
-    p.workers = ceil_div(items, p.per);
+    p.workers = ceil_div(n, p.per);
     return p;
 }
 
@@ -845,25 +766,13 @@ extern "C" size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, 
 
 namespace {
 
-template <int DT, int VE, bool FILLED>
-int launch_sums(const GradArgs& a, const Plan& p, const bool streaming, sparc_stream_t stream) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), static_cast<unsigned>(p.slices));
-    const size_t lds = static_cast<size_t>(p.per * p.in_group + 2 * MARGIN) * 2 * sizeof(uint32_t);
-    const bool streaming_g = a.n * a.ldg * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > SPARC_KEEP_BYTES;
-    auto sums = streaming ? (streaming_g ? row_sums<DT, VE, FILLED, true, true> : row_sums<DT, VE, FILLED, true, false>)
-                          : (streaming_g ? row_sums<DT, VE, FILLED, false, true> : row_sums<DT, VE, FILLED, false, false>);
-    hipLaunchKernelGGL(sums, grid, dim3(BLOCK), lds, stream, a, p.lanes_log2);
-    SPARC_CHECK_LAUNCH();
-    return SPARC_OK;
-}
-
 template <int DT, int VE>
 int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
     const int64_t half_words = a.rows * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) / 2;
     const bool streaming = 2 * half_words > SPARC_KEEP_BYTES;
     const size_t lds = (static_cast<size_t>(1) << p.bits) * (2 * sizeof(uint32_t) + SORT_WAVES * sizeof(uint16_t));
     // the zeros are dealt to the launches of the sort
-    const int64_t chunks = p.filled ? ceil_div(half_words, ZERO_CHUNK) : 0, each = ceil_div(chunks, 2 * p.passes);
+    const int64_t chunks = ceil_div(half_words, ZERO_CHUNK), each = ceil_div(chunks, 2 * p.passes);
     int64_t dealt = 0;
     Zeros z = {};
     auto grid = [&]() {
@@ -885,11 +794,15 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
         SPARC_CHECK_LAUNCH();
         in = out;
     }
-    const int rc = p.filled ? launch_sums<DT, VE, true>(a, p, false, stream) : launch_sums<DT, VE, false>(a, p, streaming, stream);
-    if (rc != SPARC_OK) return rc;
+    const size_t staged = static_cast<size_t>(p.per * p.in_group + 2 * MARGIN) * 2 * sizeof(uint32_t);
+    const bool once = a.n * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > SPARC_KEEP_BYTES;
+    hipLaunchKernelGGL((once ? row_sums<DT, VE, true> : row_sums<DT, VE, false>),
+                       dim3(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), static_cast<unsigned>(p.slices)), dim3(BLOCK), staged, stream,
+                       a, p.lanes_log2);
+    SPARC_CHECK_LAUNCH();
     const dim3 joining(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64));
-    if (a.dim >= 4) hipLaunchKernelGGL((join_rows<DT, 4>), joining, dim3(64 * JOIN_WAVES), 0, stream, a, p.filled);
-    else hipLaunchKernelGGL((join_rows<DT, 1>), joining, dim3(64 * JOIN_WAVES), 0, stream, a, p.filled);
+    if (a.dim >= 4) hipLaunchKernelGGL((join_rows<DT, 4>), joining, dim3(64 * JOIN_WAVES), 0, stream, a);
+    else hipLaunchKernelGGL((join_rows<DT, 1>), joining, dim3(64 * JOIN_WAVES), 0, stream, a);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }

@@ -52,7 +52,7 @@ def check_clip(grads, max_norm):
 @pytest.mark.parametrize("sizes,dtypes", [
     ([1], [F32]), ([3, 0, 5], [F32]), ([4096], [F32]), ([4097, 1, 8191, 0], [F32, BF16, F16, F32]),
     ([10 * 1024, 1024, 1024 * 1024, 1024, 512 * 1024, 512, 47 * 512, 47], [F32]), ([100003], [BF16]), ([65537, 8192], [F16]),
-    ([0], [F32]), ([7] * 300, [F32, BF16]), (list(range(1, 129)), [F16]), ([33333] * 129, [F32]), ([5_000_011], [F32, BF16])])
+    ([0], [F32]), ([7] * 300, [F32, BF16]), ([60_000_001], [F32]), ([500_003] * 130, [F32]), ([3, 130_000_000, 9], [BF16]), (list(range(1, 129)), [F16]), ([33333] * 129, [F32]), ([5_000_011], [F32, BF16])])
 def test_clip(sizes, dtypes):
     for max_norm in (0.5, 1e9):
         grads = [(torch.randn(s, device="cuda", generator=gen(i)) * 2.0 ** (i % 5)).to(dtypes[i % len(dtypes)]) for i, s in enumerate(sizes)]
@@ -131,7 +131,7 @@ def adam_bounds(p0, g, m0, v0, coef, step, lr, b1, b2, eps, wd):
     return (p0 - move, m, v), (dp, dm, dv)
 
 
-@pytest.mark.parametrize("sizes", [[1], [1000, 0, 3], [5, 1023, 1024, 1025, 300001], [47] * 60, [2_000_003]])
+@pytest.mark.parametrize("sizes", [[1], [1000, 0, 3], [5, 1023, 1024, 1025, 300001], [47] * 130, [2_000_003], [9, 13_000_001]])
 @pytest.mark.parametrize("max_norm,wd", [(0.5, 0.0), (2.0, 0.01), (1e9, 0.1)])
 def test_adam_step(sizes, max_norm, wd):
     from sparc_amd.optim import adam_step_

@@ -119,7 +119,11 @@ def test_lookup_far_into_a_large_table():
     ("zipf", 20000, 5000, 257), ("zipf", 70001, 30000, 33), ("zipf", 4096, 64, 1024),
     ("one", 1, 9, 8), ("one", 64, 9, 8), ("one", 65, 9, 8), ("one", 20000, 3, 47), ("one", 9000, 1, 600),
     ("falling", 4000, 4000, 20), ("falling", 9999, 700, 3), ("lengths", 0, 10, 64), ("lengths", 0, 4001, 72),
-    ("stray", 5000, 90, 12), ("stray", 100, 1, 4)])
+    ("stray", 5000, 90, 12), ("stray", 100, 1, 4),
+    # one launch or the sort: 16384 tokens, 4 MiB of gradient
+    ("zipf", 16384, 900, 5), ("zipf", 16385, 900, 5), ("one", 16385, 9, 3), ("falling", 16400, 5000, 3), ("stray", 40000, 70, 6),
+    ("lengths", 0, 200, 1030), ("zipf", 30000, 20000, 65), ("uniform", 17000, 1, 2), ("uniform", 66000, 2050, 1),
+    ("zipf", 300000, 70000, 2)])
 def test_gradient(pattern, n, rows, dim, dtype):
     from sparc_amd.embedding import embedding_grad
     ids = make_ids(pattern, n, rows, 3)
@@ -138,6 +142,33 @@ def test_gradient_of_many_rows_or_tokens(n, rows, dim):
     ids = make_ids("uniform", n, rows, 6)
     g = torch.randn(n, dim, device="cuda", generator=gen(7))
     check_grad(embedding_grad(ids, g, rows), ids, g, rows)
+
+
+@pytest.mark.parametrize("n,rows,dim,dtype", [(20000, 800_001, 64, torch.float32), (200_003, 1000, 256, torch.float32),
+                                              (120_001, 500_000, 1024, torch.bfloat16)])
+def test_gradients_that_outgrow_the_cache(n, rows, dim, dtype):
+    """The table's zeros, the gradient, both: with streaming accesses."""
+    from sparc_amd.embedding import embedding_grad
+    ids = make_ids("zipf", n, rows, 16)
+    g = torch.randn(n, dim, device="cuda", generator=gen(17)).to(dtype)
+    out = embedding_grad(ids, g, rows, padding_idx=1)
+    keep = torch.cat([ids.unique()[:3000], torch.randint(rows, (3000,), generator=gen(18), device="cuda")]).unique()
+    slot = torch.full((rows,), -1, dtype=torch.int64, device="cuda")
+    slot[keep] = torch.arange(keep.numel(), device="cuda")
+    of = slot[ids]
+    of[ids == 1] = -1
+    check_grad(out[keep], of[of >= 0], g[of >= 0], keep.numel())
+    touched = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    touched[ids] = True
+    touched[1] = False
+    assert int(((out != 0).any(1) != touched).sum()) == 0
+
+
+def test_lookup_that_outgrows_the_cache():
+    from sparc_amd.embedding import embedding_lookup
+    table = torch.randn(5000, 1000, device="cuda", generator=gen(19)).half()
+    ids = make_ids("zipf", 110_000, 5000, 20)
+    assert torch.equal(embedding_lookup(ids, table, scale=0.5), (table * 0.5)[ids])
 
 
 def test_gradient_past_32_bit_offsets():
