@@ -101,7 +101,7 @@ struct GradArgs {
     int64_t tile;              // tokens of a tile, a multiple of CHUNK
     int tiles;
     int dim, wide_ids;
-    int per;                   // places of a worker (few_tokens: rows of a workgroup)
+    int per;                   // places of a worker
     float scale;
     uint32_t* counts;          // [tiles][1 << bits]: digits of a tile
     uint2* sorted;             // [n] {row, place}; the last pass leaves the result here
@@ -489,18 +489,32 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
 
 // ---- gradient of few tokens: one launch ------------------------------------------------------------------
 
-// Up to FEW tokens a workgroup can look through all of them itself: it owns `per` consecutive rows, writes their zeros,
-// collects the places of its rows as keys {row, place} (in any order), sorts the keys and adds up the runs.  No workspace,
-// one launch instead of six dependent ones.
-constexpr int FEW = 16384, PLACE_BITS = 14;
+// Up to FEW tokens a workgroup can look through all of them itself: it writes the zeros of its rows, collects their places
+// as keys {row, place} (in any order), sorts the keys and adds up the runs.  No workspace, one launch instead of six
+// dependent ones.  The rows are dealt out in turn, in groups of at least GROUP_BYTES, because frequent tokens are often
+// neighbours.
+constexpr int FEW = 8192, PLACE_BITS = 13;
 constexpr int64_t FEW_BYTES = 4 << 20;   // of gradient: one workgroup adds it up alone where all tokens are the same
 constexpr int FEW_THREADS = 512;
-constexpr int FEW_BLOCKS = 512;   // rows are dealt to at most about that many workgroups
-constexpr int FEW_AHEAD = 8;       // gradient rows in flight per worker
-constexpr int FEW_TURNS = 4;       // 16-byte vectors of tokens in flight per thread
+constexpr int FEW_BLOCKS_LOG2 = 9;   // workgroups that the rows are dealt to
+constexpr int FEW_AHEAD = 8;         // gradient rows in flight per worker
+constexpr int FEW_TURNS = 4;         // 16-byte vectors of tokens in flight per thread
+constexpr int GROUP_BYTES = 256;
+
+// Row r belongs to workgroup (r >> group) mod 2^blocks, where it is row local(r).
+struct Dealt {
+    int group, blocks;
+    __device__ __forceinline__ uint32_t block_of(const uint32_t r) const { return (r >> group) & ((1u << blocks) - 1u); }
+    __device__ __forceinline__ uint32_t local(const uint32_t r) const {
+        return (r >> group >> blocks) << group | (r & ((1u << group) - 1u));
+    }
+    __device__ __forceinline__ int64_t row(const uint32_t block, const uint32_t local) const {
+        return ((static_cast<int64_t>(local >> group) << blocks | block) << group) | (local & ((1u << group) - 1u));
+    }
+};
 
 template <typename ID>
-__device__ __forceinline__ void collect_rows(const ID* ids, const int n, const int64_t row0, const int in_block, const int64_t padding,
+__device__ __forceinline__ void collect_rows(const ID* ids, const int n, const int64_t rows, const int64_t padding, const Dealt dealt,
                                              uint32_t* keys, uint32_t* count) {
     constexpr int VE = 16 / sizeof(ID);
     typedef ID mem __attribute__((ext_vector_type(VE), aligned(sizeof(ID))));
@@ -522,7 +536,8 @@ __device__ __forceinline__ void collect_rows(const ID* ids, const int n, const i
 #pragma unroll
             for (int c = 0; c < VE; ++c) {
                 const int64_t id = v[k][c];
-                const bool hit = id >= row0 && id < row0 + in_block && id != padding;
+                const uint32_t row = static_cast<uint32_t>(id);
+                const bool hit = dealt.block_of(row) == blockIdx.x && id >= 0 && id < rows && id != padding;
                 const uint64_t hits = __ballot(hit);
                 if (hits == 0) continue;                 // (the whole wave, nearly always)
                 uint32_t at = 0;
@@ -530,14 +545,14 @@ __device__ __forceinline__ void collect_rows(const ID* ids, const int n, const i
                 at = __builtin_amdgcn_readfirstlane(at);
                 if (hit) {
                     const int i = i0 + (k * FEW_THREADS + static_cast<int>(threadIdx.x)) * VE + c;
-                    keys[at + __popcll(hits & ((1ull << lane) - 1ull))] = static_cast<uint32_t>(id - row0) << PLACE_BITS | static_cast<uint32_t>(i);
+                    keys[at + __popcll(hits & ((1ull << lane) - 1ull))] = dealt.local(row) << PLACE_BITS | static_cast<uint32_t>(i);
                 }
             }
     }
 }
 
 template <int DT, int VE>
-__global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const int lanes_log2) {
+__global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const Dealt dealt, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t keys[];     // a power of two of them, at least n
     __shared__ uint32_t total_found;
@@ -547,8 +562,6 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
     T* out = static_cast<T*>(a.out);
     const int tid = threadIdx.x;
     const int n = static_cast<int>(a.n);
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.per;
-    const int in_block = static_cast<int>(min(static_cast<int64_t>(a.per), a.rows - row0));
     if (tid == 0) n_long = total_found = 0;
     const int lanes = 1 << lanes_log2, workers = FEW_THREADS >> lanes_log2, worker = tid >> lanes_log2;
     const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + (tid & (lanes - 1));
@@ -557,16 +570,25 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
     Vec<DT, VE> zero;
 #pragma unroll
     for (int i = 0; i < VE; ++i) zero.set(i, 0.f);
-    if (gridDim.y == 1) {
-        T* block = out + row0 * a.dim;                   // the rows are one stretch of memory
-        const int64_t len = static_cast<int64_t>(in_block) * a.dim;
-        for (int64_t e = static_cast<int64_t>(tid) * VE; e < len; e += FEW_THREADS * VE) zero.store(block + min(e, len - VE));
+    if (dealt.group > 0) {                               // narrow rows, one slice: a group of them is one stretch of memory
+        const int64_t stretch = static_cast<int64_t>(a.dim) << dealt.group, len = a.rows * a.dim;
+        const int per_stretch = static_cast<int>((stretch + VE - 1) / VE);
+        int log2 = 0;
+        while ((1 << log2) < per_stretch) ++log2;        // (at most FEW_THREADS: a stretch is shorter than 2 GROUP_BYTES)
+        const int e = (tid & ((1 << log2) - 1)) * VE;
+        for (int64_t q = tid >> log2;; q += FEW_THREADS >> log2) {
+            const int64_t from = ((q << dealt.blocks) + blockIdx.x) * stretch;
+            if (from >= len) break;
+            const int64_t here = min(stretch, len - from);
+            if (e < here) zero.store(out + from + min(static_cast<int64_t>(e), here - VE));
+        }
     } else if (mine) {
-        for (int r = worker; r < in_block; r += workers) zero.store(out + (row0 + r) * a.dim + col);
+        for (int64_t r = blockIdx.x + (static_cast<int64_t>(worker) << dealt.blocks); r < a.rows; r += static_cast<int64_t>(workers) << dealt.blocks)
+            zero.store(out + r * a.dim + col);
     }
     __syncthreads();
-    if (a.wide_ids) collect_rows(static_cast<const int64_t*>(a.ids), n, row0, in_block, a.padding, keys, &total_found);
-    else collect_rows(static_cast<const int32_t*>(a.ids), n, row0, in_block, a.padding, keys, &total_found);
+    if (a.wide_ids) collect_rows(static_cast<const int64_t*>(a.ids), n, a.rows, a.padding, dealt, keys, &total_found);
+    else collect_rows(static_cast<const int32_t*>(a.ids), n, a.rows, a.padding, dealt, keys, &total_found);
     __syncthreads();
     const int count = static_cast<int>(total_found);
     if (count == 0) return;                              // (the whole workgroup)
@@ -609,15 +631,19 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
             if ((tid & (lanes - 1)) == 0) long_runs[atomicAdd(&n_long, 1u)] = i;
             continue;
         }
-        int end = i + 1;
-        while (same_row(end, row)) ++end;
         if (!mine) continue;
+        int end = i + 1, behind = min(i + LONG_ROW, count);
+        while (end < behind) {
+            const int mid = (end + behind) >> 1;
+            if (keys[mid] >> PLACE_BITS == row) end = mid + 1;
+            else behind = mid;
+        }
         float acc[VE] = {};
         add(acc, i, end);
         Vec<DT, VE> v;
 #pragma unroll
         for (int c = 0; c < VE; ++c) v.set(c, acc[c] * a.scale);
-        v.store(out + (row0 + row) * a.dim + col);
+        v.store(out + dealt.row(blockIdx.x, row) * a.dim + col);
     }
     __syncthreads();
     for (uint32_t m = 0; m < n_long; ++m) {              // a long run: every worker takes a part, joined in order
@@ -643,7 +669,7 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
                 for (int w = 0; w < workers; ++w) s += piece[(w * lanes + tid) * VE + c];
                 v.set(c, static_cast<float>(s) * a.scale);
             }
-            v.store(out + (row0 + row) * a.dim + col);
+            v.store(out + dealt.row(blockIdx.x, row) * a.dim + col);
         }
         __syncthreads();
     }
@@ -808,11 +834,20 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
 }
 
 template <int DT, int VE>
-int launch_few(const GradArgs& a, const int lanes_log2, const int slices, sparc_stream_t stream) {
+int launch_few(const GradArgs& a, sparc_stream_t stream) {
+    int slices;
+    const int lanes_log2 = lanes_for(ceil_div(a.dim, VE), &slices);
+    Dealt d = {0, 0};
+    while ((static_cast<int64_t>(a.dim) * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) << d.group) < GROUP_BYTES) ++d.group;
+    const int64_t groups = ceil_div(a.rows, static_cast<int64_t>(1) << d.group);
+    while (d.blocks < FEW_BLOCKS_LOG2 && (static_cast<int64_t>(1) << d.blocks) < groups) ++d.blocks;
+    // (a row's number inside its workgroup leaves a bit of the key for the one that pads the sort)
+    while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (1 << (31 - PLACE_BITS))) ++d.blocks;
+    const unsigned grid = static_cast<unsigned>(groups < (1 << d.blocks) ? groups : 1 << d.blocks);
     size_t keys = 1;
     while (keys < static_cast<size_t>(a.n)) keys <<= 1;
-    hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(static_cast<unsigned>(ceil_div(a.rows, a.per)), static_cast<unsigned>(slices)), dim3(FEW_THREADS),
-                       keys * sizeof(uint32_t), stream, a, lanes_log2);
+    hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(grid, static_cast<unsigned>(slices)), dim3(FEW_THREADS), keys * sizeof(uint32_t), stream, a, d,
+                       lanes_log2);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
@@ -830,13 +865,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
     GradArgs a = {};
     Plan p = {};
     const bool few = few_enough(n, dim, dtype);
-    if (few) {
-        p.lanes_log2 = lanes_for(ceil_div(dim, used_ve), &p.slices);
-        int64_t per = ceil_div(rows, FEW_BLOCKS);
-        const int64_t most = static_cast<int64_t>(1) << (32 - PLACE_BITS - 1);   // (keys stay below the one that pads the sort)
-        if (per > most) per = most;
-        a.per = static_cast<int>(per);
-    } else {
+    if (!few) {
         p = plan_of(n, rows, static_cast<int>(dim), used_ve);
         bool ok;
         size_t used;
@@ -858,6 +887,6 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
     a.scale = static_cast<float>(scale);
     return dispatch(dtype, dim, [&](auto type, auto width) {
         constexpr int DT = decltype(type)::value, VE = decltype(width)::value;
-        return few ? launch_few<DT, VE>(a, p.lanes_log2, p.slices, stream) : launch_grad<DT, VE>(a, p, stream);
+        return few ? launch_few<DT, VE>(a, stream) : launch_grad<DT, VE>(a, p, stream);
     });
 }

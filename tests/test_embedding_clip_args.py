@@ -28,8 +28,8 @@ def test_embedding_arguments():
     assert grad(rows=0) == 0 and grad(dim=0, ldg=0) == 0
     assert lib.sparc_embedding_grad_workspace_bytes(1 << 31, 5, 8, 0) == 0
     assert lib.sparc_embedding_grad_workspace_bytes(4, 5, 8, 7) == 0
-    assert lib.sparc_embedding_grad_workspace_bytes(16384, 5, 8, 0) == 0        # one launch, without scratch
-    assert lib.sparc_embedding_grad_workspace_bytes(16385, 5, 8, 0) > 0
+    assert lib.sparc_embedding_grad_workspace_bytes(8192, 5, 8, 0) == 0        # one launch, without scratch
+    assert lib.sparc_embedding_grad_workspace_bytes(8193, 5, 8, 0) > 0
 
 
 def test_gradient_workspace_stays_near_its_operands():

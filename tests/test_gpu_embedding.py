@@ -120,8 +120,9 @@ def test_lookup_far_into_a_large_table():
     ("one", 1, 9, 8), ("one", 64, 9, 8), ("one", 65, 9, 8), ("one", 20000, 3, 47), ("one", 9000, 1, 600),
     ("falling", 4000, 4000, 20), ("falling", 9999, 700, 3), ("lengths", 0, 10, 64), ("lengths", 0, 4001, 72),
     ("stray", 5000, 90, 12), ("stray", 100, 1, 4),
-    # one launch or the sort: 16384 tokens, 4 MiB of gradient
-    ("zipf", 16384, 900, 5), ("zipf", 16385, 900, 5), ("one", 16385, 9, 3), ("falling", 16400, 5000, 3), ("stray", 40000, 70, 6),
+    # one launch or the sort: 8192 tokens, 4 MiB of gradient
+    ("zipf", 8192, 900, 5), ("zipf", 8193, 900, 5), ("one", 8193, 9, 3), ("one", 8192, 900, 7), ("uniform", 8192, 3000, 128),
+    ("uniform", 8192, 3000, 129), ("zipf", 2000, 100_000, 1), ("falling", 8000, 9_000, 16), ("zipf", 16384, 900, 5), ("falling", 16400, 5000, 3), ("stray", 40000, 70, 6),
     ("lengths", 0, 200, 1030), ("zipf", 30000, 20000, 65), ("uniform", 17000, 1, 2), ("uniform", 66000, 2050, 1),
     ("zipf", 300000, 70000, 2)])
 def test_gradient(pattern, n, rows, dim, dtype):
@@ -136,7 +137,7 @@ def test_gradient(pattern, n, rows, dim, dtype):
     check_grad(embedding_grad(ids, g, rows, padding_idx=pad), ids, g, rows, 1.0, pad)
 
 
-@pytest.mark.parametrize("n,rows,dim", [(5000, 9_000_001, 1), (4_500_000, 1000, 1), (3000, 4_300_000, 2), (49_000, 2_449_029, 4)])
+@pytest.mark.parametrize("n,rows,dim", [(5000, 9_000_001, 1), (300, 140_000_000, 1), (300, 70_000_000, 4), (4_500_000, 1000, 1), (3000, 4_300_000, 2), (49_000, 2_449_029, 4)])
 def test_gradient_of_many_rows_or_tokens(n, rows, dim):
     from sparc_amd.embedding import embedding_grad
     ids = make_ids("uniform", n, rows, 6)
