@@ -66,7 +66,8 @@ def check_grad(got, ids, g, rows, scale=1.0, padding_idx=None):
     bound = SLACK * (places[:, None] * U * size + HALF[g.dtype] * want.abs()) + TINY[g.dtype]
     off = (got.double() - want).abs()
     assert bool((off <= bound).all()), float((off - bound).max())
-    assert bool((got[places == 0] == 0).all())
+    # (elementwise: torch's selection of 70 million rows returned rows that it had not written)
+    assert not bool(((got != 0).any(1) & (places == 0)).any())
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
