@@ -86,19 +86,19 @@ __device__ __forceinline__ double squares(const void* p, const int64_t n, const 
         for (int j = 0; j < TURNS; ++j) v[j].template load<STREAM>(g + j * NORM_THREADS * VE);
 #pragma unroll
         for (int j = 0; j < TURNS; ++j) add(v[j]);
-    } else {   // the tensor's end
-        const int64_t left = n - e0 - static_cast<int64_t>(threadIdx.x) * VE;
-        int j = 0;
-#pragma unroll 2
-        for (; j + VE <= left; j += NORM_THREADS * VE) {
-            Vec<DT, VE> v;
-            v.load(g + j);
-            add(v);
-        }
-        for (; j < left; ++j) {   // (less than a vector, of one thread)
-            const double x = Elem<DT>::up(g[j]);
-            s = fma(x, x, s);
-        }
+    } else {   // the tensor's end: whole vectors, all loads at once, and an element each for the first threads
+        const int64_t here = n - e0, left = here - static_cast<int64_t>(threadIdx.x) * VE;
+        const int rest = static_cast<int>(here % VE);
+        const T* last = static_cast<const T*>(p) + n - rest;
+        const double x = static_cast<int>(threadIdx.x) < rest ? Elem<DT>::up(last[threadIdx.x]) : 0.f;
+        Vec<DT, VE> v[TURNS];
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j)
+            if (j * NORM_THREADS * VE + VE <= left) v[j].load(g + j * NORM_THREADS * VE);
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j)
+            if (j * NORM_THREADS * VE + VE <= left) add(v[j]);
+        s = fma(x, x, s);
     }
     return s;
 }
@@ -113,7 +113,7 @@ __device__ __forceinline__ double squares_of_block(const Records& records, const
            : dtype == SPARC_BF16 ? squares<SPARC_BF16, STREAM>(p, n, k) : squares<SPARC_F16, STREAM>(p, n, k);
 }
 
-__global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(const GradArgs a, double* parts) {
+__global__ __launch_bounds__(NORM_THREADS, 8) void grad_squares_kernel(const GradArgs a, double* parts) {
     __shared__ double lds[NORM_THREADS / 64];
     const Records records(a);
     double s = 0.0;
@@ -146,20 +146,24 @@ struct Clip {
     int n_parts;
 };
 
-// The coefficient, in every thread; computed where it is first asked for, behind the loads that do not need it.  A norm that
-// is not finite gives what the formula gives: 0 for an infinite one (so infinite gradients become NaN), NaN for NaN; an
+// The coefficient, in every thread: the partial sums are requested first of all, and added up where the coefficient is first
+// asked for, behind the loads that do not need it.  A norm that is not finite gives what the formula gives: 0 for an infinite one (so infinite gradients become NaN), NaN for NaN; an
 // infinite max_norm never clips.
 struct Coefficient {
     const Clip& c;
     double* lds;
+    double parts;
     float value;
     bool known;
-    __device__ __forceinline__ Coefficient(const Clip& clip, double* scratch) : c(clip), lds(scratch), value(0.f), known(false) {}
+    __device__ __forceinline__ Coefficient(const Clip& clip, double* scratch) : c(clip), lds(scratch), parts(0.0), value(0.f), known(false) {
+        static_assert(PARTS <= 2 * BLOCK, "two partial sums per thread");
+        const int i = threadIdx.x;
+        const double first = i < c.n_parts ? c.parts[i] : 0.0, second = i + BLOCK < c.n_parts ? c.parts[i + BLOCK] : 0.0;
+        parts = first + second;
+    }
     __device__ __forceinline__ float get() {   // by the whole workgroup
         if (!known) {
-            double s = 0.0;
-            for (int i = threadIdx.x; i < c.n_parts; i += BLOCK) s += c.parts[i];
-            const double norm = sqrt(block_sum(s, lds));
+            const double norm = sqrt(block_sum(parts, lds));
             if (c.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *c.norm_out = static_cast<float>(norm);
             const double coef = isinf(c.max_norm) ? 1.0 : c.max_norm / (norm + 1e-6);
             value = coef >= 1.0 ? 1.f : static_cast<float>(coef);
@@ -189,18 +193,23 @@ __device__ __forceinline__ void scale_block(void* p, const int64_t n, const int6
             scaled(v[j], coef);
             v[j].template store<STREAM>(g + j * BLOCK * VE);
         }
-    } else {
-        const int64_t left = n - e0 - static_cast<int64_t>(threadIdx.x) * VE;
+    } else {   // the tensor's end: whole vectors, all loads at once, and an element each for the first threads
+        const int64_t here = n - e0, left = here - static_cast<int64_t>(threadIdx.x) * VE;
+        const int rest = static_cast<int>(here % VE);
+        T* last = static_cast<T*>(p) + n - rest;
+        const float x = static_cast<int>(threadIdx.x) < rest ? Elem<DT>::up(last[threadIdx.x]) : 0.f;
+        Vec<DT, VE> v[TURNS];
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j)
+            if (j * BLOCK * VE + VE <= left) v[j].load(g + j * BLOCK * VE);
         const float coef = c.get();
-        int j = 0;
-#pragma unroll 2
-        for (; j + VE <= left; j += BLOCK * VE) {
-            Vec<DT, VE> v;
-            v.load(g + j);
-            scaled(v, coef);
-            v.store(g + j);
-        }
-        for (; j < left; ++j) g[j] = Elem<DT>::down(Elem<DT>::up(g[j]) * coef);
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j)
+            if (j * BLOCK * VE + VE <= left) {
+                scaled(v[j], coef);
+                v[j].store(g + j * BLOCK * VE);
+            }
+        if (static_cast<int>(threadIdx.x) < rest) last[threadIdx.x] = Elem<DT>::down(x * coef);
     }
 }
 
@@ -208,8 +217,8 @@ __device__ __forceinline__ void scale_block(void* p, const int64_t n, const int6
 template <bool STREAM>
 __global__ __launch_bounds__(BLOCK) void grad_scale_kernel(const GradArgs a, const Clip clip) {
     __shared__ double lds[BLOCK / 64];
-    const Records records(a);
     Coefficient c(clip, lds);
+    const Records records(a);
     for (int b = a.blocks - 1 - static_cast<int>(blockIdx.x); b >= 0; b -= gridDim.x) {
         void* p;
         int64_t n, k;
@@ -242,11 +251,11 @@ template <bool STREAM>
 __global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, const Clip clip) {
     __shared__ double lds[BLOCK / 64];
     typedef Vec<SPARC_F32, 4> V4;
+    Coefficient c(clip, lds);
     const int lane = threadIdx.x & 63;
-    const sparc_adam_tensor_t mine = a.t[lane];   // (ADAM_MOST lanes)
+    const sparc_adam_tensor_t mine = a.t[lane];
     const int32_t first = a.first_block[lane];
     static_assert(ADAM_MOST == 64, "a record per lane");
-    Coefficient c(clip, lds);
     for (int b = blockIdx.x; b < a.blocks; b += gridDim.x) {
         const int of = __popcll(__ballot(first <= b)) - 1;
         float* tp = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.p), of));
@@ -256,30 +265,42 @@ __global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, 
         const int64_t n = lane_value(mine.n, of);
         const int64_t e = static_cast<int64_t>(b - __builtin_amdgcn_readlane(first, of)) * ADAM_ELEMS + threadIdx.x * 4;
         const bool whole = e + 4 <= n;
-        V4 p, g, m, v;
+        V4 p = {}, g = {}, m = {}, v = {};
         if (whole) {
             g.load<STREAM>(tg + e);
             p.load<STREAM>(tp + e);
             m.load<STREAM>(tm + e);
             v.load<STREAM>(tv + e);
+        } else {   // the tensor's end
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (e + i < n) {
+                    g.v[i] = tg[e + i];
+                    p.v[i] = tp[e + i];
+                    m.v[i] = tm[e + i];
+                    v.v[i] = tv[e + i];
+                }
         }
         const float coef = c.get();
-        if (whole) {
+        if (e >= n) continue;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float pi = p.v[i], mi = m.v[i], vi = v.v[i];
-                adam_one(pi, g.v[i], mi, vi, a, coef);
-                p.v[i] = pi; m.v[i] = mi; v.v[i] = vi;
-            }
+        for (int i = 0; i < 4; ++i) {
+            float pi = p.v[i], mi = m.v[i], vi = v.v[i];
+            adam_one(pi, g.v[i], mi, vi, a, coef);
+            p.v[i] = pi; m.v[i] = mi; v.v[i] = vi;
+        }
+        if (whole) {
             p.store<STREAM>(tp + e);
             m.store<STREAM>(tm + e);
             v.store<STREAM>(tv + e);
         } else {
-            for (int64_t i = e; i < n; ++i) {
-                float pi = tp[i], mi = tm[i], vi = tv[i];
-                adam_one(pi, tg[i], mi, vi, a, coef);
-                tp[i] = pi; tm[i] = mi; tv[i] = vi;
-            }
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (e + i < n) {
+                    tp[e + i] = p.v[i];
+                    tm[e + i] = m.v[i];
+                    tv[e + i] = v.v[i];
+                }
         }
     }
     c.get();   // (a list without elements has a norm too)
