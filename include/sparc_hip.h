@@ -456,9 +456,9 @@ int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr
  * tensors: a HOST array of records of device pointers, elements dense in memory, in any order, at any element alignment.
  *   sparc_grad_norm          the sums of squares (float64) as partial sums: parts[0 .. *n_parts), n_parts a HOST
  *                            word written before the call returns; parts: the query's bytes, 8-byte aligned.
- *   sparc_grad_scale         g <- c g, rounded to nearest, in place, and *norm_out = N (one device float)
+ *   sparc_clip_grad_norm     the same, then g <- c g, rounded to nearest, in place, and *norm_out = N (one device float)
  *   sparc_adam_step_clipped  sparc_adam_step on c g (the gradients themselves stay), any number of tensors, and *norm_out
- * The two consumers add the partial sums up themselves, in a fixed order. */
+ * Whoever scales adds the partial sums up itself, in a fixed order. */
 #define SPARC_F32 0
 #define SPARC_BF16 1
 #define SPARC_F16 2
@@ -472,8 +472,8 @@ typedef struct {
 size_t sparc_grad_norm_workspace_bytes(int64_t n_tensors);
 int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double* parts, size_t parts_bytes,
                     int64_t* n_parts, sparc_stream_t stream);
-int sparc_grad_scale(int64_t n_tensors, const sparc_grad_tensor_t* tensors, const double* parts, int64_t n_parts,
-                     double max_norm, float* norm_out, sparc_stream_t stream);
+int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double max_norm, double* parts,
+                         size_t parts_bytes, float* norm_out, sparc_stream_t stream);
 int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
                             double eps, double weight_decay, int64_t step, const double* parts, int64_t n_parts,
                             double max_norm, float* norm_out, sparc_stream_t stream);

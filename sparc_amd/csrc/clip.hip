@@ -370,9 +370,12 @@ extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* ten
     return SPARC_OK;
 }
 
-extern "C" int sparc_grad_scale(int64_t n_tensors, const sparc_grad_tensor_t* tensors, const double* parts, int64_t n_parts,
-                                double max_norm, float* norm_out, sparc_stream_t stream) {
-    if (!parts || !norm_out || n_parts < 0 || n_parts > PARTS || !(max_norm >= 0.0) || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
+extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double max_norm, double* parts,
+                                    size_t parts_bytes, float* norm_out, sparc_stream_t stream) {
+    if (!norm_out || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
+    int64_t n_parts = 0;
+    const int rc = sparc_grad_norm(n_tensors, tensors, parts, parts_bytes, &n_parts, stream);
+    if (rc != SPARC_OK) return rc;
     Clip c = {parts, norm_out, max_norm, static_cast<int>(n_parts)};
     int64_t left = 0;
     const int64_t launches = n_tensors ? (n_tensors + SPARC_GRAD_MAX_TENSORS - 1) / SPARC_GRAD_MAX_TENSORS : 1;

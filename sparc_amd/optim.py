@@ -47,7 +47,8 @@ def _grad_records(grads, device):
     types = list(map(_type_of, grads))
     if not _dense_on(grads, device, _dense) or not DTYPES.keys() >= set(types):
         raise ValueError("the gradients of one norm are dense float32, bfloat16 or float16 tensors on one device")
-    return _records(list(map(_address_of, grads)), list(map(_size_of, grads)), [DTYPES[t] for t in types])
+    codes = [DTYPES[types[0]]] * len(types) if types.count(types[0]) == len(types) else [DTYPES[t] for t in types]
+    return _records(list(map(_address_of, grads)), list(map(_size_of, grads)), codes)
 
 
 def _records(*columns):
@@ -95,9 +96,10 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if not grads[0].is_cuda:
         require_gpu(device)
     records = _grad_records(grads, device)
-    parts, count = _norm_of(records, len(grads), device)
+    nbytes = lib.sparc_grad_norm_workspace_bytes(len(grads))
+    parts = torch.empty(nbytes >> 3, dtype=torch.float64, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    launch("sparc_grad_scale", lib.sparc_grad_scale, device, len(grads), _address(records), parts.data_ptr(), count, max_norm,
+    launch("sparc_clip_grad_norm", lib.sparc_clip_grad_norm, device, len(grads), _address(records), max_norm, parts.data_ptr(), nbytes,
            norm.data_ptr())
     return norm
 

@@ -51,9 +51,10 @@ def test_clip_arguments():
     for bad in ((P, -1, 0), (0, 1, 0), (P, 1, 3), (P, 1, -1), (P, (1 << 34) + 1, 0)):
         assert norm(t=(ctypes.c_int64 * 3)(*bad)) == -1, bad
     assert norm(n=0, t=None) == 0 and count.value == 0                       # an empty list has no partial sums
-    scale = lambda n=1, t=one, parts=P, k=1, limit=1.0, out=P: lib.sparc_grad_scale(n, t, parts, k, limit, out, None)  # noqa: E731
-    for bad in (dict(n=-1), dict(t=None), dict(parts=None), dict(k=-1), dict(k=1025), dict(limit=-1.0), dict(limit=float("nan")), dict(out=None)):
-        assert scale(**bad) == -1, bad
+    clip = lambda n=1, t=one, limit=1.0, parts=P, nbytes=1 << 20, out=P: lib.sparc_clip_grad_norm(n, t, limit, parts, nbytes, out, None)  # noqa: E731
+    for bad in (dict(n=-1), dict(t=None), dict(parts=None), dict(limit=-1.0), dict(limit=float("nan")), dict(out=None)):
+        assert clip(**bad) == -1, bad
+    assert clip(nbytes=8) == -2
     rec = (ctypes.c_int64 * 5)(P, P, P, P, 100)
     adam = lambda n=1, t=rec, b1=0.9, b2=0.999, eps=1e-8, step=1, parts=P, k=1, limit=1.0, out=P: lib.sparc_adam_step_clipped(  # noqa: E731
         n, t, 1e-3, b1, b2, eps, 0.0, step, parts, k, limit, out, None)
