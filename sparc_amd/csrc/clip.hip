@@ -7,6 +7,16 @@
 // PARTS of them, in the grid's order); whoever needs the coefficient adds them up itself, every workgroup the same
 // numbers in the same order, so there is neither a launch nor an arrival counter between the two passes and runs repeat
 // bit for bit.
+//
+// Measured.  629 MB of float32 (a table and an MLP): norm 100 us = 6.3 TB/s, scaling 194 us = 6.5 TB/s; plain accesses:
+// 161 and 204 us, because what the norm's pass leaves in the Infinity Cache is gone when the scaling comes to it, and what
+// the scaling leaves there has to be written back under the next pass.  Without the last 192 MB that the norm's pass reads
+// plainly for the scaling, which goes backwards: 94 and 205 us.  Lists below 192 MB stay plain: 160 MB, three lists in turn, 80 us
+// streamed, 93 us plain; one list again and again 80 and 72 us.
+// 6.4 MB (the MLP alone): 4.0 + 6.0 us, of which launches and the chain parts -> sum -> root -> quotient are most; the
+// host's two launches and checks take longer (16.7 us a call).
+// Adam on 31.5 M floats (883 MB): norm 24 us, update 136 us = 6.5 TB/s; plain accesses 40 and 160 us.  Below 192 MB plain:
+// 8 M floats 49.1 us streamed, 49.7 us plain; 4 M 27.8 and 25.1.
 #include "elem.h"
 
 namespace {

@@ -51,6 +51,10 @@ __device__ __forceinline__ int64_t token(const void* ids, const int wide, const 
 // A group of 2^lanes_log2 lanes per row, a 16-byte vector per lane (an element of rows shorter than that), slice blockIdx.y
 // of the columns; TURNS rows in flight per group, neighbouring groups on neighbouring rows.  A row's last vector ends with
 // the row: it overlaps the one before it and both write the same values.
+// STREAM, for outputs that outgrow the Infinity Cache: they leave with nontemporal stores, and the caches keep the table's
+// frequent rows.  262147 bfloat16 rows of 1024 (537 MB), frequent tokens first: 106 us = 6.0 TB/s, 157 us with plain
+// stores; 134 MB: 29.5 against 31.1 us, but 71.3 against 69.5 us with a pass behind it that reads the output.  Bound by
+// the stores (a fill of that size runs at 6.85 TB/s).  TURNS 2 / 8: 163 / 159 us (plain stores).
 constexpr int TURNS = 4;
 
 template <int DT, int VE, bool STREAM>
@@ -178,6 +182,12 @@ __device__ __forceinline__ void take(const GradArgs& a, const bool first, const 
     }
 }
 
+// The sort: two or three passes of a count and a scatter.  262147 tokens over 50021 rows, two passes of 8 bits: 6.0 + 10.0 us
+// each; 48979 tokens over 2449029 rows, two of 11 bits: 28 us a launch with a quarter of the 627 MB of zeros in it (4.7 and
+// 9 us without).  Bound by latency: of a scatter's 9 us 3.5 are the ranking (ballots: six vector instructions a bit), 2 the
+// other tiles' counts, the rest start, loads and stores.  512 threads with 4 tokens each: 5.0 + 9.4 us; 8 each: 5.7 + 11.1;
+// 1024 threads with 8: 7.3 + 13.6.  Sorting by buckets of rows instead (a workgroup per bucket) took 115 to 514 us where
+// frequent tokens share a bucket.
 // Digits of the tokens of a tile: digit = (row >> shift) & (1 << bits) - 1.
 __global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, const Zeros z, const uint2* in, const int shift, const int bits) {
     __shared__ uint32_t cnt[1 << MOST_BITS];
@@ -316,7 +326,12 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
 }
 
 // Workers are groups of `lanes` lanes (a power of two); lane u of a group owns VE columns of the slice blockIdx.y.
-// STREAM: a gradient that is read once and outgrows the Infinity Cache goes by it.
+// STREAM: a gradient that outgrows the Infinity Cache goes by it with nontemporal loads: 262147 rows of 512 bfloat16, three
+// gradients in turn, 71 -> 58 us (the same one again and again: 91 -> 99 us for the whole call).  Now 53 us = 6.0 TB/s of
+// gradient and table, bound by the loads of whole rows at random places; 8 rows in flight per worker, 4: 64 us.
+// Walking rows and places together, so that a worker also writes the zeros of the rows between its own, saves the second
+// write of the rows that have places (1024 columns, as many rows as places: 251 against 271 us) and lost everywhere
+// else (48979 places in 2449029 rows: 153 against 125 us).
 constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
 
 template <int DT, int VE, bool STREAM>
@@ -422,6 +437,7 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
 
 // Long rows: slice blockIdx.y of 64 columns, VE (four, or one where a row has fewer) columns to a lane.  The pieces of a
 // row are dealt to the groups of 16 lanes, which have JOIN_AHEAD of them in flight; the groups' sums meet in their order.
+// 9 us for the 300 long rows of 262147 tokens, frequent ones first; 4.6 us (the wait for the launch before) for none.
 constexpr int JOIN_WAVES = 4, JOIN_GROUPS = JOIN_WAVES * 4, JOIN_AHEAD = 8;
 
 template <int DT, int VE>
@@ -492,7 +508,10 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
 // Up to FEW tokens a workgroup can look through all of them itself: it writes the zeros of its rows, collects their places
 // as keys {row, place} (in any order), sorts the keys and adds up the runs.  No workspace, one launch instead of six
 // dependent ones.  The rows are dealt out in turn, in groups of at least GROUP_BYTES, because frequent tokens are often
-// neighbours.
+// neighbours (8192 tokens, frequent first: 26 us; dealt out in stretches 156 us, sorted 40 us).
+// 2437 tokens over 2708 rows of 64 floats: 6.8 us, the call 9.0 (the sort: 26); 8192 over 50000: 10.7 (29).  Bound by its
+// chain of tokens -> keys -> rows -> stores.  The price is the call whose tokens are all the same: one workgroup adds them
+// up, 8192 rows of 64 floats take 145 us (the sort: 36), 4096 of 512 bfloat16 178 (42).
 constexpr int FEW = 8192, PLACE_BITS = 13;
 constexpr int64_t FEW_BYTES = 4 << 20;   // of gradient: one workgroup adds it up alone where all tokens are the same
 constexpr int FEW_THREADS = 512;
