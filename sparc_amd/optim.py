@@ -10,6 +10,7 @@ import operator
 from array import array
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ._lib import AdamTensor, lib
 from .embedding import DTYPES
@@ -28,7 +29,7 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-_type_of = operator.attrgetter("dtype")
+_type_of, _needs_grad = operator.attrgetter("dtype"), operator.attrgetter("requires_grad")
 _device_of, _address_of, _size_of = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
 _is_contiguous = torch.Tensor.is_contiguous
 
@@ -43,12 +44,25 @@ def _dense_on(tensors, device, dense=None) -> bool:
 
 
 def _grad_records(grads, device):
-    """The list as the C calls take it (an array of {address, elements, type}: keep it while they run)."""
+    """(the list as the C calls take it, an array of {address, elements, type}: keep it while they run; how many records)."""
     types = list(map(_type_of, grads))
     if not _dense_on(grads, device, _dense) or not DTYPES.keys() >= set(types):
         raise ValueError("the gradients of one norm are dense float32, bfloat16 or float16 tensors on one device")
     codes = [DTYPES[types[0]]] * len(types) if types.count(types[0]) == len(types) else [DTYPES[t] for t in types]
-    return _records(list(map(_address_of, grads)), list(map(_size_of, grads)), codes)
+    at, sizes = list(map(_address_of, grads)), list(map(_size_of, grads))
+    if len(set(at)) < len(at):
+        at, sizes, codes = _each_once(at, sizes, codes)
+    return _records(at, sizes, codes), len(at)
+
+
+def _each_once(at, sizes, codes):
+    """The three columns without the empty tensors and those whose memory an earlier one has: two workgroups that scale the
+    same elements would race."""
+    seen = {}
+    for a, n, code in zip(at, sizes, codes):
+        if n and seen.setdefault(a, (a, n, code)) != (a, n, code):
+            raise ValueError("gradients that overlap in part")
+    return [[r[i] for r in seen.values()] for i in range(3)]
 
 
 def _records(*columns):
@@ -81,45 +95,54 @@ def _limit(max_norm) -> float:
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the gradients of `parameters` (one tensor or several; those without a gradient are passed over, a gradient met
-    twice counts once) in place by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them together, and
-    returns the norm before (float32, on the device; nothing synchronises).  float32, bfloat16 and float16 gradients may be
-    mixed; sums in float64.  A norm that is not finite leaves what the formula gives; an infinite max_norm never clips."""
+    twice, the same memory, counts once) in place by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them
+    together, and returns the norm before (float32, on the device; nothing synchronises).  float32, bfloat16 and float16
+    gradients may be mixed, each dense in memory (any order of the dimensions, views into a bucket too) and none overlapping
+    another in part; sums in float64.  A norm that is not finite leaves what the formula gives; an infinite max_norm never
+    clips."""
     max_norm = _limit(max_norm)
     if torch.is_tensor(parameters):
         parameters = (parameters,)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
-    if len(set(map(id, grads))) < len(grads):
-        grads = list({id(g): g for g in grads}.values())
     if not grads:
         return torch.zeros(())
     device = grads[0].device
     if not grads[0].is_cuda:
         require_gpu(device)
-    records = _grad_records(grads, device)
-    nbytes = lib.sparc_grad_norm_workspace_bytes(len(grads))
+    records, n = _grad_records(grads, device)
+    nbytes = lib.sparc_grad_norm_workspace_bytes(n)
     parts = torch.empty(nbytes >> 3, dtype=torch.float64, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    launch("sparc_clip_grad_norm", lib.sparc_clip_grad_norm, device, len(grads), _address(records), max_norm, parts.data_ptr(), nbytes,
+    launch("sparc_clip_grad_norm", lib.sparc_clip_grad_norm, device, n, _address(records), max_norm, parts.data_ptr(), nbytes,
            norm.data_ptr())
+    if True in map(_needs_grad, grads):   # of a backward with create_graph: who goes on through them is told
+        increment_version([g for g in grads if g.requires_grad])
     return norm
 
 
 def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
-    """(records of the update, records of the gradients)."""
+    """(records of the update, records of the gradients, how many of those)."""
     n = len(params)
     every = [*params, *grads, *exp_avgs, *exp_avg_sqs]
     sizes = list(map(_size_of, every))
     if set(map(_type_of, every)) != {torch.float32} or not _dense_on(every, device) or sizes != sizes[:n] * 4:
         raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
     at = list(map(_address_of, every))
-    return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), _records(at[n:2 * n], sizes[:n], [0] * n)
+    of_grads = (at[n:2 * n], sizes[:n], [0] * n)
+    if len(set(at)) < 4 * n:   # empty tensors, or a gradient that several parameters share: nothing else may occur twice
+        full = [a for a, size in zip(at, sizes) if size]
+        of_grads = _each_once(*of_grads)
+        if len(set(full)) < len(full) // 4 * 3 + len(of_grads[0]):
+            raise ValueError("an Adam step writes every parameter and moment once")
+    return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), _records(*of_grads), len(of_grads[0])
 
 
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 0.0, max_grad_norm=None):
     """Update number `step` (from 1) of torch.optim.Adam on lists of tensors, in place: params, exp_avgs and exp_avg_sqs.
     With max_grad_norm the gradients enter as clip_grad_norm_(..., max_grad_norm) would leave them, but are only read
-    (once for the norm, once by the update); returns their norm then, None otherwise."""
+    (once for the norm, once by the update); returns their norm then, None otherwise.  Gradients may be shared, what is written
+    may not."""
     params = list(params)
     if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs)):
         raise ValueError("as many gradients and moments as parameters")
@@ -128,16 +151,18 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     device = params[0].device
     if not params[0].is_cuda:
         require_gpu(device)
-    records, of_grads = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
+    records, of_grads, n_grads = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
     rates = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
     if max_grad_norm is None:
         _adam_launches(records, len(params), rates, device)
+        increment_version(params)
         return None
     max_grad_norm = _limit(max_grad_norm)
-    parts, count = _norm_of(of_grads, len(params), device)
+    parts, count = _norm_of(of_grads, n_grads, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, len(params), _address(records), *rates, parts.data_ptr(),
            count, max_grad_norm, norm.data_ptr())
+    increment_version(params)
     return norm
 
 
@@ -206,11 +231,11 @@ class Adam(torch.optim.Optimizer):
             device = work[0][1][0].device
             require_gpu(device)
             grads = [g for w in work for g in w[2]]
-            parts, count = _norm_of(_grad_records(grads, device), len(grads), device)
+            parts, count = _norm_of(*_grad_records(grads, device), device)
             self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
         for group, live, grads, ms, vs in work:
             dev = live[0].device
-            records, _ = _adam_records(live, grads, ms, vs, dev)
+            records, _, _ = _adam_records(live, grads, ms, vs, dev)
             rates = (float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                      float(group["weight_decay"]), int(group["step"]))
             if max_norm is not None:

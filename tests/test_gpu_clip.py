@@ -244,3 +244,51 @@ def test_refusals_on_the_device():
         adam_step_([z], [z], [z], [z[:3]], 1, max_grad_norm=1.0)
     with pytest.raises(ValueError):
         adam_step_([z], [], [z], [z], 1)
+
+
+def test_gradients_that_share_memory():
+    """Counted and scaled once, by whatever tensors the memory is met; an overlap from the same element on is refused."""
+    from sparc_amd.optim import adam_step_, clip_grad_norm_
+    flat = torch.full((70_000,), 2.0, device="cuda")
+    ps = params_of([flat, flat.view(700, 100), flat.view(100, 700).t()])
+    want = norm64([flat])
+    coef = np.float32(3.0 / (want + 1e-6))
+    assert abs(float(clip_grad_norm_(ps, 3.0)) - want) <= SLACK * U * want
+    assert bool((flat == 2.0 * coef).all())
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params_of([flat, flat[:5]]), 1.0)
+    empty = [torch.zeros(0, device="cuda") for _ in range(3)]
+    assert float(clip_grad_norm_(params_of(empty), 1.0)) == 0.0
+    assert float(clip_grad_norm_(params_of([*empty, torch.full((4,), 3.0, device="cuda")]), 100.0)) == 6.0
+    new = lambda: [torch.ones(33, device="cuda") for _ in range(2)]  # noqa: E731
+    g = torch.full((33,), 5.0, device="cuda")
+    p, m, v = new(), new(), new()
+    norm = adam_step_(p, [g, g], m, v, 1, max_grad_norm=1.0)
+    assert abs(float(norm) - 5.0 * math.sqrt(33.0)) <= SLACK * U * 5.0 * math.sqrt(33.0)
+    p1, m1, v1 = (t[:1] for t in (new(), new(), new()))
+    adam_step_(p1, [g], m1, v1, 1, max_grad_norm=1.0)
+    assert torch.equal(p[0], p1[0]) and torch.equal(p[1], p1[0]) and torch.equal(v[1], v1[0])
+    t = new()
+    for bad in (([t[0], t[0]], new(), new(), new()), (new(), new(), [t[0], t[0]], new()), (new(), new(), [t[0], t[1]], [t[1], new()[0]]),
+                ([t[0]], [t[0]], new()[:1], new()[:1])):
+        with pytest.raises(ValueError):
+            adam_step_(*bad, 1)
+
+
+def test_what_is_written_counts_as_written():
+    """Autograd refuses to go back through values that a step or a clipping has replaced."""
+    from sparc_amd.optim import adam_step_, clip_grad_norm_
+    p = torch.randn(50, device="cuda", generator=gen(3)).requires_grad_()
+    state = [torch.zeros(50, device="cuda") for _ in range(3)]
+    for limit in (None, 1.0):
+        loss = (p * p).sum()
+        adam_step_([p], state[:1], state[1:2], state[2:], 1, max_grad_norm=limit)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
+    loss = (p ** 3).sum()
+    loss.backward(create_graph=True)
+    penalty = (p.grad * p.grad).sum()
+    clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        penalty.backward()
+    p.grad = None
