@@ -731,15 +731,22 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
 }
 
 template <int DT, int VE>
-int launch_lookup(const LookupArgs& a, sparc_stream_t stream) {
+int launch_lookup(LookupArgs a, sparc_stream_t stream) {
+    typedef typename Elem<DT>::type T;
     int slices;
     const int lanes_log2 = lanes_for(ceil_div(a.dim, VE), &slices);
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.n, static_cast<int64_t>(BLOCK >> lanes_log2) * TURNS)), static_cast<unsigned>(slices));
-    if (a.n * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > SPARC_KEEP_BYTES)
-        hipLaunchKernelGGL((lookup_kernel<DT, VE, true>), grid, dim3(BLOCK), 0, stream, a, lanes_log2);
-    else
-        hipLaunchKernelGGL((lookup_kernel<DT, VE, false>), grid, dim3(BLOCK), 0, stream, a, lanes_log2);
-    SPARC_CHECK_LAUNCH();
+    const bool streaming = a.n * a.dim * static_cast<int64_t>(sizeof(T)) > SPARC_KEEP_BYTES;
+    const int64_t rows_of_block = static_cast<int64_t>(BLOCK >> lanes_log2) * TURNS;
+    const int64_t most = static_cast<int64_t>(UINT32_MAX / BLOCK) * rows_of_block;   // a launch has fewer than 2^32 threads along x
+    for (int64_t left = a.n; left > 0; left -= most) {
+        a.n = left < most ? left : most;
+        const dim3 grid(static_cast<unsigned>(ceil_div(a.n, rows_of_block)), static_cast<unsigned>(slices));
+        if (streaming) hipLaunchKernelGGL((lookup_kernel<DT, VE, true>), grid, dim3(BLOCK), 0, stream, a, lanes_log2);
+        else hipLaunchKernelGGL((lookup_kernel<DT, VE, false>), grid, dim3(BLOCK), 0, stream, a, lanes_log2);
+        SPARC_CHECK_LAUNCH();
+        a.ids = static_cast<const char*>(a.ids) + a.n * (a.wide_ids ? 8 : 4);
+        a.out = static_cast<T*>(a.out) + a.n * a.ldo;
+    }
     return SPARC_OK;
 }
 

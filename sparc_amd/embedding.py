@@ -11,7 +11,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from ._lib import lib
-from .graph import launch, require_gpu
+from .graph import _raw_stream, launch, require_gpu
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SPARC_F32, SPARC_BF16, SPARC_F16
 _ID_DTYPES = {torch.int32: 0, torch.int64: 1}
@@ -91,6 +91,11 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
     return out
 
 
+# A leaf's node in the autograd graph lives as long as any graph that it is in and keeps the stream that was current when it
+# was made: written down there by the first lookup.
+_BORN_ON = "sparc_amd.stream"
+
+
 class EmbeddingLookup(torch.autograd.Function):
     """Arguments ids, table, scale, padding_idx; gradient for the table."""
 
@@ -105,6 +110,11 @@ class EmbeddingLookup(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
+        leaf = ctx.next_functions[1][0]
+        if leaf.metadata.get(_BORN_ON) == 0 and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("embedding_lookup: a backward is being captured while the graph of an earlier lookup in the same "
+                               "table, made on the default stream, is alive: autograd would have that stream, which cannot be "
+                               "captured, wait for the capture. Drop what holds it (its outputs, its loss) before capturing")
         return None, embedding_grad(ids, g, ctx.rows, ctx.scale, ctx.padding_idx), None, None
 
 
@@ -116,7 +126,10 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     if padding_idx is not None:
         _padding(padding_idx, table.shape[0])
     if table.requires_grad and torch.is_grad_enabled():
-        return EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
+        out = EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
+        if table.is_leaf:
+            out.grad_fn.next_functions[1][0].metadata.setdefault(_BORN_ON, _raw_stream(table.device.index))
+        return out
     return _lookup(ids, table, float(scale))
 
 

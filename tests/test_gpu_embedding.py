@@ -298,3 +298,46 @@ def test_refusals_on_the_device():
                 lambda: embedding_grad(ids, table[:3], -1), lambda: NodeTable(0, 3), lambda: NodeTable(3, 3, padding_idx=3)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_capture_beside_a_living_eager_graph_is_refused():
+    """The earlier graph's leaf keeps the default stream, which no capture may make wait; without it the capture works."""
+    from sparc_amd.embedding import embedding_grad, embedding_lookup
+    table = torch.randn(300, 24, device="cuda", generator=gen(70), requires_grad=True)
+    ids, w = make_ids("zipf", 1000, 300, 71), torch.randn(1000, 24, device="cuda", generator=gen(72))
+    want = embedding_grad(ids, w, 300)
+    eager = embedding_lookup(ids, table)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="is alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            embedding_lookup(ids, table).backward(w)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):                # a forward alone is no matter
+        embedding_lookup(ids, table)
+    eager.backward(w)
+    assert torch.equal(table.grad, want)
+    del eager
+    table.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        embedding_lookup(ids, table).backward(w)
+    for turn in range(3):
+        w.copy_(torch.randn(w.shape, device="cuda", generator=gen(73 + turn)))
+        graph.replay()
+        assert torch.equal(table.grad, embedding_grad(ids, w, 300))
+        torch.cuda.synchronize()
+
+
+def test_lookup_of_more_rows_than_one_launch_takes():
+    """A launch has fewer than 2^32 threads along x: 268435440 rows of 33 vectors."""
+    from sparc_amd.embedding import embedding_lookup
+    n, rows, dim, one = 268_500_000, 1000, 264, 268_435_440
+    if torch.cuda.mem_get_info()[0] < 160e9:
+        pytest.skip("142 GB of output")
+    table = torch.randn(rows, dim, device="cuda", generator=gen(80)).bfloat16()
+    ids = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(997)
+    out = embedding_lookup(ids, table)
+    for a in (0, one // 2, one - 50_000, n - 20_000):
+        assert torch.equal(out[a:a + 100_000], table[ids[a:a + 100_000].long()]), a
+    del out, ids
+    torch.cuda.empty_cache()
