@@ -458,6 +458,7 @@ int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr
  *                            word written before the call returns; parts: the query's bytes, 8-byte aligned.
  *   sparc_clip_grad_norm     the same, then g <- c g, rounded to nearest, in place, and *norm_out = N (one device float)
  *   sparc_adam_step_clipped  sparc_adam_step on c g (the gradients themselves stay), any number of tensors, and *norm_out
+ *   sparc_clip_adam_step     the same with c of these tensors' own gradients, each counted (parts as in sparc_grad_norm)
  * Whoever scales adds the partial sums up itself, in a fixed order. */
 #define SPARC_F32 0
 #define SPARC_BF16 1
@@ -477,6 +478,9 @@ int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, 
 int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
                             double eps, double weight_decay, int64_t step, const double* parts, int64_t n_parts,
                             double max_norm, float* norm_out, sparc_stream_t stream);
+int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
+                         double eps, double weight_decay, int64_t step, double max_norm, double* parts, size_t parts_bytes,
+                         float* norm_out, sparc_stream_t stream);
 
 /* ---- table lookup by token, and its gradient ----------------------------------------------
  * For node features that are categories or node numbers: the reference's model starts at a float matrix

@@ -96,6 +96,7 @@ _SIGS = {
     "sparc_clip_grad_norm": (c_int, [c_int64, P, c_double, P, c_size_t, P, P]),
     "sparc_adam_step_clipped": (c_int, [c_int64, P, c_double, c_double, c_double, c_double, c_double, c_int64, P, c_int64, c_double,
                                         P, P]),
+    "sparc_clip_adam_step": (c_int, [c_int64, P, c_double, c_double, c_double, c_double, c_double, c_int64, c_double, P, c_size_t, P, P]),
     "sparc_embedding_fwd": (c_int, [c_int64, c_int64, c_int64, c_int, P, c_int, P, c_int64, c_double, P, c_int64, P]),
     "sparc_embedding_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
     "sparc_embedding_grad": (c_int, [c_int64, c_int64, c_int64, c_int, P, c_int, P, c_int64, c_double, c_int64, P, P, c_size_t, P]),

@@ -14,7 +14,7 @@
 // plainly for the scaling, which goes backwards: 94 and 205 us.  Lists below 192 MB stay plain: 160 MB, three lists in turn, 80 us
 // streamed, 93 us plain; one list again and again 80 and 72 us.
 // 6.4 MB (the MLP alone): 4.0 + 6.0 us, of which launches and the chain parts -> sum -> root -> quotient are most; the
-// host's two launches and checks take longer (16.7 us a call).
+// host's two launches and checks take longer (16.0 us a call).
 // Adam on 31.5 M floats (883 MB): norm 24 us, update 136 us = 6.5 TB/s; plain accesses 40 and 160 us.  Below 192 MB plain:
 // 8 M floats 49.1 us streamed, 49.7 us plain; 4 M 27.8 and 25.1.
 #include "elem.h"
@@ -325,45 +325,42 @@ bool grads_ok(const int64_t n_tensors, const sparc_grad_tensor_t* t) {
 
 int64_t bytes_of(const sparc_grad_tensor_t& t) { return t.n * (t.dtype == SPARC_F32 ? 4 : 2); }
 
-// The first `count` tensors of t as kernel arguments.  Their number of blocks stays below 2^30 (SPARC_GRAD_MAX_ELEMS).
-// left: bytes of the list from t on.
-void fill(GradArgs& a, const sparc_grad_tensor_t* t, const int count, const int block_bytes, const int64_t left) {
+// The `count` tensors t(from), t(from + 1) ... as kernel arguments.  Their number of blocks stays below 2^30
+// (SPARC_GRAD_MAX_ELEMS).  left: bytes of the list from there on.  Returns these tensors' bytes.
+template <typename F>
+int64_t fill(GradArgs& a, F&& t, const int64_t from, const int count, const int block_bytes, const int64_t left) {
     int64_t blocks = 0, bytes = 0;
     for (int i = 0; i < SPARC_GRAD_MAX_TENSORS; ++i) {
-        const bool real = i < count;
-        a.p[i] = real ? t[i].p : nullptr;
-        a.n_dtype[i] = real ? t[i].n << 2 | t[i].dtype : 0;
-        a.first_block[i] = real ? static_cast<int32_t>(blocks) : INT32_MAX;
-        if (!real) continue;
-        bytes += bytes_of(t[i]);
-        blocks += (bytes_of(t[i]) + block_bytes - 1) / block_bytes;
+        const sparc_grad_tensor_t r = i < count ? t(from + i) : sparc_grad_tensor_t{nullptr, 0, 0};
+        a.p[i] = r.p;
+        a.n_dtype[i] = r.n << 2 | r.dtype;
+        a.first_block[i] = i < count ? static_cast<int32_t>(blocks) : INT32_MAX;
+        bytes += bytes_of(r);
+        blocks += (bytes_of(r) + block_bytes - 1) / block_bytes;
     }
     a.blocks = static_cast<int>(blocks);
     const int64_t keep = KEEP_BYTES - (left - bytes);   // of these tensors' bytes
     const int64_t plain = keep <= 0 ? 0 : keep / block_bytes;
     a.plain_from = static_cast<int>(keep >= bytes || plain >= blocks ? 0 : blocks - plain);
+    return bytes;
 }
 
-}  // namespace
-
-extern "C" size_t sparc_grad_norm_workspace_bytes(int64_t n_tensors) {
-    if (n_tensors < 0) return 0;
+size_t parts_bytes_of(const int64_t n_tensors) {
     const int64_t launches = (n_tensors + SPARC_GRAD_MAX_TENSORS - 1) / SPARC_GRAD_MAX_TENSORS;
     return static_cast<size_t>(launches > 0 ? launches : 1) * PARTS * sizeof(double);
 }
 
-extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double* parts, size_t parts_bytes,
-                               int64_t* n_parts, sparc_stream_t stream) {
-    if (!parts || !n_parts || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
-    if (parts_bytes < sparc_grad_norm_workspace_bytes(n_tensors) || (reinterpret_cast<uintptr_t>(parts) & 7)) return SPARC_ERR_WS;
+// The partial sums of the tensors t(0) ... t(n_tensors - 1), checked by the caller.
+template <typename F>
+int launch_norm(const int64_t n_tensors, F&& t, double* parts, const size_t parts_bytes, int64_t* n_parts, sparc_stream_t stream) {
+    if (parts_bytes < parts_bytes_of(n_tensors) || (reinterpret_cast<uintptr_t>(parts) & 7)) return SPARC_ERR_WS;
     int64_t total = 0, left = 0;
     int launches = 0;
-    for (int64_t i = 0; i < n_tensors; ++i) left += bytes_of(tensors[i]);
+    for (int64_t i = 0; i < n_tensors; ++i) left += bytes_of(t(i));
     for (int64_t from = 0; from < n_tensors; from += SPARC_GRAD_MAX_TENSORS) {
         GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
-        fill(a, tensors + from, count, NORM_BYTES, left);
-        for (int i = 0; i < count; ++i) left -= bytes_of(tensors[from + i]);
+        left -= fill(a, t, from, count, NORM_BYTES, left);
         if (a.blocks == 0) continue;
         const int grid = a.blocks < PARTS ? a.blocks : PARTS;
         hipLaunchKernelGGL(grad_squares_kernel, dim3(grid), dim3(NORM_THREADS), 0, stream, a, parts + total);
@@ -380,6 +377,61 @@ extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* ten
     return SPARC_OK;
 }
 
+struct AdamRates {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;
+};
+
+bool adam_ok(const int64_t n_tensors, const sparc_adam_tensor_t* t, const AdamRates& r) {
+    if (n_tensors < 0 || (n_tensors > 0 && !t) || r.step < 1 || !(r.beta1 >= 0.0 && r.beta1 < 1.0) || !(r.beta2 >= 0.0 && r.beta2 < 1.0) ||
+        !(r.eps >= 0.0))
+        return false;
+    for (int64_t i = 0; i < n_tensors; ++i)
+        if (t[i].n < 0 || t[i].n > SPARC_GRAD_MAX_ELEMS || (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v))) return false;
+    return true;
+}
+
+int launch_adam(const int64_t n_tensors, const sparc_adam_tensor_t* tensors, const AdamRates& r, Clip c, sparc_stream_t stream) {
+    int64_t all = 0;
+    for (int64_t i = 0; i < n_tensors; ++i) all += tensors[i].n;
+    const double bc1 = 1.0 - pow(r.beta1, static_cast<double>(r.step)), bc2 = 1.0 - pow(r.beta2, static_cast<double>(r.step));
+    for (int64_t from = 0; from < n_tensors || from == 0; from += ADAM_MOST) {
+        AdamClipArgs a;
+        int64_t blocks = 0;   // below 2^30
+        for (int i = 0; i < ADAM_MOST; ++i) {
+            const bool real = from + i < n_tensors;
+            a.t[i] = real ? tensors[from + i] : sparc_adam_tensor_t{};
+            a.first_block[i] = real ? static_cast<int32_t>(blocks) : INT32_MAX;
+            blocks += (a.t[i].n + ADAM_ELEMS - 1) / ADAM_ELEMS;
+        }
+        a.blocks = static_cast<int>(blocks);
+        a.step_size = static_cast<float>(r.lr / bc1);
+        a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
+        a.beta2 = static_cast<float>(r.beta2);
+        a.one_minus_beta1 = static_cast<float>(1.0 - r.beta1);
+        a.one_minus_beta2 = static_cast<float>(1.0 - r.beta2);
+        a.eps = static_cast<float>(r.eps);
+        a.weight_decay = static_cast<float>(r.weight_decay);
+        if (blocks == 0 && !c.norm_out) continue;
+        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
+        if (16 * all > KEEP_BYTES) hipLaunchKernelGGL(adam_clip_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
+        else hipLaunchKernelGGL(adam_clip_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
+        SPARC_CHECK_LAUNCH();
+        c.norm_out = nullptr;
+    }
+    return SPARC_OK;
+}
+
+}  // namespace
+
+extern "C" size_t sparc_grad_norm_workspace_bytes(int64_t n_tensors) { return n_tensors < 0 ? 0 : parts_bytes_of(n_tensors); }
+
+extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double* parts, size_t parts_bytes,
+                               int64_t* n_parts, sparc_stream_t stream) {
+    if (!parts || !n_parts || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
+    return launch_norm(n_tensors, [&](int64_t i) { return tensors[i]; }, parts, parts_bytes, n_parts, stream);
+}
+
 extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double max_norm, double* parts,
                                     size_t parts_bytes, float* norm_out, sparc_stream_t stream) {
     if (!norm_out || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
@@ -394,7 +446,7 @@ extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t
         GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
         for (int k = 0; k < count; ++k) left += bytes_of(tensors[from + k]);
-        fill(a, tensors + from, count, BLOCK_BYTES, left);
+        fill(a, [&](int64_t k) { return tensors[k]; }, from, count, BLOCK_BYTES, left);
         if (a.blocks == 0 && !c.norm_out) continue;
         const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
         if (a.plain_from > 0) hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
@@ -408,40 +460,19 @@ extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t
 extern "C" int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
                                        double eps, double weight_decay, int64_t step, const double* parts, int64_t n_parts,
                                        double max_norm, float* norm_out, sparc_stream_t stream) {
-    if (n_tensors < 0 || (n_tensors > 0 && !tensors) || step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) ||
-        !(eps >= 0.0) || !parts || !norm_out || n_parts < 0 || n_parts > PARTS || !(max_norm >= 0.0))
-        return SPARC_ERR_ARG;
-    int64_t all = 0;
-    for (int64_t i = 0; i < n_tensors; ++i) {
-        const sparc_adam_tensor_t& t = tensors[i];
-        if (t.n < 0 || t.n > SPARC_GRAD_MAX_ELEMS || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v))) return SPARC_ERR_ARG;
-        all += t.n;
-    }
-    const double bc1 = 1.0 - pow(beta1, static_cast<double>(step)), bc2 = 1.0 - pow(beta2, static_cast<double>(step));
-    Clip c = {parts, norm_out, max_norm, static_cast<int>(n_parts)};
-    for (int64_t from = 0; from < n_tensors || from == 0; from += ADAM_MOST) {
-        AdamClipArgs a;
-        int64_t blocks = 0;   // below 2^30
-        for (int i = 0; i < ADAM_MOST; ++i) {
-            const bool real = from + i < n_tensors;
-            a.t[i] = real ? tensors[from + i] : sparc_adam_tensor_t{};
-            a.first_block[i] = real ? static_cast<int32_t>(blocks) : INT32_MAX;
-            blocks += (a.t[i].n + ADAM_ELEMS - 1) / ADAM_ELEMS;
-        }
-        a.blocks = static_cast<int>(blocks);
-        a.step_size = static_cast<float>(lr / bc1);
-        a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
-        a.beta2 = static_cast<float>(beta2);
-        a.one_minus_beta1 = static_cast<float>(1.0 - beta1);
-        a.one_minus_beta2 = static_cast<float>(1.0 - beta2);
-        a.eps = static_cast<float>(eps);
-        a.weight_decay = static_cast<float>(weight_decay);
-        if (blocks == 0 && !c.norm_out) continue;
-        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
-        if (16 * all > KEEP_BYTES) hipLaunchKernelGGL(adam_clip_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
-        else hipLaunchKernelGGL(adam_clip_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
-        SPARC_CHECK_LAUNCH();
-        c.norm_out = nullptr;
-    }
-    return SPARC_OK;
+    const AdamRates rates = {lr, beta1, beta2, eps, weight_decay, step};
+    if (!adam_ok(n_tensors, tensors, rates) || !parts || !norm_out || n_parts < 0 || n_parts > PARTS || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
+    return launch_adam(n_tensors, tensors, rates, Clip{parts, norm_out, max_norm, static_cast<int>(n_parts)}, stream);
+}
+
+extern "C" int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
+                                    double eps, double weight_decay, int64_t step, double max_norm, double* parts,
+                                    size_t parts_bytes, float* norm_out, sparc_stream_t stream) {
+    const AdamRates rates = {lr, beta1, beta2, eps, weight_decay, step};
+    if (!adam_ok(n_tensors, tensors, rates) || !parts || !norm_out || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
+    int64_t n_parts = 0;
+    auto gradient = [&](int64_t i) { return sparc_grad_tensor_t{const_cast<float*>(tensors[i].g), tensors[i].n, SPARC_F32}; };
+    const int rc = launch_norm(n_tensors, gradient, parts, parts_bytes, &n_parts, stream);
+    if (rc != SPARC_OK) return rc;
+    return launch_adam(n_tensors, tensors, rates, Clip{parts, norm_out, max_norm, static_cast<int>(n_parts)}, stream);
 }

@@ -67,10 +67,10 @@ def _each_once(at, sizes, codes):
 
 def _records(*columns):
     """One int64 array of the columns' entries, record by record."""
-    out = array("q", bytes(8 * len(columns) * len(columns[0])))
+    out = [0] * (len(columns) * len(columns[0]))
     for i, column in enumerate(columns):
-        out[i::len(columns)] = array("q", column)
-    return out
+        out[i::len(columns)] = column
+    return array("q", out)
 
 
 def _norm_of(records, n, device):
@@ -121,20 +121,20 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 
 
 def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
-    """(records of the update, records of the gradients, how many of those)."""
+    """(records of the update as the C calls take them; None, or, where parameters share gradients, these once)."""
     n = len(params)
     every = [*params, *grads, *exp_avgs, *exp_avg_sqs]
     sizes = list(map(_size_of, every))
     if set(map(_type_of, every)) != {torch.float32} or not _dense_on(every, device) or sizes != sizes[:n] * 4:
         raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
     at = list(map(_address_of, every))
-    of_grads = (at[n:2 * n], sizes[:n], [0] * n)
+    once = None
     if len(set(at)) < 4 * n:   # empty tensors, or a gradient that several parameters share: nothing else may occur twice
         full = [a for a, size in zip(at, sizes) if size]
-        of_grads = _each_once(*of_grads)
-        if len(set(full)) < len(full) // 4 * 3 + len(of_grads[0]):
+        once = _each_once(at[n:2 * n], sizes[:n], [0] * n)
+        if len(set(full)) < len(full) // 4 * 3 + len(once[0]):
             raise ValueError("an Adam step writes every parameter and moment once")
-    return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), _records(*of_grads), len(of_grads[0])
+    return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), once
 
 
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -151,18 +151,29 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     device = params[0].device
     if not params[0].is_cuda:
         require_gpu(device)
-    records, of_grads, n_grads = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
+    records, once = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
     rates = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
     if max_grad_norm is None:
         _adam_launches(records, len(params), rates, device)
         increment_version(params)
         return None
-    max_grad_norm = _limit(max_grad_norm)
-    parts, count = _norm_of(of_grads, n_grads, device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, len(params), _address(records), *rates, parts.data_ptr(),
-           count, max_grad_norm, norm.data_ptr())
+    norm = _clipped_step(records, once, len(params), rates, _limit(max_grad_norm), device)
     increment_version(params)
+    return norm
+
+
+def _clipped_step(records, once, n, rates, max_norm, device):
+    """The update of n records by their own gradients' norm, which is returned."""
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    if once is not None:
+        parts, count = _norm_of(_records(*once), len(once[0]), device)
+        launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, device, n, _address(records), *rates, parts.data_ptr(), count,
+               max_norm, norm.data_ptr())
+        return norm
+    nbytes = lib.sparc_grad_norm_workspace_bytes(n)
+    parts = torch.empty(nbytes >> 3, dtype=torch.float64, device=device)
+    launch("sparc_clip_adam_step", lib.sparc_clip_adam_step, device, n, _address(records), *rates, max_norm, parts.data_ptr(), nbytes,
+           norm.data_ptr())
     return norm
 
 
@@ -227,20 +238,21 @@ class Adam(torch.optim.Optimizer):
             work.append((group, live, grads, ms, vs))
         if not work:
             return loss
-        if max_norm is not None:
+        if max_norm is not None and len(work) > 1:   # the norm over all groups
             device = work[0][1][0].device
             require_gpu(device)
-            grads = [g for w in work for g in w[2]]
-            parts, count = _norm_of(*_grad_records(grads, device), device)
+            parts, count = _norm_of(*_grad_records([g for w in work for g in w[2]], device), device)
             self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
         for group, live, grads, ms, vs in work:
             dev = live[0].device
-            records, _, _ = _adam_records(live, grads, ms, vs, dev)
+            records, once = _adam_records(live, grads, ms, vs, dev)
             rates = (float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                      float(group["weight_decay"]), int(group["step"]))
-            if max_norm is not None:
+            if max_norm is None:
+                _adam_launches(records, len(live), rates, dev)
+            elif len(work) == 1:
+                self.grad_norm = _clipped_step(records, once, len(live), rates, max_norm, dev)
+            else:
                 launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, dev, len(live), _address(records), *rates,
                        parts.data_ptr(), count, max_norm, self.grad_norm.data_ptr())
-            else:
-                _adam_launches(records, len(live), rates, dev)
         return loss

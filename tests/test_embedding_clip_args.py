@@ -94,3 +94,15 @@ def test_trainer_configuration():
     tr._setup_model(12)
     with pytest.raises(ValueError):
         tr._setup_optimizer(False)
+
+
+def test_clipping_step_arguments():
+    from sparc_amd._lib import lib
+    rec = (ctypes.c_int64 * 5)(P, P, P, P, 100)
+    step = lambda n=1, t=rec, b1=0.9, b2=0.999, eps=1e-8, step=1, limit=1.0, parts=P, nbytes=1 << 20, out=P: lib.sparc_clip_adam_step(  # noqa: E731
+        n, t, 1e-3, b1, b2, eps, 0.0, step, limit, parts, nbytes, out, None)
+    for bad in (dict(n=-1), dict(t=None), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(step=0), dict(parts=None), dict(limit=-2.0),
+                dict(limit=float("nan")), dict(out=None), dict(t=(ctypes.c_int64 * 5)(P, 0, P, P, 4)),
+                dict(t=(ctypes.c_int64 * 5)(P, P, P, P, -4)), dict(t=(ctypes.c_int64 * 5)(P, P, P, P, (1 << 34) + 1))):
+        assert step(**bad) == -1, bad
+    assert step(nbytes=8) == -2 and step(parts=P + 4) == -2
