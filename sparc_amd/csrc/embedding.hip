@@ -503,23 +503,33 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
 // ---- gradient of few tokens: one launch ------------------------------------------------------------------
 
 // Up to FEW tokens a workgroup can look through all of them itself: it writes the zeros of its rows, collects their places
-// as keys {row, place} (in any order), sorts the keys and adds up the runs.  No workspace, one launch instead of six
-// dependent ones.  The rows are dealt out in turn, in groups of at least GROUP_BYTES, because frequent tokens are often
-// neighbours (8192 tokens, frequent first: 26 us; dealt out in stretches 156 us, sorted 40 us).
-// 2437 tokens over 2708 rows of 64 floats: 6.8 us, the call 9.0 (the sort: 26); 8192 over 50000: 10.7 (29).  Bound by its
-// chain of tokens -> keys -> rows -> stores.  The price is the call whose tokens are all the same: one workgroup adds them
-// up, 8192 rows of 64 floats take 145 us (the sort: 36), 4096 of 512 bfloat16 178 (42).
+// as keys {row, place}, sorts the keys by row and adds up the runs.  No workspace, one launch instead of six dependent
+// ones.  The rows are dealt out in turn, in groups of at least GROUP_BYTES, because frequent tokens are often neighbours.
+// A workgroup may get all tokens as well as none: the keys are collected in an order fixed by the tokens, so that a radix
+// sort of the row alone will do, and dealt to the workers in equal shares, of which one long run has many.
+//
+// Measured, a call in us for uniform tokens, frequent first, all the same: 2437 tokens over 2708 rows of 64 floats 8.9, 11.2,
+// 21 (the sort takes 26 for the first); 8192 over 50000 rows of 64 floats 11.7, 16.3, 57 (9000 tokens by the sort: 30, 40, 38);
+// 8192 of 512 floats 27, 33, 76 (by the sort 40, 49, 55), of 2048 floats 100, 108, 201 (105, 110, 113): beyond 16 MiB of
+// gradient the sort.  Bound by the chain tokens -> keys -> rows -> stores, and where all tokens are the same by what one CU
+// reads, 45 GB/s; hence workers of at most 16 lanes, so that wider rows have several workgroups: 4096 of 512 bfloat16 all the
+// same 111 -> 44 us, uniform 14.4 -> 15.2; 8 lanes 33 and 16.2.  FEW_LONG 16, 32: frequent first 17.3, 17.7; FEW_AHEAD 4, 16:
+// all the same 66, 54, uniform 11.7, 12.6.  With a bitonic sort of all keys and long runs one by one: 8192 tokens over 300
+// rows of one float, frequent first, 306 us, now 20.
 constexpr int FEW = 8192, PLACE_BITS = 13;
-constexpr int64_t FEW_BYTES = 4 << 20;   // of gradient: one workgroup adds it up alone where all tokens are the same
-constexpr int FEW_THREADS = 512;
+constexpr int64_t FEW_BYTES = 16 << 20;   // of gradient
+constexpr int FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES;
+constexpr int FEW_TOKENS = FEW / FEW_THREADS;   // of a thread
 constexpr int FEW_BLOCKS_LOG2 = 9;   // workgroups that the rows are dealt to
 constexpr int FEW_AHEAD = 8;         // gradient rows in flight per worker
-constexpr int FEW_TURNS = 4;         // 16-byte vectors of tokens in flight per thread
-constexpr int GROUP_BYTES = 256;
+constexpr int FEW_LONG = 8;         // places of the longest run that is one worker's
+constexpr int FEW_BITS = 8;          // of a digit of the radix sort
+constexpr int FEW_LANES_LOG2 = 4;    // of a worker at most: slices of 256 bytes
+constexpr int GROUP_BYTES = 16 << FEW_LANES_LOG2;   // (rows narrower than that are one slice)
 
 // Row r belongs to workgroup (r >> group) mod 2^blocks, where it is row local(r).
 struct Dealt {
-    int group, blocks;
+    int group, blocks, bits;   // bits: of a local row
     __device__ __forceinline__ uint32_t block_of(const uint32_t r) const { return (r >> group) & ((1u << blocks) - 1u); }
     __device__ __forceinline__ uint32_t local(const uint32_t r) const {
         return (r >> group >> blocks) << group | (r & ((1u << group) - 1u));
@@ -529,41 +539,153 @@ struct Dealt {
     }
 };
 
+// The keys of this workgroup's tokens, in the order of (wave, turn, element, lane), whatever the type; returns how many.
 template <typename ID>
-__device__ __forceinline__ void collect_rows(const ID* ids, const int n, const int64_t rows, const int64_t padding, const Dealt dealt,
-                                             uint32_t* keys, uint32_t* count) {
-    constexpr int VE = 16 / sizeof(ID);
+__device__ __forceinline__ int collect_rows(const ID* ids, const int n, const int64_t rows, const int64_t padding, const Dealt dealt,
+                                            uint32_t* keys, uint32_t* found) {
+    constexpr int VE = 4, TURNS = FEW_TOKENS / VE;
     typedef ID mem __attribute__((ext_vector_type(VE), aligned(sizeof(ID))));
-    const int lane = threadIdx.x & 63;
-    for (int i0 = 0; i0 < n; i0 += FEW_THREADS * VE * FEW_TURNS) {
-        mem v[FEW_TURNS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto place = [](const int k, const int c) { return (k * FEW_THREADS + static_cast<int>(threadIdx.x)) * VE + c; };
+    mem v[TURNS];
 #pragma unroll
-        for (int k = 0; k < FEW_TURNS; ++k) {
-            const int i = i0 + (k * FEW_THREADS + static_cast<int>(threadIdx.x)) * VE;
-            if (i + VE <= n) {
-                v[k] = *reinterpret_cast<const mem*>(ids + i);
-            } else {
+    for (int k = 0; k < TURNS; ++k) {
+        if (k * FEW_THREADS * VE >= n) break;
+        const int i = place(k, 0);
+        if (i + VE <= n) {
+            v[k] = *reinterpret_cast<const mem*>(ids + i);
+        } else {
 #pragma unroll
-                for (int c = 0; c < VE; ++c) v[k][c] = i + c < n ? ids[i + c] : static_cast<ID>(-1);
-            }
+            for (int c = 0; c < VE; ++c) v[k][c] = i + c < n ? ids[i + c] : static_cast<ID>(-1);
         }
+    }
+    uint32_t hits = 0;
+    int count = 0;
 #pragma unroll
-        for (int k = 0; k < FEW_TURNS; ++k)
+    for (int k = 0; k < TURNS; ++k) {
+        if (k * FEW_THREADS * VE >= n) break;
+#pragma unroll
+        for (int c = 0; c < VE; ++c) {
+            const int64_t id = v[k][c];
+            const bool hit = dealt.block_of(static_cast<uint32_t>(id)) == blockIdx.x && id >= 0 && id < rows && id != padding;
+            hits |= hit ? 1u << (k * VE + c) : 0u;
+            count += __popcll(__ballot(hit));
+        }
+    }
+    if (lane == 0) found[wave] = count;
+    __syncthreads();
+    int at = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w) {
+        if (w < wave) at += found[w];
+        total += found[w];
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (count > 0)
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            if (k * FEW_THREADS * VE >= n) break;
 #pragma unroll
             for (int c = 0; c < VE; ++c) {
-                const int64_t id = v[k][c];
-                const uint32_t row = static_cast<uint32_t>(id);
-                const bool hit = dealt.block_of(row) == blockIdx.x && id >= 0 && id < rows && id != padding;
-                const uint64_t hits = __ballot(hit);
-                if (hits == 0) continue;                 // (the whole wave, nearly always)
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(count, static_cast<uint32_t>(__popcll(hits)));
-                at = __builtin_amdgcn_readfirstlane(at);
-                if (hit) {
-                    const int i = i0 + (k * FEW_THREADS + static_cast<int>(threadIdx.x)) * VE + c;
-                    keys[at + __popcll(hits & ((1ull << lane) - 1ull))] = dealt.local(row) << PLACE_BITS | static_cast<uint32_t>(i);
-                }
+                const bool hit = hits >> (k * VE + c) & 1u;
+                const uint64_t here = __ballot(hit);
+                if (here == 0) continue;
+                if (hit)
+                    keys[at + __popcll(here & ((1ull << lane) - 1ull))] =
+                        dealt.local(static_cast<uint32_t>(v[k][c])) << PLACE_BITS | static_cast<uint32_t>(place(k, c));
+                at += __popcll(here);
             }
+        }
+    return total;
+}
+
+// By row and place, up to a key per thread: every key counts the smaller ones.  (Bitonic: 10 to 45 barriers.)
+__device__ __forceinline__ void rank_sort(uint32_t* keys, const int count) {
+    const int tid = threadIdx.x;
+    if (count <= 64) {
+        if (tid >= 64) return;
+        const uint32_t key = tid < count ? keys[tid] : ~0u;
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += __builtin_amdgcn_readlane(static_cast<int>(key), j) < static_cast<int>(key) ? 1 : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // read by all before any writes
+        if (tid < count) keys[rank] = key;
+        return;
+    }
+    const int fours = (count + 3) >> 2;
+    if (tid < 4 * fours - count) keys[count + tid] = ~0u;
+    __syncthreads();
+    const uint32_t key = tid < count ? keys[tid] : 0u;
+    uint32_t rank = 0;
+    if ((tid & ~63) < count)
+#pragma unroll 4
+        for (int j = 0; j < fours; ++j) {
+            const uint4 k = reinterpret_cast<const uint4*>(keys)[j];
+            rank += (k.x < key ? 1u : 0u) + (k.y < key ? 1u : 0u) + (k.z < key ? 1u : 0u) + (k.w < key ? 1u : 0u);
+        }
+    __syncthreads();
+    if (tid < count) keys[rank] = key;
+}
+
+// By row, keys of a row as they came.  cnt: [FEW_WAVES][1 << FEW_BITS], sums: [FEW_WAVES].
+__device__ __forceinline__ void radix_sort(uint32_t* keys, const int count, const int row_bits, uint16_t* cnt, uint32_t* sums) {
+    constexpr int DIGITS = 1 << FEW_BITS;
+    static_assert(DIGITS <= FEW_THREADS && FEW_BITS <= MOST_BITS, "a digit per thread");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int steps = (count + FEW_THREADS - 1) / FEW_THREADS;   // keys of a lane
+    const int from = wave * steps * 64 + lane;
+    uint16_t* own = cnt + wave * DIGITS;
+    for (int shift = PLACE_BITS; shift < PLACE_BITS + row_bits; shift += FEW_BITS) {
+        uint32_t e[FEW_TOKENS], at[FEW_TOKENS];   // at: rank among the wave's keys of the digit
+#pragma unroll
+        for (int k = 0; k < FEW_TOKENS; ++k)
+            if (k < steps) e[k] = from + k * 64 < count ? keys[from + k * 64] : 0u;
+        for (int i = tid; i < FEW_WAVES * DIGITS / 2; i += FEW_THREADS) reinterpret_cast<uint32_t*>(cnt)[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < FEW_TOKENS; ++k) {
+            if (k >= steps) break;
+            const bool ok = from + k * 64 < count;
+            const uint32_t digit = (e[k] >> shift) & (DIGITS - 1);
+            const uint64_t same = equals(digit, FEW_BITS, __ballot(ok));
+            const int r = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(same >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(same), 0u));
+            if (ok) {
+                const uint32_t c0 = own[digit];
+                at[k] = c0 + r;
+                if (r == 0) own[digit] = static_cast<uint16_t>(c0 + __popcll(same));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the counters as the next turn's lanes find them
+        }
+        __syncthreads();
+        uint32_t of_digit = 0, upto = 0;
+        if (tid < DIGITS) {
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; ++w) of_digit += cnt[w * DIGITS + tid];
+            upto = of_digit;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t below = __shfl_up(upto, off);
+                if (lane >= off) upto += below;
+            }
+            if (lane == 63) sums[wave] = upto;
+        }
+        __syncthreads();
+        if (tid < DIGITS) {
+            uint32_t run = upto - of_digit;
+#pragma unroll
+            for (int w = 0; w < DIGITS / 64; ++w)
+                if (w < wave) run += sums[w];
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; ++w) {
+                const uint32_t c0 = cnt[w * DIGITS + tid];
+                cnt[w * DIGITS + tid] = static_cast<uint16_t>(run);
+                run += c0;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < FEW_TOKENS; ++k)
+            if (k < steps && from + k * 64 < count) keys[own[(e[k] >> shift) & (DIGITS - 1)] + at[k]] = e[k];
+        __syncthreads();
     }
 }
 
@@ -571,14 +693,15 @@ template <int DT, int VE>
 __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const Dealt dealt, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t keys[];     // a power of two of them, at least n
-    __shared__ uint32_t total_found;
-    __shared__ float piece[FEW_THREADS * VE];
-    __shared__ uint32_t long_runs[FEW / LONG_ROW], n_long;
+    __shared__ uint32_t sums[FEW_WAVES];
+    // counters of the sort, then sums of the workers' pieces
+    __shared__ __align__(16) uint32_t shared[VE > 2 ? FEW_THREADS * VE : FEW_THREADS * 2];
+    static_assert(sizeof(shared) >= sizeof(uint16_t) * FEW_WAVES << FEW_BITS, "the sort's counters fit");
+    float* piece = reinterpret_cast<float*>(shared);
     const T* g = static_cast<const T*>(a.g);
     T* out = static_cast<T*>(a.out);
     const int tid = threadIdx.x;
     const int n = static_cast<int>(a.n);
-    if (tid == 0) n_long = total_found = 0;
     const int lanes = 1 << lanes_log2, workers = FEW_THREADS >> lanes_log2, worker = tid >> lanes_log2;
     const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + (tid & (lanes - 1));
     const bool mine = unit * VE < a.dim;
@@ -602,92 +725,109 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
         for (int64_t r = blockIdx.x + (static_cast<int64_t>(worker) << dealt.blocks); r < a.rows; r += static_cast<int64_t>(workers) << dealt.blocks)
             zero.store(out + r * a.dim + col);
     }
-    __syncthreads();
-    if (a.wide_ids) collect_rows(static_cast<const int64_t*>(a.ids), n, a.rows, a.padding, dealt, keys, &total_found);
-    else collect_rows(static_cast<const int32_t*>(a.ids), n, a.rows, a.padding, dealt, keys, &total_found);
-    __syncthreads();
-    const int count = static_cast<int>(total_found);
+    const int count = a.wide_ids ? collect_rows(static_cast<const int64_t*>(a.ids), n, a.rows, a.padding, dealt, keys, sums)
+                                 : collect_rows(static_cast<const int32_t*>(a.ids), n, a.rows, a.padding, dealt, keys, sums);
     if (count == 0) return;                              // (the whole workgroup)
-    int size = 1;
-    while (size < count) size <<= 1;
-    for (int i = count + tid; i < size; i += FEW_THREADS) keys[i] = 0xffffffffu;
     __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)                  // bitonic: the keys are distinct, so this is the order of the places
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = tid; i < size / 2; i += FEW_THREADS) {
-                const int x = ((i & ~(j - 1)) << 1) | (i & (j - 1)), y = x | j;
-                const uint32_t p = keys[x], q = keys[y];
-                if ((p > q) == ((x & k) == 0)) {
-                    keys[x] = q;
-                    keys[y] = p;
-                }
-            }
-            __syncthreads();
-        }
+    if (count <= FEW_THREADS) {
+        rank_sort(keys, count);
+    } else {
+        bool in_order = true;
+        for (int i = tid + 1; i < count; i += FEW_THREADS) in_order &= keys[i - 1] >> PLACE_BITS <= keys[i] >> PLACE_BITS;
+        if (!__syncthreads_and(in_order)) radix_sort(keys, count, dealt.bits, reinterpret_cast<uint16_t*>(shared), sums);
+    }
     __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0): the zeros have left before any wave writes sums over them
     __syncthreads();
-    auto same_row = [&](const int i, const uint32_t row) { return i < count && keys[i] >> PLACE_BITS == row; };
-    auto add = [&](float* acc, const int from, const int to) {   // keys [from, to)
-        for (int i = from; i < to; i += FEW_AHEAD) {
-            Vec<DT, VE> v[FEW_AHEAD];
-#pragma unroll
-            for (int k = 0; k < FEW_AHEAD; ++k)
-                if (i + k < to) v[k].load(g + static_cast<int64_t>(keys[i + k] & ((1 << PLACE_BITS) - 1)) * a.ldg + col);
-#pragma unroll
-            for (int k = 0; k < FEW_AHEAD; ++k)
-                if (i + k < to)
-#pragma unroll
-                    for (int c = 0; c < VE; ++c) acc[c] += v[k].get(c);
+    auto row_at = [&](const int i) { return keys[i] >> PLACE_BITS; };
+    // behind the last key of the run that key i is in (the keys up to `last` are looked at)
+    auto end_of = [&](const int i, int last) {
+        const uint32_t row = row_at(i);
+        int end = i + 1;
+        while (end < last) {
+            const int mid = (end + last) >> 1;
+            if (row_at(mid) == row) end = mid + 1;
+            else last = mid;
         }
+        return end;
     };
-    for (int i = worker; i < count; i += workers) {
-        const uint32_t row = keys[i] >> PLACE_BITS;
-        if (i > 0 && keys[i - 1] >> PLACE_BITS == row) continue;   // not the first of its run
-        if (same_row(i + LONG_ROW, row)) {
-            if ((tid & (lanes - 1)) == 0) long_runs[atomicAdd(&n_long, 1u)] = i;
-            continue;
+    // The workers' shares.  A run of at most FEW_LONG keys belongs to the worker that meets its first; a longer one is cut.
+    // Where does the run that is cut in front of key i end?  0: none is, -1: it is a long one.
+    auto cut = [&](const int i) {
+        if (i == 0 || i >= count || row_at(i - 1) != row_at(i)) return 0;
+        const uint32_t row = row_at(i);
+        int begin = max(i - FEW_LONG - 1, 0), here = i - 1;
+        while (begin < here) {
+            const int mid = (begin + here) >> 1;
+            if (row_at(mid) != row) begin = mid + 1;
+            else here = mid;
         }
-        if (!mine) continue;
-        int end = i + 1, behind = min(i + LONG_ROW, count);
-        while (end < behind) {
-            const int mid = (end + behind) >> 1;
-            if (keys[mid] >> PLACE_BITS == row) end = mid + 1;
-            else behind = mid;
-        }
-        float acc[VE] = {};
-        add(acc, i, end);
+        const int end = end_of(i, min(i + FEW_LONG + 1, count));
+        return end - begin > FEW_LONG ? -1 : end;
+    };
+    const int per = (count + workers - 1) / workers;
+    int i = min(worker * per, count), stop = min(i + per, count);
+    int c = i < stop ? cut(i) : 0;
+    bool inside = c < 0;                                 // a long run that began in an earlier worker
+    if (c > 0) i = c;
+    c = i < stop ? cut(stop) : 0;
+    const bool goes_on = c < 0;                          // a long run goes on in the next worker
+    if (c > 0) stop = c;
+    float acc[VE] = {};
+    bool begun = false;                                  // and it began here: this worker adds up its pieces
+    uint32_t row = 0;
+    auto store = [&](const uint32_t local) {
         Vec<DT, VE> v;
 #pragma unroll
-        for (int c = 0; c < VE; ++c) v.set(c, acc[c] * a.scale);
-        v.store(out + dealt.row(blockIdx.x, row) * a.dim + col);
+        for (int k = 0; k < VE; ++k) v.set(k, acc[k] * a.scale);
+        v.store(out + dealt.row(blockIdx.x, local) * a.dim + col);
+    };
+    auto leave = [&]() {                                 // a piece of a long run
+#pragma unroll
+        for (int k = 0; k < VE; ++k) piece[tid * VE + k] = acc[k];
+    };
+    if (mine && i < stop) {
+        row = row_at(i);
+        auto load = [&](Vec<DT, VE>& v, const int k) {
+            v.load(g + static_cast<int64_t>(keys[k] & ((1 << PLACE_BITS) - 1)) * a.ldg + col);
+        };
+        Vec<DT, VE> ahead[FEW_AHEAD];
+#pragma unroll
+        for (int k = 0; k < FEW_AHEAD; ++k)
+            if (i + k < stop) load(ahead[k], i + k);
+        for (; i < stop; i += FEW_AHEAD) {
+#pragma unroll
+            for (int k = 0; k < FEW_AHEAD; ++k) {
+                if (i + k >= stop) break;
+                if (row_at(i + k) != row) {
+                    if (inside) leave();
+                    else store(row);
+                    inside = false;
+                    row = row_at(i + k);
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) acc[j] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < VE; ++j) acc[j] += ahead[k].get(j);
+                if (i + k + FEW_AHEAD < stop) load(ahead[k], i + k + FEW_AHEAD);
+            }
+        }
+        if (inside) leave();
+        else if (goes_on) begun = true;
+        else store(row);
     }
     __syncthreads();
-    for (uint32_t m = 0; m < n_long; ++m) {              // a long run: every worker takes a part, joined in order
-        const int first = long_runs[m];
-        const uint32_t row = keys[first] >> PLACE_BITS;
-        int lo = first + LONG_ROW, hi = count;           // its end
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (keys[mid] >> PLACE_BITS == row) lo = mid;
-            else hi = mid;
-        }
-        const int each = (hi - first + workers - 1) / workers;
-        float acc[VE] = {};
-        if (mine) add(acc, min(first + worker * each, hi), min(first + (worker + 1) * each, hi));
+    if (begun) {
+        const int last = (end_of(stop - 1, count) - 1) / per;
+        double s[VE];
 #pragma unroll
-        for (int c = 0; c < VE; ++c) piece[tid * VE + c] = acc[c];
-        __syncthreads();
-        if (worker == 0 && mine) {
-            Vec<DT, VE> v;
+        for (int k = 0; k < VE; ++k) s[k] = acc[k];
+#pragma unroll 8
+        for (int w = worker + 1; w <= last; ++w)
 #pragma unroll
-            for (int c = 0; c < VE; ++c) {
-                double s = 0.0;
-                for (int w = 0; w < workers; ++w) s += piece[(w * lanes + tid) * VE + c];
-                v.set(c, static_cast<float>(s) * a.scale);
-            }
-            v.store(out + dealt.row(blockIdx.x, row) * a.dim + col);
-        }
-        __syncthreads();
+            for (int k = 0; k < VE; ++k) s[k] += piece[(tid + ((w - worker) << lanes_log2)) * VE + k];
+#pragma unroll
+        for (int k = 0; k < VE; ++k) acc[k] = static_cast<float>(s[k]);
+        store(row);
     }
 }
 
@@ -700,9 +840,9 @@ struct Plan {
 int64_t ceil_div(const int64_t a, const int64_t b) { return (a + b - 1) / b; }
 
 // Lanes (as a power of two, at most a wave) and slices that cover `units` vectors of a row.
-int lanes_for(const int64_t units, int* slices) {
+int lanes_for(const int64_t units, int* slices, const int most_log2 = 6) {
     int l = 0;
-    while ((1 << l) < units && l < 6) ++l;
+    while ((1 << l) < units && l < most_log2) ++l;
     *slices = static_cast<int>((units + (1 << l) - 1) >> l);
     return l;
 }
@@ -856,14 +996,16 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
 
 template <int DT, int VE>
 int launch_few(const GradArgs& a, sparc_stream_t stream) {
-    int slices;
-    const int lanes_log2 = lanes_for(ceil_div(a.dim, VE), &slices);
-    Dealt d = {0, 0};
+    int slices, blocks_log2 = FEW_BLOCKS_LOG2;
+    const int lanes_log2 = lanes_for(ceil_div(a.dim, VE), &slices, FEW_LANES_LOG2);
+    for (int k = slices; k > 1 && blocks_log2 > 4; k >>= 1) --blocks_log2;
+    Dealt d = {0, 0, 0};
     while ((static_cast<int64_t>(a.dim) * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) << d.group) < GROUP_BYTES) ++d.group;
     const int64_t groups = ceil_div(a.rows, static_cast<int64_t>(1) << d.group);
-    while (d.blocks < FEW_BLOCKS_LOG2 && (static_cast<int64_t>(1) << d.blocks) < groups) ++d.blocks;
+    while (d.blocks < blocks_log2 && (static_cast<int64_t>(1) << d.blocks) < groups) ++d.blocks;
     // (a row's number inside its workgroup leaves a bit of the key for the one that pads the sort)
     while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (1 << (31 - PLACE_BITS))) ++d.blocks;
+    while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (static_cast<int64_t>(1) << d.bits)) ++d.bits;
     const unsigned grid = static_cast<unsigned>(groups < (1 << d.blocks) ? groups : 1 << d.blocks);
     size_t keys = 1;
     while (keys < static_cast<size_t>(a.n)) keys <<= 1;

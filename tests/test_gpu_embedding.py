@@ -341,3 +341,19 @@ def test_lookup_of_more_rows_than_one_launch_takes():
         assert torch.equal(out[a:a + 100_000], table[ids[a:a + 100_000].long()]), a
     del out, ids
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("pattern", ["uniform", "zipf", "one", "falling", "stray"])
+@pytest.mark.parametrize("n,rows,dim,dtype", [(8192, 11, 2, torch.float32), (8192, 300, 1, torch.float32), (8191, 40_000, 64, torch.float32),
+                                              (8000, 2_449_029, 3, torch.bfloat16), (4096, 2, 512, torch.bfloat16), (257, 1, 33, torch.float32),
+                                              (1500, 7, 700, torch.float16), (8192, 4000, 256, torch.float16), (513, 3, 1000, torch.float32),
+                                              (6000, 100_000_000, 1, torch.float32), (300, 19, 8, torch.bfloat16)])
+def test_gradient_of_few_tokens_however_they_fall(pattern, n, rows, dim, dtype):
+    """What one launch takes: all tokens in one workgroup or none, runs of every length, in order and out of it."""
+    from sparc_amd.embedding import embedding_grad
+    ids = make_ids(pattern, n, rows, n + dim)
+    g = torch.randn(n, dim, device="cuda", generator=gen(n + rows)).to(dtype)
+    got = embedding_grad(ids, g, rows, scale=0.75, padding_idx=rows // 3)
+    check_grad(got, ids, g, rows, 0.75, rows // 3)
+    assert torch.equal(got, embedding_grad(ids, g, rows, scale=0.75, padding_idx=rows // 3))
+    check_grad(embedding_grad(ids.clamp(-1, rows).int(), g, rows, scale=0.75), ids, g, rows, 0.75)
