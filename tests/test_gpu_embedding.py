@@ -357,3 +357,24 @@ def test_gradient_of_few_tokens_however_they_fall(pattern, n, rows, dim, dtype):
     check_grad(got, ids, g, rows, 0.75, rows // 3)
     assert torch.equal(got, embedding_grad(ids, g, rows, scale=0.75, padding_idx=rows // 3))
     check_grad(embedding_grad(ids.clamp(-1, rows).int(), g, rows, scale=0.75), ids, g, rows, 0.75)
+
+
+@pytest.mark.parametrize("n", [3, 1001, 8190, 20_001])
+def test_tokens_at_any_element_and_nan_in_places_left_out(n):
+    """Tokens and gradients that start at any element; what padding and stray tokens carry reaches no row."""
+    from sparc_amd.embedding import embedding_grad, embedding_lookup
+    rows, pad = 500, 7
+    for offset in (1, 2, 3):
+        ids = make_ids("stray", n + offset, rows, n)
+        g = torch.randn(n + offset, 37, device="cuda", generator=gen(n))
+        left_out = (ids < 0) | (ids >= rows) | (ids == pad)
+        g[left_out] = torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda").repeat(13)[:37]
+        kept = torch.where(left_out[:, None], torch.zeros_like(g), g)
+        for dtype in DTYPES:
+            tokens, some, clean = ids[offset:], g.to(dtype)[offset:, 1:], kept.to(dtype)[offset:, 1:]
+            got = embedding_grad(tokens, some, rows, padding_idx=pad)
+            check_grad(got, tokens, clean, rows, padding_idx=pad)
+            assert torch.equal(got, embedding_grad(ids.clamp(-1, rows).int()[offset:], some, rows, padding_idx=pad))
+        table = torch.randn(rows, 37, device="cuda", generator=gen(1))
+        out = embedding_lookup(ids.clamp(-1, rows).int()[offset:], table)
+        assert torch.equal(out.nan_to_num(5.0), embedding_lookup(ids[offset:], table).nan_to_num(5.0))
