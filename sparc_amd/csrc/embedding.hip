@@ -692,7 +692,7 @@ __device__ __forceinline__ void radix_sort(uint32_t* keys, const int count, cons
 template <int DT, int VE>
 __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const Dealt dealt, const int lanes_log2) {
     typedef typename Elem<DT>::type T;
-    extern __shared__ __align__(16) uint32_t keys[];     // a power of two of them, at least n
+    extern __shared__ __align__(16) uint32_t keys[];     // n, and up to a multiple of four
     __shared__ uint32_t sums[FEW_WAVES];
     // counters of the sort, then sums of the workers' pieces
     __shared__ __align__(16) uint32_t shared[VE > 2 ? FEW_THREADS * VE : FEW_THREADS * 2];
@@ -1007,8 +1007,7 @@ int launch_few(const GradArgs& a, sparc_stream_t stream) {
     while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (1 << (31 - PLACE_BITS))) ++d.blocks;
     while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (static_cast<int64_t>(1) << d.bits)) ++d.bits;
     const unsigned grid = static_cast<unsigned>(groups < (1 << d.blocks) ? groups : 1 << d.blocks);
-    size_t keys = 1;
-    while (keys < static_cast<size_t>(a.n)) keys <<= 1;
+    const size_t keys = a.n > 0 ? (static_cast<size_t>(a.n) + 3) & ~static_cast<size_t>(3) : 4;
     hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(grid, static_cast<unsigned>(slices)), dim3(FEW_THREADS), keys * sizeof(uint32_t), stream, a, d,
                        lanes_log2);
     SPARC_CHECK_LAUNCH();
