@@ -130,29 +130,25 @@ __device__ __forceinline__ uint64_t equals(const uint32_t key, const int bits, c
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-// Zeros that a launch of the sort writes with workgroups of its own behind the sorting ones.
-// Plain stores: nontemporal ones change 120 to 112 us at 512 MB of zeros, nothing at 627 MB and 50 to 55 us at 200 MB, where
-// the Infinity Cache takes part of them.
+// Zeros that a launch writes with workgroups of its own behind those that do something else: one 16-byte store per thread,
+// so that the workgroups that run at once write one stretch of memory.  627 MB in a launch: 98 us with one store per thread,
+// 108 with eight, 125 with a grid of 1024 workgroups that goes round (a fill by the library: 92).  Plain stores: nontemporal
+// ones change 120 to 112 us at 512 MB of zeros, nothing at 627 MB and 50 to 55 us at 200 MB, where the Infinity Cache takes part
+// of them.
 struct Zeros {
     uint16_t* p;
     int64_t count;         // of uint16
 };
-constexpr int ZERO_CHUNK = SORT_BLOCK * 8 * 8;   // uint16 of a workgroup: eight 16-byte stores per thread
+constexpr int ZERO_CHUNK = SORT_BLOCK * 8;      // uint16 of a workgroup and turn
+constexpr int64_t ZERO_GROUPS = 1 << 22;        // at most (a launch has fewer than 2^32 threads): more zeros take turns
 
-__device__ __forceinline__ void write_zeros(const Zeros& z, const int64_t chunk) {
+__device__ __forceinline__ void write_zeros(const Zeros& z, const int64_t first, const int64_t groups) {
     typedef uint16_t mem __attribute__((ext_vector_type(8), aligned(2)));
     const mem zero = {};
-    const int64_t from = chunk * ZERO_CHUNK + threadIdx.x * 8;
-    if ((chunk + 1) * ZERO_CHUNK <= z.count) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) *reinterpret_cast<mem*>(z.p + from + k * SORT_BLOCK * 8) = zero;
-        return;
-    }
-    for (int64_t i = from; i < z.count; i += SORT_BLOCK * 8) {
-        if (i + 8 <= z.count) *reinterpret_cast<mem*>(z.p + i) = zero;
-        else
-            for (int64_t k = i; k < z.count; ++k) z.p[k] = 0;
-    }
+    int64_t i = first * ZERO_CHUNK + threadIdx.x * 8;
+    for (; i + 8 <= z.count; i += groups * ZERO_CHUNK) *reinterpret_cast<mem*>(z.p + i) = zero;
+    for (; i < z.count; i += groups * ZERO_CHUNK)
+        for (int64_t k = i; k < z.count && k < i + 8; ++k) z.p[k] = 0;
 }
 
 // The next UP_FRONT {row, place} of this lane, places i0 + 64 k + lane below hi; row = ~0: none.
@@ -180,7 +176,7 @@ __device__ __forceinline__ void take(const GradArgs& a, const bool first, const 
 }
 
 // The sort: two or three passes of a count and a scatter.  262147 tokens over 50021 rows, two passes of 8 bits: 6.0 + 10.0 us
-// each; 48979 tokens over 2449029 rows, two of 11 bits: 28 us a launch with a quarter of the 627 MB of zeros in it (4.7 and
+// each; 48979 tokens over 2449029 rows, two of 11 bits: 26 us a launch with a quarter of the 627 MB of zeros in it (4.7 and
 // 9 us without).  Bound by latency: of a scatter's 9 us 3.5 are the ranking (ballots: six vector instructions a bit), 2 the
 // other tiles' counts, the rest start, loads and stores.  512 threads with 4 tokens each: 5.0 + 9.4 us; 8 each: 5.7 + 11.1;
 // 1024 threads with 8: 7.3 + 13.6.  Sorting by buckets of rows instead (a workgroup per bucket) took 115 to 514 us where
@@ -188,7 +184,7 @@ __device__ __forceinline__ void take(const GradArgs& a, const bool first, const 
 // Digits of the tokens of a tile: digit = (row >> shift) & (1 << bits) - 1.
 __global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, const Zeros z, const uint2* in, const int shift, const int bits) {
     __shared__ uint32_t cnt[1 << MOST_BITS];
-    if (static_cast<int>(blockIdx.x) >= a.tiles) return write_zeros(z, blockIdx.x - a.tiles);
+    if (static_cast<int>(blockIdx.x) >= a.tiles) return write_zeros(z, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     const bool first = in == nullptr;
     const int digits = 1 << bits;
     const int64_t n = first ? a.n : *a.kept;
@@ -209,7 +205,7 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_counts(const GradArgs a, con
 __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, const Zeros z, const uint2* in, uint2* out, const int shift, const int bits) {
     extern __shared__ __align__(16) uint32_t lds[];   // base [digits], total [digits], cnt uint16 [SORT_WAVES][digits]
     __shared__ uint32_t sums[SORT_WAVES];
-    if (static_cast<int>(blockIdx.x) >= a.tiles) return write_zeros(z, blockIdx.x - a.tiles);
+    if (static_cast<int>(blockIdx.x) >= a.tiles) return write_zeros(z, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     const bool first = in == nullptr;
     const int digits = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     static_assert(4 * SORT_BLOCK >= 1 << MOST_BITS, "a thread has four digits");
@@ -689,8 +685,11 @@ __device__ __forceinline__ void radix_sort(uint32_t* keys, const int count, cons
     }
 }
 
+__global__ __launch_bounds__(SORT_BLOCK) void zeros_kernel(const Zeros z) { write_zeros(z, blockIdx.x, gridDim.x); }
+
+// zeros: write them here, too.
 template <int DT, int VE>
-__global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const Dealt dealt, const int lanes_log2) {
+__global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, const Dealt dealt, const int lanes_log2, const bool zeros) {
     typedef typename Elem<DT>::type T;
     extern __shared__ __align__(16) uint32_t keys[];     // n, and up to a multiple of four
     __shared__ uint32_t sums[FEW_WAVES];
@@ -709,7 +708,8 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
     Vec<DT, VE> zero;
 #pragma unroll
     for (int i = 0; i < VE; ++i) zero.set(i, 0.f);
-    if (dealt.group > 0) {                               // narrow rows, one slice: a group of them is one stretch of memory
+    if (!zeros) {
+    } else if (dealt.group > 0) {                        // narrow rows, one slice: a group of them is one stretch of memory
         const int64_t stretch = static_cast<int64_t>(a.dim) << dealt.group, len = a.rows * a.dim;
         const int per_stretch = static_cast<int>((stretch + VE - 1) / VE);
         int log2 = 0;
@@ -968,7 +968,7 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
         z.p = static_cast<uint16_t*>(a.out) + dealt * ZERO_CHUNK;
         z.count = half_words - dealt * ZERO_CHUNK < mine * ZERO_CHUNK ? half_words - dealt * ZERO_CHUNK : mine * ZERO_CHUNK;
         dealt += mine;
-        return dim3(static_cast<unsigned>(p.tiles + mine));
+        return dim3(static_cast<unsigned>(p.tiles + (mine < ZERO_GROUPS ? mine : ZERO_GROUPS)));
     };
     const uint2* in = nullptr;   // the ids themselves
     for (int pass = 0; pass < p.passes; ++pass) {
@@ -1007,9 +1007,21 @@ int launch_few(const GradArgs& a, sparc_stream_t stream) {
     while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (1 << (31 - PLACE_BITS))) ++d.blocks;
     while ((ceil_div(groups, static_cast<int64_t>(1) << d.blocks) << d.group) > (static_cast<int64_t>(1) << d.bits)) ++d.bits;
     const unsigned grid = static_cast<unsigned>(groups < (1 << d.blocks) ? groups : 1 << d.blocks);
+    // Zeros that outgrow the Infinity Cache come in a launch of their own, line after line; where a workgroup's rows are not
+    // whole lines of 128 bytes, from a third of that on, because lines that two workgroups write leave the cache half written.
+    // Ten tokens, three outputs in turn, together and apart: 2449029 rows of 47 floats 173, 78 us; of 64 floats 115, 105;
+    // 100000 of 507 halves 32, 22; of 512 halves 21.9, 22.9; 50000 of 507 halves 11.9, 12.7.
+    const int64_t row_bytes = a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)), bytes = a.rows * row_bytes;
+    const bool apart = bytes > ((row_bytes << d.group) % 128 ? SPARC_KEEP_BYTES / 3 : SPARC_KEEP_BYTES);
+    if (apart) {
+        const int64_t chunks = ceil_div(bytes / 2, ZERO_CHUNK);
+        hipLaunchKernelGGL(zeros_kernel, dim3(static_cast<unsigned>(chunks < ZERO_GROUPS ? chunks : ZERO_GROUPS)), dim3(SORT_BLOCK), 0, stream,
+                           (Zeros{static_cast<uint16_t*>(a.out), bytes / 2}));
+        SPARC_CHECK_LAUNCH();
+    }
     const size_t keys = a.n > 0 ? (static_cast<size_t>(a.n) + 3) & ~static_cast<size_t>(3) : 4;
     hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(grid, static_cast<unsigned>(slices)), dim3(FEW_THREADS), keys * sizeof(uint32_t), stream, a, d,
-                       lanes_log2);
+                       lanes_log2, !apart);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }

@@ -378,3 +378,15 @@ def test_tokens_at_any_element_and_nan_in_places_left_out(n):
         table = torch.randn(rows, 37, device="cuda", generator=gen(1))
         out = embedding_lookup(ids.clamp(-1, rows).int()[offset:], table)
         assert torch.equal(out.nan_to_num(5.0), embedding_lookup(ids[offset:], table).nan_to_num(5.0))
+
+
+@pytest.mark.parametrize("rows,dim,dtype", [(300_001, 127, torch.float16), (420_000, 47, torch.float32), (300_000, 256, torch.float16),
+                                            (64_000_001, 1, torch.bfloat16), (90_001, 601, torch.float32), (1_500_000, 32, torch.float32)])
+def test_gradient_of_few_tokens_in_a_large_table(rows, dim, dtype):
+    """Zeros in the same launch and in one of their own."""
+    from sparc_amd.embedding import embedding_grad
+    for n in (0, 5, 3000):
+        ids = make_ids("zipf", n, rows, 90 + n)
+        g = torch.randn(n, dim, device="cuda", generator=gen(91)).to(dtype)
+        torch.full((rows, dim), 3.0, dtype=dtype, device="cuda")          # what a new allocation may hold
+        check_grad(embedding_grad(ids, g, rows), ids, g, rows)
