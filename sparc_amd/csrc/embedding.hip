@@ -11,7 +11,7 @@
 //                  further workgroups of its launches write the table's zeros meanwhile;
 //   row_sums       adds up, over the zeros.  A worker has `per` sorted places whatever the rows hold; a row of at most
 //                  LONG_ROW places belongs to the worker that meets its first, a longer one is cut and leaves one partial
-//                  sum per worker,
+//                  sum per worker, or per workgroup where it has all its places,
 //   join_rows      which are added in order (float64) here.  Usually nothing to do.
 // Few tokens take one launch instead (few_tokens).
 #include <type_traits>
@@ -106,6 +106,7 @@ struct GradArgs {
     int tiles;
     int dim, wide_ids;
     int per;                   // places of a worker
+    int in_group;              // workers of a workgroup of row_sums
     float scale;
     uint32_t* counts;          // [tiles][1 << bits]: digits of a tile
     uint2* sorted;             // [n] {row, place}; the last pass leaves the result here
@@ -349,7 +350,6 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     const int64_t worker = static_cast<int64_t>(blockIdx.x) * in_group + (tid >> lanes_log2);
     const int64_t w0 = worker * a.per, w1 = min(w0 + a.per, all);
     const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + u, col = min(unit * VE, a.dim - VE);
-    if (w0 >= w1 || unit * VE >= a.dim) return;          // no barrier below
     // from here on: places relative to `from`
     const int n_staged = static_cast<int>(to - from);
     // Where does the row that is cut in front of place i end?  0: no row is, -1: it is longer than LONG_ROW, otherwise its end
@@ -371,6 +371,45 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
         return f_lo - s_lo > LONG_ROW ? -1 : f_lo;
     };
     int i = static_cast<int>(w0 - from), i_stop = static_cast<int>(w1 - from);
+    float acc[VE] = {};
+    const int b0 = static_cast<int>(e0 - from), b1 = static_cast<int>(e1 - from);
+    if (e0 > 0 && e1 < all && row_of[b0 - 1] == row_of[b1] && cut(b0) < 0) {   // the workgroup is inside one long row: one piece
+        const bool mine = unit * VE < a.dim;
+        if (mine) {
+            Vec<DT, VE> ahead[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (i + k < i_stop) ahead[k].template load<STREAM>(g + static_cast<int64_t>(places[i + k]) * a.ldg + col);
+            for (; i < i_stop; i += AHEAD)
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (i + k >= i_stop) break;
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) acc[j] += ahead[k].get(j);
+                    if (i + k + AHEAD < i_stop) ahead[k].template load<STREAM>(g + static_cast<int64_t>(places[i + k + AHEAD]) * a.ldg + col);
+                }
+        }
+        if (u == 0 && blockIdx.y == 0) a.begins[worker] = 0u;
+        float* joined = reinterpret_cast<float*>(places + (in_group * a.per + 2 * MARGIN));   // [WAVES][lanes][VE]
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+            double s = acc[k];
+            for (int off = lanes; off < 64; off <<= 1) s += __shfl_xor(s, off);
+            if ((tid & 63) < lanes) joined[((tid >> 6) * lanes + u) * VE + k] = static_cast<float>(s);
+        }
+        __syncthreads();
+        if (tid < lanes && mine) {
+            float* p = a.part + 2 * worker * a.dim + col;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                double s = 0.0;
+                for (int w = 0; w < WAVES; ++w) s += joined[(w * lanes + u) * VE + k];
+                p[k] = static_cast<float>(s);
+            }
+        }
+        return;
+    }
+    if (w0 >= w1 || unit * VE >= a.dim) return;          // no barrier below
     int c = cut(i);
     bool inside = c < 0;                                 // a long row that began in an earlier worker
     if (c > 0) i = c;                                    // an earlier worker has the whole row
@@ -379,7 +418,6 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     if (c > 0) i_stop = c;                               // the row that is cut here is this worker's
     if (i >= i_stop) return;
     uint32_t row = row_of[i];
-    float acc[VE] = {};
     auto finish_row = [&]() {
         if (inside) {
             float* p = a.part + (2 * worker) * a.dim + col;
@@ -462,9 +500,15 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
         }
         __syncthreads();
         const int64_t first = begun;
-        const int64_t pieces = last - first + 1;
-        // the first worker's piece begins the row: its second slot
-        const float* part = a.part + 2 * first * a.dim + col;
+        // a piece per worker, but one for all workers of a workgroup that is wholly inside the row; the first worker's piece
+        // begins the row: its second slot
+        const int64_t g0 = first / a.in_group, g1 = last / a.in_group;
+        const int64_t head = g0 == g1 ? last - first + 1 : (g0 + 1) * a.in_group - first, middle = g0 == g1 ? 0 : g1 - g0 - 1;
+        const int64_t pieces = g0 == g1 ? head : head + middle + last - g1 * a.in_group + 1;
+        auto piece = [&](const int64_t p) {
+            const int64_t worker = p < head ? first + p : p < head + middle ? (g0 + 1 + p - head) * a.in_group : g1 * a.in_group + (p - head - middle);
+            return a.part + (2 * worker + (p == 0 ? 1 : 0)) * a.dim + col;
+        };
         double s[VE] = {};
         if (unit < a.dim) {
             for (int64_t p0 = group; p0 < pieces; p0 += JOIN_GROUPS * JOIN_AHEAD) {
@@ -472,7 +516,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
 #pragma unroll
                 for (int j = 0; j < JOIN_AHEAD; ++j) {
                     const int64_t p = p0 + j * JOIN_GROUPS;
-                    if (p < pieces) v[j].load(part + (2 * p + (p == 0 ? 1 : 0)) * a.dim);
+                    if (p < pieces) v[j].load(piece(p));
                 }
 #pragma unroll
                 for (int j = 0; j < JOIN_AHEAD; ++j)
@@ -981,7 +1025,8 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
         SPARC_CHECK_LAUNCH();
         in = out;
     }
-    const size_t staged = static_cast<size_t>(p.per * p.in_group + 2 * MARGIN) * 2 * sizeof(uint32_t);
+    const size_t staged = static_cast<size_t>(p.per * p.in_group + 2 * MARGIN) * 2 * sizeof(uint32_t) +
+                          (static_cast<size_t>(WAVES * VE) << p.lanes_log2) * sizeof(float);
     const bool once = a.n * a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)) > SPARC_KEEP_BYTES;
     hipLaunchKernelGGL((once ? row_sums<DT, VE, true> : row_sums<DT, VE, false>),
                        dim3(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), static_cast<unsigned>(p.slices)), dim3(BLOCK), staged, stream,
@@ -1046,6 +1091,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         a = carve(p, n, static_cast<int>(dim), ws, ws_bytes, &ok, &used);
         if (!ws || !ok) return SPARC_ERR_WS;
         a.per = p.per;
+        a.in_group = p.in_group;
     }
     a.ids = ids;
     a.g = g;
