@@ -9,8 +9,8 @@
 //                  between waves, the other tiles' counts before it) and scatters {row, place}.  However often one
 //                  token occurs, every tile is the same work.  The sort waits on latency and leaves the memory idle, so
 //                  further workgroups of its launches write the table's zeros meanwhile;
-//   row_sums       adds up, over the zeros.  A worker has `per` sorted places whatever the rows hold; a row of at most
-//                  LONG_ROW places belongs to the worker that meets its first, a longer one is cut and leaves one partial
+//   row_sums       adds up, over the zeros.  A worker has `per` sorted places whatever the rows hold; a row of few
+//                  places belongs to the worker that meets its first, a longer one is cut and leaves one partial
 //                  sum per worker, or per workgroup where it has all its places,
 //   join_rows      which are added in order (float64) here.  Usually nothing to do.
 // Few tokens take one launch instead (few_tokens).
@@ -28,10 +28,9 @@ constexpr int MOST_TILES = 256;                // every tile reads all tiles' co
 constexpr int MOST_BITS = 11;                  // of a digit
 constexpr int WAVES = 4;
 constexpr int BLOCK = 64 * WAVES;
-constexpr int LONG_ROW = 64;
+constexpr int LONG_ROW = 64;       // places of the longest row that is one worker's, at most
 constexpr int STAGE = 4096;        // places of a workgroup of row_sums at most
 constexpr int AHEAD = 8;           // gradient rows in flight per worker
-constexpr int JOIN_GRID = 256;
 
 // ---- lookup ------------------------------------------------------------------------------------------------
 
@@ -107,6 +106,7 @@ struct GradArgs {
     int dim, wide_ids;
     int per;                   // places of a worker
     int in_group;              // workers of a workgroup of row_sums
+    int long_row;              // places of the longest row that is one worker's
     float scale;
     uint32_t* counts;          // [tiles][1 << bits]: digits of a tile
     uint2* sorted;             // [n] {row, place}; the last pass leaves the result here
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(SORT_BLOCK) void digit_scatter(const GradArgs a, co
 // Walking rows and places together, so that a worker also writes the zeros of the rows between its own, saves the second
 // write of the rows that have places (1024 columns, as many rows as places: 251 against 271 us) and lost everywhere
 // else (48979 places in 2449029 rows: 153 against 125 us).
-constexpr int MARGIN = LONG_ROW + 1;   // places looked at on both sides of a cut
+constexpr int MARGIN = LONG_ROW + 1;   // places staged on both sides of a workgroup's
 
 template <int DT, int VE, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int lanes_log2) {
@@ -352,23 +352,23 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
     const int unit = (static_cast<int>(blockIdx.y) << lanes_log2) + u, col = min(unit * VE, a.dim - VE);
     // from here on: places relative to `from`
     const int n_staged = static_cast<int>(to - from);
-    // Where does the row that is cut in front of place i end?  0: no row is, -1: it is longer than LONG_ROW, otherwise its end
+    // Where does the row that is cut in front of place i end?  0: no row is, -1: it is a long one, otherwise its end
     auto cut = [&](const int i) {
         if (i == 0 || i == n_staged || row_of[i - 1] != row_of[i]) return 0;   // (0 and n_staged only where all places end)
         const uint32_t r = row_of[i];
-        int s_lo = max(i - MARGIN, 0), s_hi = i - 1;     // its first place, as far as MARGIN sees
+        int s_lo = max(i - a.long_row - 1, 0), s_hi = i - 1;   // its first place, as far as a long row shows
         while (s_lo < s_hi) {
             const int mid = (s_lo + s_hi) >> 1;
             if (row_of[mid] < r) s_lo = mid + 1;
             else s_hi = mid;
         }
-        int f_lo = i + 1, f_hi = min(i + MARGIN, n_staged);   // behind its last place
+        int f_lo = i + 1, f_hi = min(i + a.long_row + 1, n_staged);   // behind its last place
         while (f_lo < f_hi) {
             const int mid = (f_lo + f_hi) >> 1;
             if (row_of[mid] <= r) f_lo = mid + 1;
             else f_hi = mid;
         }
-        return f_lo - s_lo > LONG_ROW ? -1 : f_lo;
+        return f_lo - s_lo > a.long_row ? -1 : f_lo;
     };
     int i = static_cast<int>(w0 - from), i_stop = static_cast<int>(w1 - from);
     float acc[VE] = {};
@@ -468,19 +468,25 @@ __global__ __launch_bounds__(BLOCK) void row_sums(const GradArgs a, const int la
 
 // Long rows: slice blockIdx.y of 64 columns, VE (four, or one where a row has fewer) columns to a lane.  The pieces of a
 // row are dealt to the groups of 16 lanes, which have JOIN_AHEAD of them in flight; the groups' sums meet in their order.
+// Where there are far fewer rows than workgroups, four of these share a slice, in groups of 4 lanes: 262147 places of 512
+// bfloat16 all the same 131 -> 98 us (always: frequent tokens first 102 -> 121).
 // 9 us for the 300 long rows of 262147 tokens, frequent ones first; 4.6 us (the wait for the launch before) for none.
-constexpr int JOIN_WAVES = 4, JOIN_GROUPS = JOIN_WAVES * 4, JOIN_AHEAD = 8;
+constexpr int JOIN_THREADS = 256, JOIN_COLS = 64, JOIN_AHEAD = 8;
 
 template <int DT, int VE>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
+__global__ __launch_bounds__(JOIN_THREADS) void join_rows(const GradArgs a) {
     typedef typename Elem<DT>::type T;
-    __shared__ double sum[JOIN_GROUPS][64];
+    __shared__ double sum[JOIN_THREADS * VE];            // [groups][cols]
     __shared__ int64_t begun;
     const uint32_t count = a.long_rows[0];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 4;
-    const int base = blockIdx.y * 64, unit = base + (lane & 15) * VE, col = max(min(unit, a.dim - VE), 0);
-    for (uint32_t k = blockIdx.x; k < count; k += gridDim.x) {
-        const int64_t row = a.long_rows[1 + 2 * k], last = a.long_rows[2 + 2 * k];
+    const int parts_log2 = VE > 1 && 4 * count <= gridDim.x ? 2 : 0;
+    const int lanes_log2 = 4 - parts_log2, groups = JOIN_THREADS >> lanes_log2, cols = VE << lanes_log2;
+    static_assert(JOIN_COLS == 4 << 4, "a slice is 16 lanes of four columns");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> lanes_log2;
+    for (uint32_t k = blockIdx.x; k < count << parts_log2; k += gridDim.x) {
+        const int base = blockIdx.y * JOIN_COLS + (k & ((1u << parts_log2) - 1u)) * cols;
+        const int unit = base + (threadIdx.x & ((1 << lanes_log2) - 1)) * VE, col = max(min(unit, a.dim - VE), 0);
+        const int64_t row = a.long_rows[1 + 2 * (k >> parts_log2)], last = a.long_rows[2 + 2 * (k >> parts_log2)];
         if (wave == 0) {                                 // the worker that began the row: near by, or found by the row's first place
             const int64_t before = last - 1 - lane;
             const uint64_t found = __ballot(before >= 0 && a.begins[max(before, static_cast<int64_t>(0))] == 1u);
@@ -511,29 +517,29 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void join_rows(const GradArgs a) {
         };
         double s[VE] = {};
         if (unit < a.dim) {
-            for (int64_t p0 = group; p0 < pieces; p0 += JOIN_GROUPS * JOIN_AHEAD) {
+            for (int64_t p0 = group; p0 < pieces; p0 += groups * JOIN_AHEAD) {
                 Vec<SPARC_F32, VE> v[JOIN_AHEAD];
 #pragma unroll
                 for (int j = 0; j < JOIN_AHEAD; ++j) {
-                    const int64_t p = p0 + j * JOIN_GROUPS;
+                    const int64_t p = p0 + j * groups;
                     if (p < pieces) v[j].load(piece(p));
                 }
 #pragma unroll
                 for (int j = 0; j < JOIN_AHEAD; ++j)
-                    if (p0 + j * JOIN_GROUPS < pieces)
+                    if (p0 + j * groups < pieces)
 #pragma unroll
                         for (int c = 0; c < VE; ++c) s[c] += v[j].get(c);
             }
 #pragma unroll
             for (int c = 0; c < VE; ++c)
-                if (col + c >= base) sum[group][col + c - base] = s[c];
+                if (col + c >= base) sum[group * cols + col + c - base] = s[c];
         }
         __syncthreads();
         const int mine = base + threadIdx.x;
-        if (threadIdx.x < 64 && mine < a.dim && (VE > 1 || threadIdx.x < 16)) {
+        if (threadIdx.x < cols && mine < a.dim) {
             double all = 0.0;
-#pragma unroll
-            for (int w = 0; w < JOIN_GROUPS; ++w) all += sum[w][threadIdx.x];
+#pragma unroll 16
+            for (int w = 0; w < groups; ++w) all += sum[w * cols + threadIdx.x];
             static_cast<T*>(a.out)[row * a.dim + mine] = Elem<DT>::down(static_cast<float>(all) * a.scale);
         }
         __syncthreads();
@@ -878,7 +884,7 @@ __global__ __launch_bounds__(FEW_THREADS) void few_tokens(const GradArgs a, cons
 // Sizes of the launches and of the workspace's parts, from n, rows and dim alone.
 struct Plan {
     int64_t tile, workers;
-    int tiles, passes, bits, per, lanes_log2, slices, in_group;
+    int tiles, passes, bits, per, long_row, lanes_log2, slices, in_group;
 };
 
 int64_t ceil_div(const int64_t a, const int64_t b) { return (a + b - 1) / b; }
@@ -908,6 +914,8 @@ Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     p.per = static_cast<int>(wanted < 8 ? 8 : wanted > 64 ? 64 : wanted);
     if (static_cast<int64_t>(p.per) * p.in_group > STAGE) p.per = STAGE / p.in_group;
     p.workers = ceil_div(n, p.per);
+    // Two shares, or a worker that has a whole row would be the last by far (per is 8 to 64).  Always 64, always 16: 20000 places over 5000 rows of 64 floats, frequent first, 41, 34 us; 1000000 over 50000, uniform, 99, 488.
+    p.long_row = 2 * p.per > LONG_ROW ? LONG_ROW : 2 * p.per;
     return p;
 }
 
@@ -948,7 +956,7 @@ GradArgs carve(const Plan& p, const int64_t n, const int dim, void* ws, const si
     a.sorted = c.take<uint2>(n);
     a.other = c.take<uint2>(p.passes > 1 ? n : 0);
     a.kept = c.take<uint32_t>(1);
-    a.long_rows = c.take<uint32_t>(1 + 2 * (n / LONG_ROW + 1));
+    a.long_rows = c.take<uint32_t>(1 + 2 * (n / p.long_row + 1));
     a.begins = c.take<uint32_t>(p.workers);
     a.part = c.take<float>(static_cast<size_t>(2) * p.workers * dim);
     *ok = c.ok();
@@ -1032,9 +1040,10 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
                        dim3(static_cast<unsigned>(ceil_div(p.workers, p.in_group)), static_cast<unsigned>(p.slices)), dim3(BLOCK), staged, stream,
                        a, p.lanes_log2);
     SPARC_CHECK_LAUNCH();
-    const dim3 joining(JOIN_GRID, static_cast<unsigned>((a.dim + 63) / 64));
-    if (a.dim >= 4) hipLaunchKernelGGL((join_rows<DT, 4>), joining, dim3(64 * JOIN_WAVES), 0, stream, a);
-    else hipLaunchKernelGGL((join_rows<DT, 1>), joining, dim3(64 * JOIN_WAVES), 0, stream, a);
+    const int slices = (a.dim + JOIN_COLS - 1) / JOIN_COLS, rows_at_once = 2048 / slices;
+    const dim3 joining(static_cast<unsigned>(rows_at_once < 32 ? 32 : rows_at_once > 256 ? 256 : rows_at_once), static_cast<unsigned>(slices));
+    if (a.dim >= 4) hipLaunchKernelGGL((join_rows<DT, 4>), joining, dim3(JOIN_THREADS), 0, stream, a);
+    else hipLaunchKernelGGL((join_rows<DT, 1>), joining, dim3(JOIN_THREADS), 0, stream, a);
     SPARC_CHECK_LAUNCH();
     return SPARC_OK;
 }
@@ -1092,6 +1101,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         if (!ws || !ok) return SPARC_ERR_WS;
         a.per = p.per;
         a.in_group = p.in_group;
+        a.long_row = p.long_row;
     }
     a.ids = ids;
     a.g = g;

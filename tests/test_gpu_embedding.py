@@ -390,3 +390,19 @@ def test_gradient_of_few_tokens_in_a_large_table(rows, dim, dtype):
         g = torch.randn(n, dim, device="cuda", generator=gen(91)).to(dtype)
         torch.full((rows, dim), 3.0, dtype=dtype, device="cuda")          # what a new allocation may hold
         check_grad(embedding_grad(ids, g, rows), ids, g, rows)
+
+
+@pytest.mark.parametrize("pattern", ["one", "zipf", "uniform", "lengths"])
+@pytest.mark.parametrize("n,rows,dim,dtype", [(30_000, 3, 1, torch.float32), (30_000, 3, 3, torch.float16), (40_001, 5, 70, torch.float32),
+                                              (262_147, 3, 47, torch.float32), (20_000, 2, 515, torch.bfloat16), (9_000, 1, 1030, torch.float16),
+                                              (70_000, 120, 8, torch.bfloat16), (300_000, 30, 16, torch.float32)])
+def test_gradient_of_rows_that_many_workgroups_share(pattern, n, rows, dim, dtype):
+    """One piece per worker at a long row's ends, one per workgroup inside it; few long rows and many."""
+    from sparc_amd.embedding import embedding_grad
+    ids = make_ids(pattern, n, rows, n + dim)
+    if pattern == "lengths":
+        ids = torch.cat([ids % rows, torch.arange(n, device="cuda") * rows // n])
+    g = torch.randn(ids.numel(), dim, device="cuda", generator=gen(n + rows)).to(dtype)
+    got = embedding_grad(ids, g, rows, scale=-1.5)
+    check_grad(got, ids, g, rows, -1.5)
+    assert torch.equal(got, embedding_grad(ids, g, rows, scale=-1.5))
