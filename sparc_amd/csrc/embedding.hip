@@ -105,7 +105,7 @@ struct GradArgs {
     int tiles;
     int dim, wide_ids;
     int per;                   // places of a worker
-    int in_group;              // workers of a workgroup of row_sums
+    int group_log2;            // workers of a workgroup of row_sums, as a power of two
     int long_row;              // places of the longest row that is one worker's
     float scale;
     uint32_t* counts;          // [tiles][1 << bits]: digits of a tile
@@ -477,7 +477,7 @@ template <int DT, int VE>
 __global__ __launch_bounds__(JOIN_THREADS) void join_rows(const GradArgs a) {
     typedef typename Elem<DT>::type T;
     __shared__ double sum[JOIN_THREADS * VE];            // [groups][cols]
-    __shared__ int64_t begun;
+    __shared__ int begun;
     const uint32_t count = a.long_rows[0];
     const int parts_log2 = VE > 1 && 4 * count <= gridDim.x ? 2 : 0;
     const int lanes_log2 = 4 - parts_log2, groups = JOIN_THREADS >> lanes_log2, cols = VE << lanes_log2;
@@ -486,11 +486,12 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_rows(const GradArgs a) {
     for (uint32_t k = blockIdx.x; k < count << parts_log2; k += gridDim.x) {
         const int base = blockIdx.y * JOIN_COLS + (k & ((1u << parts_log2) - 1u)) * cols;
         const int unit = base + (threadIdx.x & ((1 << lanes_log2) - 1)) * VE, col = max(min(unit, a.dim - VE), 0);
-        const int64_t row = a.long_rows[1 + 2 * (k >> parts_log2)], last = a.long_rows[2 + 2 * (k >> parts_log2)];
+        const int64_t row = a.long_rows[1 + 2 * (k >> parts_log2)];
+        const int last = a.long_rows[2 + 2 * (k >> parts_log2)];
         if (wave == 0) {                                 // the worker that began the row: near by, or found by the row's first place
-            const int64_t before = last - 1 - lane;
-            const uint64_t found = __ballot(before >= 0 && a.begins[max(before, static_cast<int64_t>(0))] == 1u);
-            int64_t worker = last - __ffsll(static_cast<unsigned long long>(found));
+            const int before = last - 1 - lane;
+            const uint64_t found = __ballot(before >= 0 && a.begins[max(before, 0)] == 1u);
+            int worker = last - __ffsll(static_cast<unsigned long long>(found));
             if (found == 0) {
                 int64_t lo = 0, hi = *a.kept;
                 while (hi > lo) {
@@ -500,28 +501,28 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_rows(const GradArgs a) {
                     hi = min(hi, lo + smaller * width);
                     lo += (smaller - 1) * width + 1;
                 }
-                worker = lo / a.per;
+                worker = static_cast<int>(lo / a.per);
             }
             if (lane == 0) begun = worker;
         }
         __syncthreads();
-        const int64_t first = begun;
+        const int first = begun;
         // a piece per worker, but one for all workers of a workgroup that is wholly inside the row; the first worker's piece
         // begins the row: its second slot
-        const int64_t g0 = first / a.in_group, g1 = last / a.in_group;
-        const int64_t head = g0 == g1 ? last - first + 1 : (g0 + 1) * a.in_group - first, middle = g0 == g1 ? 0 : g1 - g0 - 1;
-        const int64_t pieces = g0 == g1 ? head : head + middle + last - g1 * a.in_group + 1;
-        auto piece = [&](const int64_t p) {
-            const int64_t worker = p < head ? first + p : p < head + middle ? (g0 + 1 + p - head) * a.in_group : g1 * a.in_group + (p - head - middle);
-            return a.part + (2 * worker + (p == 0 ? 1 : 0)) * a.dim + col;
+        const int g0 = first >> a.group_log2, g1 = last >> a.group_log2;
+        const int head = g0 == g1 ? last - first + 1 : ((g0 + 1) << a.group_log2) - first, inner = g0 == g1 ? head : head + g1 - g0 - 1;
+        const int pieces = g0 == g1 ? head : inner + last - (g1 << a.group_log2) + 1;
+        auto piece = [&](const int p) {
+            const int worker = p < head ? first + p : p < inner ? (g0 + 1 + p - head) << a.group_log2 : (g1 << a.group_log2) + (p - inner);
+            return a.part + (2 * static_cast<int64_t>(worker) + (p == 0 ? 1 : 0)) * a.dim + col;
         };
         double s[VE] = {};
         if (unit < a.dim) {
-            for (int64_t p0 = group; p0 < pieces; p0 += groups * JOIN_AHEAD) {
+            for (int p0 = group; p0 < pieces; p0 += groups * JOIN_AHEAD) {
                 Vec<SPARC_F32, VE> v[JOIN_AHEAD];
 #pragma unroll
                 for (int j = 0; j < JOIN_AHEAD; ++j) {
-                    const int64_t p = p0 + j * groups;
+                    const int p = p0 + j * groups;
                     if (p < pieces) v[j].load(piece(p));
                 }
 #pragma unroll
@@ -1100,7 +1101,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         a = carve(p, n, static_cast<int>(dim), ws, ws_bytes, &ok, &used);
         if (!ws || !ok) return SPARC_ERR_WS;
         a.per = p.per;
-        a.in_group = p.in_group;
+        while (1 << a.group_log2 < p.in_group) ++a.group_log2;
         a.long_row = p.long_row;
     }
     a.ids = ids;
