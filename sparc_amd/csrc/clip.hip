@@ -6,7 +6,7 @@
 // the conversion is free behind the loads.  A pass over the gradients leaves one partial sum per workgroup (at most
 // PARTS of them, in the grid's order); whoever needs the coefficient adds them up itself, every workgroup the same
 // numbers in the same order, so there is neither a launch nor an arrival counter between the two passes and runs repeat
-// bit for bit.
+// bit for bit.  Short lists take one launch (clip_once_kernel, adam_once_kernel).
 //
 // Measured.  629 MB of float32 (a table and an MLP): norm 100 us = 6.3 TB/s, scaling 194 us = 6.5 TB/s; plain accesses:
 // 161 and 204 us, because what the norm's pass leaves in the Infinity Cache is gone when the scaling comes to it, and what
@@ -156,9 +156,15 @@ struct Clip {
     int n_parts;
 };
 
+// A norm that is not finite gives what the formula gives: 0 for an infinite one (so infinite gradients become NaN), NaN for
+// NaN; an infinite max_norm never clips.
+__device__ __forceinline__ float coefficient_of(const double norm, const double max_norm) {
+    const double coef = isinf(max_norm) ? 1.0 : max_norm / (norm + 1e-6);
+    return coef >= 1.0 ? 1.f : static_cast<float>(coef);
+}
+
 // The coefficient, in every thread: the partial sums are requested first of all, and added up where the coefficient is first
-// asked for, behind the loads that do not need it.  A norm that is not finite gives what the formula gives: 0 for an infinite one (so infinite gradients become NaN), NaN for NaN; an
-// infinite max_norm never clips.
+// asked for, behind the loads that do not need it.
 struct Coefficient {
     const Clip& c;
     double* lds;
@@ -175,8 +181,7 @@ struct Coefficient {
         if (!known) {
             const double norm = sqrt(block_sum(parts, lds));
             if (c.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *c.norm_out = static_cast<float>(norm);
-            const double coef = isinf(c.max_norm) ? 1.0 : c.max_norm / (norm + 1e-6);
-            value = coef >= 1.0 ? 1.f : static_cast<float>(coef);
+            value = coefficient_of(norm, c.max_norm);
             known = true;
         }
         return value;
@@ -316,6 +321,182 @@ __global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, 
     c.get();   // (a list without elements has a norm too)
 }
 
+// ---- short lists in one launch ----------------------------------------------------------------------------
+
+// One workgroup holds the whole list in registers: squares, their sum, the coefficient, and back.  A launch less, of the two
+// that a call with little data mostly consists of.  Blocks of a tensor go to the waves in turn.  A call among others and one
+// that is waited for, two launches and one: clipping 6000 floats 13.8, 23.6 us and 10.4, 20.6; 128 KiB of bfloat16 13.6, 23.8
+// and 10.0, 24.0; 256 KiB 13.7, 24.0 and 11.6, 27.7, hence the limit of 128.  Adam on 6000 parameters 15.0, 25.0 and 11.5, 22.6;
+// on 16384 14.8, 24.9 and 11.0, 26.2.
+constexpr int ONCE_WAVES = 16, ONCE_THREADS = 64 * ONCE_WAVES, ONCE_TURNS = 4, ONCE_BLOCKS = ONCE_WAVES * ONCE_TURNS;
+constexpr int ONCE_VECTORS = 2, ONCE_BYTES = 64 * 16 * ONCE_VECTORS;   // of a block of the clipping
+constexpr int ONCE_ELEMS = 64 * 4;                                     // of a block of the Adam step
+typedef uint32_t Raw __attribute__((ext_vector_type(4)));              // 16 bytes of a gradient, whatever the type
+
+template <int DT>
+struct OnceBlock {
+    typedef typename Elem<DT>::type T;
+    static constexpr int VE = 16 / sizeof(T);
+    typedef Vec<DT, VE> V;
+    T* g;
+    int64_t left;   // elements from this lane's first on
+    __device__ __forceinline__ OnceBlock(void* p, const int64_t n, const int64_t k) {
+        const int64_t e = k * (ONCE_BYTES / static_cast<int>(sizeof(T))) + (threadIdx.x & 63) * VE;
+        g = static_cast<T*>(p) + e;
+        left = n - e;
+    }
+    __device__ __forceinline__ void load(Raw* r) const {
+#pragma unroll
+        for (int j = 0; j < ONCE_VECTORS; ++j) {
+            V v;
+            const int64_t here = left - j * 64 * VE;
+            if (here >= VE) v.load(g + j * 64 * VE);
+            else {   // the tensor's end
+#pragma unroll
+                for (int c = 0; c < VE; ++c) v.v[c] = c < here ? g[j * 64 * VE + c] : Elem<DT>::down(0.f);
+            }
+            r[j] = __builtin_bit_cast(Raw, v);
+        }
+    }
+    static __device__ __forceinline__ double squares(const Raw* r) {
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < ONCE_VECTORS; ++j) {
+            const V v = __builtin_bit_cast(V, r[j]);
+#pragma unroll
+            for (int c = 0; c < VE; ++c) {
+                const double x = v.get(c);
+                s = fma(x, x, s);
+            }
+        }
+        return s;
+    }
+    __device__ __forceinline__ void store(const Raw* r, const float coef) const {
+#pragma unroll
+        for (int j = 0; j < ONCE_VECTORS; ++j) {
+            V v = __builtin_bit_cast(V, r[j]);
+#pragma unroll
+            for (int c = 0; c < VE; ++c) v.set(c, v.get(c) * coef);
+            const int64_t here = left - j * 64 * VE;
+            if (here >= VE) v.store(g + j * 64 * VE);
+            else {
+#pragma unroll
+                for (int c = 0; c < VE; ++c)
+                    if (c < here) g[j * 64 * VE + c] = v.v[c];
+            }
+        }
+    }
+};
+
+// The coefficient of the workgroup's sum of squares; the norm goes to *norm_out.
+__device__ __forceinline__ float once_coefficient(double s, double* lds, const double max_norm, float* norm_out) {
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = lds[0];
+#pragma unroll
+    for (int w = 1; w < ONCE_WAVES; ++w) s += lds[w];
+    const double norm = sqrt(s);
+    if (threadIdx.x == 0) *norm_out = static_cast<float>(norm);
+    return coefficient_of(norm, max_norm);
+}
+
+__global__ __launch_bounds__(ONCE_THREADS) void clip_once_kernel(const GradArgs a, const double max_norm, float* norm_out) {
+    __shared__ double lds[ONCE_WAVES];
+    const Records records(a);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Raw r[ONCE_TURNS][ONCE_VECTORS];
+    auto each = [&](auto&& f) {
+#pragma unroll
+        for (int t = 0; t < ONCE_TURNS; ++t) {
+            const int b = wave + t * ONCE_WAVES;
+            if (b >= a.blocks) break;
+            void* p;
+            int64_t n, k;
+            int dtype;
+            records.find(b, &p, &n, &dtype, &k);
+            if (dtype == SPARC_F32) f(OnceBlock<SPARC_F32>(p, n, k), r[t]);
+            else if (dtype == SPARC_BF16) f(OnceBlock<SPARC_BF16>(p, n, k), r[t]);
+            else f(OnceBlock<SPARC_F16>(p, n, k), r[t]);
+        }
+    };
+    each([](const auto& block, Raw* v) { block.load(v); });
+    double s = 0.0;
+    each([&s](const auto& block, Raw* v) { s += block.squares(v); });
+    const float coef = once_coefficient(s, lds, max_norm, norm_out);
+    each([coef](const auto& block, Raw* v) { block.store(v, coef); });
+}
+
+__global__ __launch_bounds__(ONCE_THREADS) void adam_once_kernel(const AdamClipArgs a, const double max_norm, float* norm_out) {
+    __shared__ double lds[ONCE_WAVES];
+    typedef Vec<SPARC_F32, 4> V4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const sparc_adam_tensor_t mine = a.t[lane];
+    const int32_t first = a.first_block[lane];
+    V4 p[ONCE_TURNS] = {}, g[ONCE_TURNS] = {}, m[ONCE_TURNS] = {}, v[ONCE_TURNS] = {};
+    float *tp[ONCE_TURNS], *tm[ONCE_TURNS], *tv[ONCE_TURNS];
+    int64_t left[ONCE_TURNS];
+    double s = 0.0;
+#pragma unroll
+    for (int t = 0; t < ONCE_TURNS; ++t) {
+        const int b = wave + t * ONCE_WAVES;
+        if (b >= a.blocks) break;
+        const int of = __popcll(__ballot(first <= b)) - 1;
+        const int64_t e = static_cast<int64_t>(b - __builtin_amdgcn_readlane(first, of)) * ONCE_ELEMS + lane * 4;
+        left[t] = lane_value(mine.n, of) - e;
+        const float* tg = reinterpret_cast<const float*>(lane_value(reinterpret_cast<int64_t>(mine.g), of)) + e;
+        tp[t] = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.p), of)) + e;
+        tm[t] = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.m), of)) + e;
+        tv[t] = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.v), of)) + e;
+        if (left[t] >= 4) {
+            g[t].load(tg);
+            p[t].load(tp[t]);
+            m[t].load(tm[t]);
+            v[t].load(tv[t]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (i < left[t]) {
+                    g[t].v[i] = tg[i];
+                    p[t].v[i] = tp[t][i];
+                    m[t].v[i] = tm[t][i];
+                    v[t].v[i] = tv[t][i];
+                }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < ONCE_TURNS; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double x = g[t].v[i];
+            s = fma(x, x, s);
+        }
+    const float coef = once_coefficient(s, lds, max_norm, norm_out);
+#pragma unroll
+    for (int t = 0; t < ONCE_TURNS; ++t) {
+        if (wave + t * ONCE_WAVES >= a.blocks) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float pi = p[t].v[i], mi = m[t].v[i], vi = v[t].v[i];
+            adam_one(pi, g[t].v[i], mi, vi, a, coef);
+            p[t].v[i] = pi; m[t].v[i] = mi; v[t].v[i] = vi;
+        }
+        if (left[t] >= 4) {
+            p[t].store(tp[t]);
+            m[t].store(tm[t]);
+            v[t].store(tv[t]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (i < left[t]) {
+                    tp[t][i] = p[t].v[i];
+                    tm[t][i] = m[t].v[i];
+                    tv[t][i] = v[t].v[i];
+                }
+        }
+    }
+}
+
 bool grads_ok(const int64_t n_tensors, const sparc_grad_tensor_t* t) {
     if (n_tensors < 0 || (n_tensors > 0 && !t)) return false;
     for (int64_t i = 0; i < n_tensors; ++i)
@@ -350,10 +531,14 @@ size_t parts_bytes_of(const int64_t n_tensors) {
     return static_cast<size_t>(launches > 0 ? launches : 1) * PARTS * sizeof(double);
 }
 
+bool parts_ok(const int64_t n_tensors, const double* parts, const size_t bytes) {
+    return bytes >= parts_bytes_of(n_tensors) && (reinterpret_cast<uintptr_t>(parts) & 7) == 0;
+}
+
 // The partial sums of the tensors t(0) ... t(n_tensors - 1), checked by the caller.
 template <typename F>
 int launch_norm(const int64_t n_tensors, F&& t, double* parts, const size_t parts_bytes, int64_t* n_parts, sparc_stream_t stream) {
-    if (parts_bytes < parts_bytes_of(n_tensors) || (reinterpret_cast<uintptr_t>(parts) & 7)) return SPARC_ERR_WS;
+    if (!parts_ok(n_tensors, parts, parts_bytes)) return SPARC_ERR_WS;
     int64_t total = 0, left = 0;
     int launches = 0;
     for (int64_t i = 0; i < n_tensors; ++i) left += bytes_of(t(i));
@@ -391,29 +576,33 @@ bool adam_ok(const int64_t n_tensors, const sparc_adam_tensor_t* t, const AdamRa
     return true;
 }
 
+// The first ADAM_MOST of the n tensors t as kernel arguments, in fewer than 2^30 blocks.
+void fill(AdamClipArgs& a, const sparc_adam_tensor_t* t, const int64_t n, const AdamRates& r, const int block_elems) {
+    const double bc1 = 1.0 - pow(r.beta1, static_cast<double>(r.step)), bc2 = 1.0 - pow(r.beta2, static_cast<double>(r.step));
+    int64_t blocks = 0;
+    for (int i = 0; i < ADAM_MOST; ++i) {
+        a.t[i] = i < n ? t[i] : sparc_adam_tensor_t{};
+        a.first_block[i] = i < n ? static_cast<int32_t>(blocks) : INT32_MAX;
+        blocks += (a.t[i].n + block_elems - 1) / block_elems;
+    }
+    a.blocks = static_cast<int>(blocks);
+    a.step_size = static_cast<float>(r.lr / bc1);
+    a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
+    a.beta2 = static_cast<float>(r.beta2);
+    a.one_minus_beta1 = static_cast<float>(1.0 - r.beta1);
+    a.one_minus_beta2 = static_cast<float>(1.0 - r.beta2);
+    a.eps = static_cast<float>(r.eps);
+    a.weight_decay = static_cast<float>(r.weight_decay);
+}
+
 int launch_adam(const int64_t n_tensors, const sparc_adam_tensor_t* tensors, const AdamRates& r, Clip c, sparc_stream_t stream) {
     int64_t all = 0;
     for (int64_t i = 0; i < n_tensors; ++i) all += tensors[i].n;
-    const double bc1 = 1.0 - pow(r.beta1, static_cast<double>(r.step)), bc2 = 1.0 - pow(r.beta2, static_cast<double>(r.step));
     for (int64_t from = 0; from < n_tensors || from == 0; from += ADAM_MOST) {
         AdamClipArgs a;
-        int64_t blocks = 0;   // below 2^30
-        for (int i = 0; i < ADAM_MOST; ++i) {
-            const bool real = from + i < n_tensors;
-            a.t[i] = real ? tensors[from + i] : sparc_adam_tensor_t{};
-            a.first_block[i] = real ? static_cast<int32_t>(blocks) : INT32_MAX;
-            blocks += (a.t[i].n + ADAM_ELEMS - 1) / ADAM_ELEMS;
-        }
-        a.blocks = static_cast<int>(blocks);
-        a.step_size = static_cast<float>(r.lr / bc1);
-        a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
-        a.beta2 = static_cast<float>(r.beta2);
-        a.one_minus_beta1 = static_cast<float>(1.0 - r.beta1);
-        a.one_minus_beta2 = static_cast<float>(1.0 - r.beta2);
-        a.eps = static_cast<float>(r.eps);
-        a.weight_decay = static_cast<float>(r.weight_decay);
-        if (blocks == 0 && !c.norm_out) continue;
-        const int grid = static_cast<int>(blocks < 1 ? 1 : blocks < MOST_BLOCKS ? blocks : MOST_BLOCKS);
+        fill(a, tensors + from, n_tensors - from, r, ADAM_ELEMS);
+        if (a.blocks == 0 && !c.norm_out) continue;
+        const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
         if (16 * all > KEEP_BYTES) hipLaunchKernelGGL(adam_clip_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
         else hipLaunchKernelGGL(adam_clip_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
         SPARC_CHECK_LAUNCH();
@@ -434,7 +623,17 @@ extern "C" int sparc_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* ten
 
 extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t* tensors, double max_norm, double* parts,
                                     size_t parts_bytes, float* norm_out, sparc_stream_t stream) {
-    if (!norm_out || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
+    if (!norm_out || !(max_norm >= 0.0) || !parts || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
+    if (!parts_ok(n_tensors, parts, parts_bytes)) return SPARC_ERR_WS;
+    int64_t once = 0;
+    for (int64_t i = 0; i < n_tensors && once <= ONCE_BLOCKS; ++i) once += (bytes_of(tensors[i]) + ONCE_BYTES - 1) / ONCE_BYTES;
+    if (n_tensors <= SPARC_GRAD_MAX_TENSORS && once <= ONCE_BLOCKS) {
+        GradArgs a;
+        fill(a, [&](int64_t k) { return tensors[k]; }, 0, static_cast<int>(n_tensors), ONCE_BYTES, 0);
+        hipLaunchKernelGGL(clip_once_kernel, dim3(1), dim3(ONCE_THREADS), 0, stream, a, max_norm, norm_out);
+        SPARC_CHECK_LAUNCH();
+        return SPARC_OK;
+    }
     int64_t n_parts = 0;
     const int rc = sparc_grad_norm(n_tensors, tensors, parts, parts_bytes, &n_parts, stream);
     if (rc != SPARC_OK) return rc;
@@ -470,6 +669,16 @@ extern "C" int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t
                                     size_t parts_bytes, float* norm_out, sparc_stream_t stream) {
     const AdamRates rates = {lr, beta1, beta2, eps, weight_decay, step};
     if (!adam_ok(n_tensors, tensors, rates) || !parts || !norm_out || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
+    if (!parts_ok(n_tensors, parts, parts_bytes)) return SPARC_ERR_WS;
+    int64_t once = 0;
+    for (int64_t i = 0; i < n_tensors && once <= ONCE_BLOCKS; ++i) once += (tensors[i].n + ONCE_ELEMS - 1) / ONCE_ELEMS;
+    if (n_tensors <= ADAM_MOST && once <= ONCE_BLOCKS) {
+        AdamClipArgs a;
+        fill(a, tensors, n_tensors, rates, ONCE_ELEMS);
+        hipLaunchKernelGGL(adam_once_kernel, dim3(1), dim3(ONCE_THREADS), 0, stream, a, max_norm, norm_out);
+        SPARC_CHECK_LAUNCH();
+        return SPARC_OK;
+    }
     int64_t n_parts = 0;
     auto gradient = [&](int64_t i) { return sparc_grad_tensor_t{const_cast<float*>(tensors[i].g), tensors[i].n, SPARC_F32}; };
     const int rc = launch_norm(n_tensors, gradient, parts, parts_bytes, &n_parts, stream);

@@ -292,3 +292,41 @@ def test_what_is_written_counts_as_written():
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         penalty.backward()
     p.grad = None
+
+
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 5], [16384], [255, 256, 257, 1023], [131072], [2048] * 60, [1] * 64, [1] * 65, [131073], [7, 2049, 100_001],
+                                   [256] * 64, [257] * 32, [16385], [0, 0], [32768],
+                                   [32769], [65536], [65537], [1024] * 32, [1023] * 64])
+def test_short_lists_and_the_first_longer_ones(sizes):
+    """What one workgroup holds (128 KiB of gradients to clip, 16384 parameters to update) and what is just beyond it."""
+    from sparc_amd.optim import adam_step_, clip_grad_norm_
+    bucket = {d: torch.randn(sum(sizes) + len(sizes) + 1, device="cuda", generator=gen(5)).to(d) for d in (F32, BF16, F16)}
+    for kinds in ([F32], [BF16], [F16], [F32, BF16, F16]):
+        for odd in (0, 1):                                     # one after another in memory, at any element
+            views, at = [], 0
+            kept = {d: t.clone() for d, t in bucket.items()}
+            for i, s in enumerate(sizes):
+                views.append(kept[kinds[i % len(kinds)]][at + odd:at + odd + s])
+                at += s + 1
+            check_clip(views, 0.25)
+            touched = {d: torch.ones(t.numel(), dtype=torch.bool, device="cuda") for d, t in kept.items()}
+            at = 0
+            for i, s in enumerate(sizes):
+                touched[kinds[i % len(kinds)]][at + odd:at + odd + s] = False
+                at += s + 1
+            assert all(torch.equal(kept[d][touched[d]], bucket[d][touched[d]]) for d in kept)
+    new = lambda seed: [torch.randn(s, device="cuda", generator=gen(seed + i)) for i, s in enumerate(sizes)]  # noqa: E731
+    p, g, m = new(100), new(200), new(300)
+    v = [t * t for t in new(400)]
+    want = norm64(g)
+    before = [[t.clone() for t in c] for c in (p, g, m, v)]
+    norm = adam_step_(p, g, m, v, 3, lr=0.01, weight_decay=0.02, max_grad_norm=0.5)
+    assert abs(float(norm) - want) <= SLACK * U * want + 2.0 ** -149
+    coef = min(1.0, 0.5 / (want + 1e-6))
+    for i in range(len(sizes)):
+        if sizes[i] == 0:
+            continue
+        exact, bounds = adam_bounds(*(c[i] for c in before), coef, 3, 0.01, 0.9, 0.999, 1e-8, 0.02)
+        for got, w, off in zip((p[i], m[i], v[i]), exact, bounds):
+            assert bool(((got.double() - w).abs() <= off + 1e-37).all())
+        assert torch.equal(g[i], before[1][i])
