@@ -738,7 +738,7 @@ __device__ __forceinline__ void radix_sort(uint32_t* keys, const int count, cons
 
 __global__ __launch_bounds__(SORT_BLOCK) void zeros_kernel(const Zeros z) { write_zeros(z, blockIdx.x, gridDim.x); }
 
-// zeros: write them here, too.  64 registers, or a third workgroup would wait for a whole round: 4101 tokens over 451 rows of 359
+// zeros: write them here, too.  64 to 66 registers, or a third workgroup would wait for a whole round: 4101 tokens over 451 rows of 359
 // floats, 768 workgroups, 21.7 us with 84 registers, 15.6 with 64, 14.4 with 384 workgroups.
 template <int DT, int VE>
 __global__ __launch_bounds__(FEW_THREADS, 6) void few_tokens(const GradArgs a, const Dealt dealt, const int lanes_log2, const bool zeros) {
