@@ -14,7 +14,7 @@
 // plainly for the scaling, which goes backwards: 94 and 205 us.  Lists below 192 MB stay plain: 160 MB, three lists in turn, 80 us
 // streamed, 93 us plain; one list again and again 80 and 72 us.
 // 6.4 MB (the MLP alone): 4.0 + 6.0 us, of which launches and the chain parts -> sum -> root -> quotient are most; the
-// host's two launches and checks take longer (16.0 us a call).
+// host's two launches and checks take longer (17.0 us a call).
 // Adam on 31.5 M floats (883 MB): norm 24 us, update 136 us = 6.5 TB/s; plain accesses 40 and 160 us.  Below 192 MB plain:
 // 8 M floats 49.1 us streamed, 49.7 us plain; 4 M 27.8 and 25.1.
 #include "elem.h"
