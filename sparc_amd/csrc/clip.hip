@@ -14,9 +14,11 @@
 // plainly for the scaling, which goes backwards: 94 and 205 us.  Lists below 192 MB stay plain: 160 MB, three lists in turn, 80 us
 // streamed, 93 us plain; one list again and again 80 and 72 us.
 // 6.4 MB (the MLP alone): 4.0 + 6.0 us, of which launches and the chain parts -> sum -> root -> quotient are most; the
-// host's two launches and checks take longer (17.0 us a call).
+// host's two launches and checks take longer (16.3 us a call).
 // Adam on 31.5 M floats (883 MB): norm 24 us, update 136 us = 6.5 TB/s; plain accesses 40 and 160 us.  Below 192 MB plain:
 // 8 M floats 49.1 us streamed, 49.7 us plain; 4 M 27.8 and 25.1.
+#include <type_traits>
+
 #include "elem.h"
 
 namespace {
@@ -32,10 +34,14 @@ constexpr int ADAM_MOST = 64;        // tensors per launch of the Adam step
 // accesses, but for their last KEEP_BYTES in the norm's pass, which the scaling, going backwards, finds there.
 constexpr int64_t KEEP_BYTES = SPARC_KEEP_BYTES;
 
+// Arguments of 2.5 KiB make a launch 0.9 us longer than some of 0.4 (4.1, 2.9 to 3.5 us): short lists have records for SHORT.
+constexpr int SHORT = 16;
+
+template <int R>
 struct GradArgs {
-    void* p[SPARC_GRAD_MAX_TENSORS];
-    int64_t n_dtype[SPARC_GRAD_MAX_TENSORS];           // elements << 2 | type
-    int32_t first_block[SPARC_GRAD_MAX_TENSORS];       // where tensor i's blocks begin; behind the last tensor: INT32_MAX
+    void* p[R];
+    int64_t n_dtype[R];           // elements << 2 | type
+    int32_t first_block[R];       // where tensor i's blocks begin; behind the last tensor: INT32_MAX
     int blocks, plain_from;                            // blocks from plain_from on are read without streaming
 };
 
@@ -45,27 +51,32 @@ __device__ __forceinline__ int64_t lane_value(const int64_t v, const int lane) {
 }
 
 // The records of a launch, one or two per lane: a search for a block's tensor is two ballots and no load.
+template <int R>
 struct Records {
-    int64_t p[2], n_dtype[2];
-    int32_t first[2];
-    __device__ __forceinline__ Records(const GradArgs& a) {
-        const int lane = threadIdx.x & 63;
+    static_assert(R <= 64 || R == 128, "one or two records per lane");
+    static constexpr int H = R > 64 ? 2 : 1;
+    int64_t p[H], n_dtype[H];
+    int32_t first[H];
+    __device__ __forceinline__ Records(const GradArgs<R>& a) {
+        const int lane = threadIdx.x & 63, own = lane < R ? lane : 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            p[h] = reinterpret_cast<int64_t>(a.p[lane + 64 * h]);
-            n_dtype[h] = a.n_dtype[lane + 64 * h];
-            first[h] = a.first_block[lane + 64 * h];
+        for (int h = 0; h < H; ++h) {
+            p[h] = reinterpret_cast<int64_t>(a.p[own + 64 * h]);
+            n_dtype[h] = a.n_dtype[own + 64 * h];
+            first[h] = lane < R ? a.first_block[own + 64 * h] : INT32_MAX;
         }
     }
     // Block b: its tensor, elements and type, and which of the tensor's blocks it is (all uniform).
     __device__ __forceinline__ void find(const int b, void** base, int64_t* n, int* dtype, int64_t* k) const {
-        const int t = __popcll(__ballot(first[0] <= b)) + __popcll(__ballot(first[1] <= b)) - 1;
-        const int h = t >> 6, lane = t & 63;
-        *base = reinterpret_cast<void*>(lane_value(h ? p[1] : p[0], lane));
-        const int64_t nd = lane_value(h ? n_dtype[1] : n_dtype[0], lane);
+        int t = __popcll(__ballot(first[0] <= b)) - 1;
+        if constexpr (H > 1) t += __popcll(__ballot(first[H - 1] <= b));
+        const bool upper = H > 1 && t >= 64;
+        const int lane = t & 63;
+        *base = reinterpret_cast<void*>(lane_value(upper ? p[H - 1] : p[0], lane));
+        const int64_t nd = lane_value(upper ? n_dtype[H - 1] : n_dtype[0], lane);
         *n = nd >> 2;
         *dtype = static_cast<int>(nd) & 3;
-        *k = b - __builtin_amdgcn_readlane(h ? first[1] : first[0], lane);
+        *k = b - __builtin_amdgcn_readlane(upper ? first[H - 1] : first[0], lane);
     }
 };
 
@@ -113,8 +124,8 @@ __device__ __forceinline__ double squares(const void* p, const int64_t n, const 
     return s;
 }
 
-template <bool STREAM>
-__device__ __forceinline__ double squares_of_block(const Records& records, const int b) {
+template <bool STREAM, int R>
+__device__ __forceinline__ double squares_of_block(const Records<R>& records, const int b) {
     void* p;
     int64_t n, k;
     int dtype;
@@ -123,9 +134,10 @@ __device__ __forceinline__ double squares_of_block(const Records& records, const
            : dtype == SPARC_BF16 ? squares<SPARC_BF16, STREAM>(p, n, k) : squares<SPARC_F16, STREAM>(p, n, k);
 }
 
-__global__ __launch_bounds__(NORM_THREADS, 8) void grad_squares_kernel(const GradArgs a, double* parts) {
+template <int R>
+__global__ __launch_bounds__(NORM_THREADS, 8) void grad_squares_kernel(const GradArgs<R> a, double* parts) {
     __shared__ double lds[NORM_THREADS / 64];
-    const Records records(a);
+    const Records<R> records(a);
     double s = 0.0;
     int b = blockIdx.x;
     for (; b < a.plain_from; b += gridDim.x) s += squares_of_block<true>(records, b);
@@ -229,11 +241,11 @@ __device__ __forceinline__ void scale_block(void* p, const int64_t n, const int6
 }
 
 // From the last block to the first: the norm's pass left the last ones in the cache.
-template <bool STREAM>
-__global__ __launch_bounds__(BLOCK) void grad_scale_kernel(const GradArgs a, const Clip clip) {
+template <bool STREAM, int R>
+__global__ __launch_bounds__(BLOCK) void grad_scale_kernel(const GradArgs<R> a, const Clip clip) {
     __shared__ double lds[BLOCK / 64];
     Coefficient c(clip, lds);
-    const Records records(a);
+    const Records<R> records(a);
     for (int b = a.blocks - 1 - static_cast<int>(blockIdx.x); b >= 0; b -= gridDim.x) {
         void* p;
         int64_t n, k;
@@ -246,15 +258,20 @@ __global__ __launch_bounds__(BLOCK) void grad_scale_kernel(const GradArgs a, con
     c.get();   // (a list without elements has a norm too)
 }
 
-struct AdamClipArgs {
-    sparc_adam_tensor_t t[ADAM_MOST];
-    int32_t first_block[ADAM_MOST];   // where tensor i's blocks begin; behind the last tensor: INT32_MAX
-    int blocks;
+struct AdamFactors {
     float step_size, bc2_rsqrt, beta2, one_minus_beta1, one_minus_beta2, eps, weight_decay;
 };
 
+template <int R>
+struct AdamClipArgs {
+    sparc_adam_tensor_t t[R];
+    int32_t first_block[R];   // where tensor i's blocks begin; behind the last tensor: INT32_MAX
+    int blocks;
+    AdamFactors by;
+};
+
 // The update of sparc_adam_step for the gradient c g.
-__device__ __forceinline__ void adam_one(float& p, const float g0, float& m, float& v, const AdamClipArgs& a, const float coef) {
+__device__ __forceinline__ void adam_one(float& p, const float g0, float& m, float& v, const AdamFactors& a, const float coef) {
     float g = coef * g0;
     if (a.weight_decay != 0.f) g = fmaf(a.weight_decay, p, g);
     m = fmaf(a.one_minus_beta1, g - m, m);
@@ -262,15 +279,15 @@ __device__ __forceinline__ void adam_one(float& p, const float g0, float& m, flo
     p -= a.step_size * (m / (sqrtf(v) * a.bc2_rsqrt + a.eps));
 }
 
-template <bool STREAM>
-__global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, const Clip clip) {
+template <bool STREAM, int R>
+__global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs<R> a, const Clip clip) {
     __shared__ double lds[BLOCK / 64];
     typedef Vec<SPARC_F32, 4> V4;
     Coefficient c(clip, lds);
     const int lane = threadIdx.x & 63;
-    const sparc_adam_tensor_t mine = a.t[lane];
-    const int32_t first = a.first_block[lane];
-    static_assert(ADAM_MOST == 64, "a record per lane");
+    const sparc_adam_tensor_t mine = a.t[lane < R ? lane : 0];
+    const int32_t first = lane < R ? a.first_block[lane < R ? lane : 0] : INT32_MAX;
+    static_assert(R <= 64, "a record per lane");
     for (int b = blockIdx.x; b < a.blocks; b += gridDim.x) {
         const int of = __popcll(__ballot(first <= b)) - 1;
         float* tp = reinterpret_cast<float*>(lane_value(reinterpret_cast<int64_t>(mine.p), of));
@@ -301,7 +318,7 @@ __global__ __launch_bounds__(BLOCK) void adam_clip_kernel(const AdamClipArgs a, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float pi = p.v[i], mi = m.v[i], vi = v.v[i];
-            adam_one(pi, g.v[i], mi, vi, a, coef);
+            adam_one(pi, g.v[i], mi, vi, a.by, coef);
             p.v[i] = pi; m.v[i] = mi; v.v[i] = vi;
         }
         if (whole) {
@@ -401,9 +418,10 @@ __device__ __forceinline__ float once_coefficient(double s, double* lds, const d
     return coefficient_of(norm, max_norm);
 }
 
-__global__ __launch_bounds__(ONCE_THREADS) void clip_once_kernel(const GradArgs a, const double max_norm, float* norm_out) {
+template <int R>
+__global__ __launch_bounds__(ONCE_THREADS) void clip_once_kernel(const GradArgs<R> a, const double max_norm, float* norm_out) {
     __shared__ double lds[ONCE_WAVES];
-    const Records records(a);
+    const Records<R> records(a);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Raw r[ONCE_TURNS][ONCE_VECTORS];
     auto each = [&](auto&& f) {
@@ -427,12 +445,13 @@ __global__ __launch_bounds__(ONCE_THREADS) void clip_once_kernel(const GradArgs 
     each([coef](const auto& block, Raw* v) { block.store(v, coef); });
 }
 
-__global__ __launch_bounds__(ONCE_THREADS) void adam_once_kernel(const AdamClipArgs a, const double max_norm, float* norm_out) {
+template <int R>
+__global__ __launch_bounds__(ONCE_THREADS) void adam_once_kernel(const AdamClipArgs<R> a, const double max_norm, float* norm_out) {
     __shared__ double lds[ONCE_WAVES];
     typedef Vec<SPARC_F32, 4> V4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const sparc_adam_tensor_t mine = a.t[lane];
-    const int32_t first = a.first_block[lane];
+    const sparc_adam_tensor_t mine = a.t[lane < R ? lane : 0];
+    const int32_t first = lane < R ? a.first_block[lane < R ? lane : 0] : INT32_MAX;
     V4 p[ONCE_TURNS] = {}, g[ONCE_TURNS] = {}, m[ONCE_TURNS] = {}, v[ONCE_TURNS] = {};
     float *tp[ONCE_TURNS], *tm[ONCE_TURNS], *tv[ONCE_TURNS];
     int64_t left[ONCE_TURNS];
@@ -478,7 +497,7 @@ __global__ __launch_bounds__(ONCE_THREADS) void adam_once_kernel(const AdamClipA
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float pi = p[t].v[i], mi = m[t].v[i], vi = v[t].v[i];
-            adam_one(pi, g[t].v[i], mi, vi, a, coef);
+            adam_one(pi, g[t].v[i], mi, vi, a.by, coef);
             p[t].v[i] = pi; m[t].v[i] = mi; v[t].v[i] = vi;
         }
         if (left[t] >= 4) {
@@ -508,10 +527,10 @@ int64_t bytes_of(const sparc_grad_tensor_t& t) { return t.n * (t.dtype == SPARC_
 
 // The `count` tensors t(from), t(from + 1) ... as kernel arguments.  Their number of blocks stays below 2^30
 // (SPARC_GRAD_MAX_ELEMS).  left: bytes of the list from there on.  Returns these tensors' bytes.
-template <typename F>
-int64_t fill(GradArgs& a, F&& t, const int64_t from, const int count, const int block_bytes, const int64_t left) {
+template <int R, typename F>
+int64_t fill(GradArgs<R>& a, F&& t, const int64_t from, const int count, const int block_bytes, const int64_t left) {
     int64_t blocks = 0, bytes = 0;
-    for (int i = 0; i < SPARC_GRAD_MAX_TENSORS; ++i) {
+    for (int i = 0; i < R; ++i) {
         const sparc_grad_tensor_t r = i < count ? t(from + i) : sparc_grad_tensor_t{nullptr, 0, 0};
         a.p[i] = r.p;
         a.n_dtype[i] = r.n << 2 | r.dtype;
@@ -524,6 +543,13 @@ int64_t fill(GradArgs& a, F&& t, const int64_t from, const int count, const int 
     const int64_t plain = keep <= 0 ? 0 : keep / block_bytes;
     a.plain_from = static_cast<int>(keep >= bytes || plain >= blocks ? 0 : blocks - plain);
     return bytes;
+}
+
+// f(the records of a launch that `count` of at most MOST tensors take, as an integral constant).
+template <int MOST, typename F>
+int with_records(const int64_t count, F&& f) {
+    if (count <= SHORT) return f(std::integral_constant<int, SHORT>());
+    return f(std::integral_constant<int, MOST>());
 }
 
 size_t parts_bytes_of(const int64_t n_tensors) {
@@ -543,15 +569,20 @@ int launch_norm(const int64_t n_tensors, F&& t, double* parts, const size_t part
     int launches = 0;
     for (int64_t i = 0; i < n_tensors; ++i) left += bytes_of(t(i));
     for (int64_t from = 0; from < n_tensors; from += SPARC_GRAD_MAX_TENSORS) {
-        GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
-        left -= fill(a, t, from, count, NORM_BYTES, left);
-        if (a.blocks == 0) continue;
-        const int grid = a.blocks < PARTS ? a.blocks : PARTS;
-        hipLaunchKernelGGL(grad_squares_kernel, dim3(grid), dim3(NORM_THREADS), 0, stream, a, parts + total);
-        SPARC_CHECK_LAUNCH();
-        total += grid;
-        ++launches;
+        const int rc = with_records<SPARC_GRAD_MAX_TENSORS>(count, [&](auto records) {
+            constexpr int R = decltype(records)::value;
+            GradArgs<R> a;
+            left -= fill(a, t, from, count, NORM_BYTES, left);
+            if (a.blocks == 0) return SPARC_OK;
+            const int grid = a.blocks < PARTS ? a.blocks : PARTS;
+            hipLaunchKernelGGL((grad_squares_kernel<R>), dim3(grid), dim3(NORM_THREADS), 0, stream, a, parts + total);
+            SPARC_CHECK_LAUNCH();
+            total += grid;
+            ++launches;
+            return SPARC_OK;
+        });
+        if (rc != SPARC_OK) return rc;
     }
     if (launches > 1) {
         hipLaunchKernelGGL(grad_parts_kernel, dim3(1), dim3(BLOCK), 0, stream, parts, total);
@@ -576,37 +607,43 @@ bool adam_ok(const int64_t n_tensors, const sparc_adam_tensor_t* t, const AdamRa
     return true;
 }
 
-// The first ADAM_MOST of the n tensors t as kernel arguments, in fewer than 2^30 blocks.
-void fill(AdamClipArgs& a, const sparc_adam_tensor_t* t, const int64_t n, const AdamRates& r, const int block_elems) {
+// The first R of the n tensors t as kernel arguments, in fewer than 2^30 blocks.
+template <int R>
+void fill(AdamClipArgs<R>& a, const sparc_adam_tensor_t* t, const int64_t n, const AdamRates& r, const int block_elems) {
     const double bc1 = 1.0 - pow(r.beta1, static_cast<double>(r.step)), bc2 = 1.0 - pow(r.beta2, static_cast<double>(r.step));
     int64_t blocks = 0;
-    for (int i = 0; i < ADAM_MOST; ++i) {
+    for (int i = 0; i < R; ++i) {
         a.t[i] = i < n ? t[i] : sparc_adam_tensor_t{};
         a.first_block[i] = i < n ? static_cast<int32_t>(blocks) : INT32_MAX;
         blocks += (a.t[i].n + block_elems - 1) / block_elems;
     }
     a.blocks = static_cast<int>(blocks);
-    a.step_size = static_cast<float>(r.lr / bc1);
-    a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
-    a.beta2 = static_cast<float>(r.beta2);
-    a.one_minus_beta1 = static_cast<float>(1.0 - r.beta1);
-    a.one_minus_beta2 = static_cast<float>(1.0 - r.beta2);
-    a.eps = static_cast<float>(r.eps);
-    a.weight_decay = static_cast<float>(r.weight_decay);
+    a.by.step_size = static_cast<float>(r.lr / bc1);
+    a.by.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));
+    a.by.beta2 = static_cast<float>(r.beta2);
+    a.by.one_minus_beta1 = static_cast<float>(1.0 - r.beta1);
+    a.by.one_minus_beta2 = static_cast<float>(1.0 - r.beta2);
+    a.by.eps = static_cast<float>(r.eps);
+    a.by.weight_decay = static_cast<float>(r.weight_decay);
 }
 
 int launch_adam(const int64_t n_tensors, const sparc_adam_tensor_t* tensors, const AdamRates& r, Clip c, sparc_stream_t stream) {
     int64_t all = 0;
     for (int64_t i = 0; i < n_tensors; ++i) all += tensors[i].n;
     for (int64_t from = 0; from < n_tensors || from == 0; from += ADAM_MOST) {
-        AdamClipArgs a;
-        fill(a, tensors + from, n_tensors - from, r, ADAM_ELEMS);
-        if (a.blocks == 0 && !c.norm_out) continue;
-        const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
-        if (16 * all > KEEP_BYTES) hipLaunchKernelGGL(adam_clip_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
-        else hipLaunchKernelGGL(adam_clip_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
-        SPARC_CHECK_LAUNCH();
-        c.norm_out = nullptr;
+        const int rc = with_records<ADAM_MOST>(n_tensors - from, [&](auto records) {
+            constexpr int R = decltype(records)::value;
+            AdamClipArgs<R> a;
+            fill(a, tensors + from, n_tensors - from, r, ADAM_ELEMS);
+            if (a.blocks == 0 && !c.norm_out) return SPARC_OK;
+            const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
+            if (16 * all > KEEP_BYTES) hipLaunchKernelGGL((adam_clip_kernel<true, R>), dim3(grid), dim3(BLOCK), 0, stream, a, c);
+            else hipLaunchKernelGGL((adam_clip_kernel<false, R>), dim3(grid), dim3(BLOCK), 0, stream, a, c);
+            SPARC_CHECK_LAUNCH();
+            c.norm_out = nullptr;
+            return SPARC_OK;
+        });
+        if (rc != SPARC_OK) return rc;
     }
     return SPARC_OK;
 }
@@ -628,11 +665,14 @@ extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t
     int64_t once = 0;
     for (int64_t i = 0; i < n_tensors && once <= ONCE_BLOCKS; ++i) once += (bytes_of(tensors[i]) + ONCE_BYTES - 1) / ONCE_BYTES;
     if (n_tensors <= SPARC_GRAD_MAX_TENSORS && once <= ONCE_BLOCKS) {
-        GradArgs a;
-        fill(a, [&](int64_t k) { return tensors[k]; }, 0, static_cast<int>(n_tensors), ONCE_BYTES, 0);
-        hipLaunchKernelGGL(clip_once_kernel, dim3(1), dim3(ONCE_THREADS), 0, stream, a, max_norm, norm_out);
-        SPARC_CHECK_LAUNCH();
-        return SPARC_OK;
+        return with_records<SPARC_GRAD_MAX_TENSORS>(n_tensors, [&](auto records) {
+            constexpr int R = decltype(records)::value;
+            GradArgs<R> a;
+            fill(a, [&](int64_t k) { return tensors[k]; }, 0, static_cast<int>(n_tensors), ONCE_BYTES, 0);
+            hipLaunchKernelGGL((clip_once_kernel<R>), dim3(1), dim3(ONCE_THREADS), 0, stream, a, max_norm, norm_out);
+            SPARC_CHECK_LAUNCH();
+            return SPARC_OK;
+        });
     }
     int64_t n_parts = 0;
     const int rc = sparc_grad_norm(n_tensors, tensors, parts, parts_bytes, &n_parts, stream);
@@ -642,16 +682,21 @@ extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t
     const int64_t launches = n_tensors ? (n_tensors + SPARC_GRAD_MAX_TENSORS - 1) / SPARC_GRAD_MAX_TENSORS : 1;
     for (int64_t i = launches - 1; i >= 0; --i) {   // backwards, as inside a launch
         const int64_t from = i * SPARC_GRAD_MAX_TENSORS;
-        GradArgs a;
         const int count = static_cast<int>(n_tensors - from < SPARC_GRAD_MAX_TENSORS ? n_tensors - from : SPARC_GRAD_MAX_TENSORS);
         for (int k = 0; k < count; ++k) left += bytes_of(tensors[from + k]);
-        fill(a, [&](int64_t k) { return tensors[k]; }, from, count, BLOCK_BYTES, left);
-        if (a.blocks == 0 && !c.norm_out) continue;
-        const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
-        if (a.plain_from > 0) hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
-        else hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(grid), dim3(BLOCK), 0, stream, a, c);
-        SPARC_CHECK_LAUNCH();
-        c.norm_out = nullptr;
+        const int rc = with_records<SPARC_GRAD_MAX_TENSORS>(count, [&](auto records) {
+            constexpr int R = decltype(records)::value;
+            GradArgs<R> a;
+            fill(a, [&](int64_t k) { return tensors[k]; }, from, count, BLOCK_BYTES, left);
+            if (a.blocks == 0 && !c.norm_out) return SPARC_OK;
+            const int grid = a.blocks < 1 ? 1 : a.blocks < MOST_BLOCKS ? a.blocks : MOST_BLOCKS;
+            if (a.plain_from > 0) hipLaunchKernelGGL((grad_scale_kernel<true, R>), dim3(grid), dim3(BLOCK), 0, stream, a, c);
+            else hipLaunchKernelGGL((grad_scale_kernel<false, R>), dim3(grid), dim3(BLOCK), 0, stream, a, c);
+            SPARC_CHECK_LAUNCH();
+            c.norm_out = nullptr;
+            return SPARC_OK;
+        });
+        if (rc != SPARC_OK) return rc;
     }
     return SPARC_OK;
 }
@@ -673,11 +718,14 @@ extern "C" int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t
     int64_t once = 0;
     for (int64_t i = 0; i < n_tensors && once <= ONCE_BLOCKS; ++i) once += (tensors[i].n + ONCE_ELEMS - 1) / ONCE_ELEMS;
     if (n_tensors <= ADAM_MOST && once <= ONCE_BLOCKS) {
-        AdamClipArgs a;
-        fill(a, tensors, n_tensors, rates, ONCE_ELEMS);
-        hipLaunchKernelGGL(adam_once_kernel, dim3(1), dim3(ONCE_THREADS), 0, stream, a, max_norm, norm_out);
-        SPARC_CHECK_LAUNCH();
-        return SPARC_OK;
+        return with_records<ADAM_MOST>(n_tensors, [&](auto records) {
+            constexpr int R = decltype(records)::value;
+            AdamClipArgs<R> a;
+            fill(a, tensors, n_tensors, rates, ONCE_ELEMS);
+            hipLaunchKernelGGL((adam_once_kernel<R>), dim3(1), dim3(ONCE_THREADS), 0, stream, a, max_norm, norm_out);
+            SPARC_CHECK_LAUNCH();
+            return SPARC_OK;
+        });
     }
     int64_t n_parts = 0;
     auto gradient = [&](int64_t i) { return sparc_grad_tensor_t{const_cast<float*>(tensors[i].g), tensors[i].n, SPARC_F32}; };
