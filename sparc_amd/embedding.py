@@ -96,6 +96,14 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
 _BORN_ON = "sparc_amd.stream"
 
 
+def refuse_capture_beside_eager_graph(node) -> None:
+    """Raises if a leaf's node was made on the default stream: the backward that is to be captured would let that stream,
+    which cannot be captured, wait for the capture, and the process would end."""
+    if node.metadata.get(_BORN_ON) == 0:
+        raise RuntimeError("embedding_lookup: a backward is to be captured while the graph of an earlier lookup in the same table, "
+                           "made on the default stream, is alive. Drop what holds it (its outputs, its loss) before capturing")
+
+
 class EmbeddingLookup(torch.autograd.Function):
     """Arguments ids, table, scale, padding_idx; gradient for the table."""
 
@@ -111,10 +119,8 @@ class EmbeddingLookup(torch.autograd.Function):
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
         leaf = ctx.next_functions[1][0]
-        if leaf.metadata.get(_BORN_ON) == 0 and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("embedding_lookup: a backward is being captured while the graph of an earlier lookup in the same "
-                               "table, made on the default stream, is alive: autograd would have that stream, which cannot be "
-                               "captured, wait for the capture. Drop what holds it (its outputs, its loss) before capturing")
+        if _BORN_ON in leaf.metadata and torch.cuda.is_current_stream_capturing():
+            refuse_capture_beside_eager_graph(leaf)
         return None, embedding_grad(ids, g, ctx.rows, ctx.scale, ctx.padding_idx), None, None
 
 

@@ -19,6 +19,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from .embedding import refuse_capture_beside_eager_graph
 from .graph import Workspace
 from .ops import LapLoss
 from .optim import clip_grad_norm_
@@ -84,6 +85,9 @@ class GraphedSteps:
             self.net.orthonorm_weights = self.orth
             return loss.clone()
         if hit is None:
+            table = getattr(self.net, "node_table", None)
+            if table is not None:
+                refuse_capture_beside_eager_graph(torch.autograd.graph.get_gradient_edge(table.weight).node)
             # the pair's first step runs eagerly on a side stream (it sizes the workspace and configures the
             # kernels); the capture that follows records the pair's NEXT step without executing it
             side = torch.cuda.Stream(device=self.device)

@@ -330,3 +330,33 @@ def test_short_lists_and_the_first_longer_ones(sizes):
         for got, w, off in zip((p[i], m[i], v[i]), exact, bounds):
             assert bool(((got.double() - w).abs() <= off + 1e-37).all())
         assert torch.equal(g[i], before[1][i])
+
+
+@pytest.mark.parametrize("sizes", [[300, 5], [70_001, 33], [64] * 20])
+def test_adam_step_captured_and_on_another_stream(sizes):
+    """Replays with new gradients, eager work between them: the same bits as eager calls (the number of the step is the
+    capture's)."""
+    from sparc_amd.optim import adam_step_, clip_grad_norm_
+    new = lambda seed: [torch.randn(s, device="cuda", generator=gen(seed + i)) for i, s in enumerate(sizes)]  # noqa: E731
+    p, g, m, v = new(1), new(2), new(3), [t * t for t in new(4)]
+    q, n, w = ([t.clone() for t in c] for c in (p, m, v))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = adam_step_(p, g, m, v, 5, lr=0.02, max_grad_norm=0.7)
+    for turn in range(4):
+        fresh = new(10 * turn + 20)
+        for a, b in zip(g, fresh):
+            a.copy_(b)
+        graph.replay()
+        if turn % 2:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+                eager = adam_step_(q, fresh, n, w, 5, lr=0.02, max_grad_norm=0.7)
+                torch.cuda.default_stream().wait_stream(torch.cuda.current_stream())
+        else:
+            eager = adam_step_(q, fresh, n, w, 5, lr=0.02, max_grad_norm=0.7)
+        assert torch.equal(eager, norm) and all(torch.equal(a, b) for x, y in ((p, q), (m, n), (v, w)) for a, b in zip(x, y))
+        want = norm64(fresh)
+        assert abs(float(clip_grad_norm_(params_of(fresh), 0.7)) - want) <= SLACK * U * want
+        torch.cuda.synchronize()

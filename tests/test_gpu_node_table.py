@@ -155,3 +155,15 @@ def test_autoencoder_clips(dev, tmp_path, monkeypatch):
     for a, b in zip(net.parameters(), ref.parameters()):
         # two Adam steps move every weight by about lr; a gradient entry near zero may take another sign of its last bits
         assert float((a - b).detach().abs().max()) <= 2 * 2 * 1e-2 * 1e-3 + 1e-5 * float(b.detach().abs().max())
+
+
+def test_graphed_step_beside_a_living_eager_graph_is_refused(dev):
+    tr = sharded(dev, max_grad_norm=0.05, hip_graph=True)
+    head = np.arange(ARCH["output_dim"])
+    kept = tr.net.forward_pair(tr.features[1], tr.features[0])    # on the default stream, and alive
+    with pytest.raises(RuntimeError, match="is alive"):
+        tr.step(0, 1, head)
+    del kept
+    tr.net.orthonorm_weights = None
+    losses = [float(tr.step(0, 1, head)) for _ in range(4)]
+    assert np.isfinite(losses).all()
