@@ -406,3 +406,15 @@ def test_gradient_of_rows_that_many_workgroups_share(pattern, n, rows, dim, dtyp
     got = embedding_grad(ids, g, rows, scale=-1.5)
     check_grad(got, ids, g, rows, -1.5)
     assert torch.equal(got, embedding_grad(ids, g, rows, scale=-1.5))
+
+
+@pytest.mark.parametrize("dim,dtype", [(8192, torch.float32), (8193, torch.float32), (16384, torch.float16), (16385, torch.bfloat16), (1 << 20, torch.float16)])
+def test_gradient_of_very_wide_rows(dim, dtype):
+    from sparc_amd.embedding import embedding_grad, embedding_lookup
+    for pattern, n, rows in (("zipf", 37, 9), ("one", 90, 4), ("uniform", 1, 3)):
+        if n * dim > 1 << 23:
+            n = 5
+        ids = make_ids(pattern, n, rows, dim)
+        g = torch.randn(n, dim, device="cuda", generator=gen(dim)).to(dtype)
+        check_grad(embedding_grad(ids, g, rows, scale=3.0), ids, g, rows, 3.0)
+        assert torch.equal(embedding_lookup(ids, g[:min(n, rows)]).isnan().any(1), ids >= min(n, rows))
