@@ -492,7 +492,7 @@ int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t* tensors, 
  *   sparc_embedding_grad  out[v] = round(scale * sum over ids[i] = v of g[i]) for ALL rows v (dense [rows][dim]; rows
  *                         without a token, and row padding_idx when it is a row, are 0); tokens outside the table are left
  *                         out.  Sums in float32, of long rows joined in float64, in an order fixed by the tokens alone.
- * The gradient needs the query's workspace, 256-byte aligned; where the query gives 0 (few tokens; sizes that the call
+ * The gradient needs the query's workspace, 256-byte aligned; where the query gives 0 (none or few tokens; sizes that the call
  * refuses) none, and ws may be NULL. */
 #define SPARC_EMBEDDING_MAX 2147483647LL      /* tokens, and rows */
 #define SPARC_EMBEDDING_MAX_DIM 1048576LL

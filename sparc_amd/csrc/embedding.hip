@@ -902,8 +902,8 @@ int lanes_for(const int64_t units, int* slices, const int most_log2 = 6) {
 
 Plan plan_of(const int64_t n, const int64_t rows, const int dim, const int ve) {
     Plan p;
-    p.tile = CHUNK * ceil_div(n > 0 ? n : 1, static_cast<int64_t>(CHUNK) * MOST_TILES);
-    p.tiles = static_cast<int>(ceil_div(n > 0 ? n : 1, p.tile));
+    p.tile = CHUNK * ceil_div(n, static_cast<int64_t>(CHUNK) * MOST_TILES);
+    p.tiles = static_cast<int>(ceil_div(n, p.tile));
     int bits = 2;
     while ((static_cast<int64_t>(1) << bits) < rows) ++bits;
     // wide digits save passes, but every tile reads the counts of all digits of all tiles
@@ -1003,7 +1003,7 @@ extern "C" size_t sparc_embedding_grad_workspace_bytes(int64_t n, int64_t rows, 
     if (n < 0 || rows < 0 || dim < 0 || n > SPARC_EMBEDDING_MAX || rows > SPARC_EMBEDDING_MAX || dim > SPARC_EMBEDDING_MAX_DIM ||
         dtype < SPARC_F32 || dtype > SPARC_F16)
         return 0;
-    if (few_enough(n, dim, dtype)) return 0;
+    if (n == 0 || few_enough(n, dim, dtype)) return 0;
     const int ve = elements_of_16_bytes(dtype);
     const Plan p = plan_of(n, rows, static_cast<int>(dim), dim >= ve ? ve : 1);
     bool ok;
@@ -1055,6 +1055,14 @@ int launch_grad(const GradArgs& a, const Plan& p, sparc_stream_t stream) {
     return SPARC_OK;
 }
 
+int launch_zeros(void* out, const int64_t bytes, sparc_stream_t stream) {
+    const int64_t chunks = ceil_div(bytes / 2, ZERO_CHUNK);
+    hipLaunchKernelGGL(zeros_kernel, dim3(static_cast<unsigned>(chunks < ZERO_GROUPS ? chunks : ZERO_GROUPS)), dim3(SORT_BLOCK), 0, stream,
+                       (Zeros{static_cast<uint16_t*>(out), bytes / 2}));
+    SPARC_CHECK_LAUNCH();
+    return SPARC_OK;
+}
+
 template <int DT, int VE>
 int launch_few(const GradArgs& a, sparc_stream_t stream) {
     int slices, blocks_log2 = FEW_BLOCKS_LOG2;
@@ -1075,12 +1083,10 @@ int launch_few(const GradArgs& a, sparc_stream_t stream) {
     const int64_t row_bytes = a.dim * static_cast<int64_t>(sizeof(typename Elem<DT>::type)), bytes = a.rows * row_bytes;
     const bool apart = bytes > ((row_bytes << d.group) % 128 ? SPARC_KEEP_BYTES / 3 : SPARC_KEEP_BYTES);
     if (apart) {
-        const int64_t chunks = ceil_div(bytes / 2, ZERO_CHUNK);
-        hipLaunchKernelGGL(zeros_kernel, dim3(static_cast<unsigned>(chunks < ZERO_GROUPS ? chunks : ZERO_GROUPS)), dim3(SORT_BLOCK), 0, stream,
-                           (Zeros{static_cast<uint16_t*>(a.out), bytes / 2}));
-        SPARC_CHECK_LAUNCH();
+        const int rc = launch_zeros(a.out, bytes, stream);
+        if (rc != SPARC_OK) return rc;
     }
-    const size_t keys = a.n > 0 ? (static_cast<size_t>(a.n) + 3) & ~static_cast<size_t>(3) : 4;
+    const size_t keys = (static_cast<size_t>(a.n) + 3) & ~static_cast<size_t>(3);
     hipLaunchKernelGGL((few_tokens<DT, VE>), dim3(grid, static_cast<unsigned>(slices)), dim3(FEW_THREADS), keys * sizeof(uint32_t), stream, a, d,
                        lanes_log2, !apart);
     SPARC_CHECK_LAUNCH();
@@ -1096,6 +1102,7 @@ extern "C" int sparc_embedding_grad(int64_t n, int64_t rows, int64_t dim, int dt
         return SPARC_ERR_ARG;
     if (n > SPARC_EMBEDDING_MAX || rows > SPARC_EMBEDDING_MAX || dim > SPARC_EMBEDDING_MAX_DIM) return SPARC_ERR_SIZE;
     if (rows == 0 || dim == 0) return SPARC_OK;
+    if (n == 0) return launch_zeros(out, rows * dim * (dtype == SPARC_F32 ? 4 : 2), stream);   // (the sort would launch empty grids)
     const int ve = elements_of_16_bytes(dtype), used_ve = dim >= ve ? ve : 1;
     GradArgs a = {};
     Plan p = {};
