@@ -29,7 +29,7 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-_type_of, _needs_grad = operator.attrgetter("dtype"), operator.attrgetter("requires_grad")
+_type_of = operator.attrgetter("dtype")
 _device_of, _address_of, _size_of = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
 _is_contiguous = torch.Tensor.is_contiguous
 
@@ -115,8 +115,7 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     norm = torch.empty((), dtype=torch.float32, device=device)
     launch("sparc_clip_grad_norm", lib.sparc_clip_grad_norm, device, n, _address(records), max_norm, parts.data_ptr(), nbytes,
            norm.data_ptr())
-    if True in map(_needs_grad, grads):   # of a backward with create_graph: who goes on through them is told
-        increment_version([g for g in grads if g.requires_grad])
+    increment_version(grads)   # whatever graph has saved one of them refuses to go back through it
     return norm
 
 

@@ -8,3 +8,19 @@ def test_no_tokens_need_no_scratch(dim, dtype):
     """The gradient of no tokens is the zeros of the table, whatever the rows' width: nothing to sort."""
     from sparc_amd._lib import lib
     assert lib.sparc_embedding_grad_workspace_bytes(0, 9, dim, dtype) == 0
+
+
+def test_every_clipped_gradient_counts_as_written(monkeypatch):
+    """clip_grad_norm_ raises the version of all gradients that it scales (the launch itself is left out here)."""
+    from sparc_amd import optim
+    monkeypatch.setattr(optim, "require_gpu", lambda device: None)
+    monkeypatch.setattr(optim, "launch", lambda *a: None)
+    monkeypatch.setattr(optim, "_dense_on", lambda *a: True)
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(2))
+    p.grad, q.grad = torch.ones(3), torch.ones(2)
+    x = torch.ones(3, requires_grad=True)
+    loss = (p.grad * x).sum()
+    optim.clip_grad_norm_([p, q], 1.0)
+    assert p.grad._version > 0 and q.grad._version > 0
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()

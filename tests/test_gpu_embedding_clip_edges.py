@@ -31,3 +31,19 @@ def test_gradient_of_no_tokens(rows, dim, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert not bool((got != 0).any())
+
+
+def test_every_clipped_gradient_counts_as_written():
+    """Also one that requires no gradient itself and that another graph has saved."""
+    from sparc_amd.optim import clip_grad_norm_
+    p, x = (torch.randn(50, device="cuda", generator=gen(i)).requires_grad_() for i in (3, 4))
+    p.grad = torch.randn(50, device="cuda", generator=gen(5))
+    loss = (p.grad * x).sum()
+    before = p.grad._version
+    clip_grad_norm_([p], 0.1)
+    assert p.grad._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    loss = (p.grad * x).sum()                                             # saved after the clipping: fine
+    loss.backward()
+    assert torch.equal(x.grad, p.grad)
