@@ -152,12 +152,12 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
         require_gpu(device)
     records, once = _adam_records(params, grads, exp_avgs, exp_avg_sqs, device)
     rates = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step))
+    norm = None
     if max_grad_norm is None:
         _adam_launches(records, len(params), rates, device)
-        increment_version(params)
-        return None
-    norm = _clipped_step(records, once, len(params), rates, _limit(max_grad_norm), device)
-    increment_version(params)
+    else:
+        norm = _clipped_step(records, once, len(params), rates, _limit(max_grad_norm), device)
+    increment_version([*params, *exp_avgs, *exp_avg_sqs])
     return norm
 
 
@@ -254,4 +254,5 @@ class Adam(torch.optim.Optimizer):
             else:
                 launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, dev, len(live), _address(records), *rates,
                        parts.data_ptr(), count, max_norm, self.grad_norm.data_ptr())
+            increment_version([*live, *ms, *vs])
         return loss

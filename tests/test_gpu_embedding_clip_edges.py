@@ -47,3 +47,39 @@ def test_every_clipped_gradient_counts_as_written():
     loss = (p.grad * x).sum()                                             # saved after the clipping: fine
     loss.backward()
     assert torch.equal(x.grad, p.grad)
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+@pytest.mark.parametrize("limit", [None, 1.0])
+def test_adam_class_counts_as_written(limit, groups):
+    """Parameters and moments: a graph that saved them refuses to go back, as with torch's Adam."""
+    from sparc_amd.optim import Adam
+    ps = [torch.nn.Parameter(torch.randn(50, device="cuda", generator=gen(3 + i))) for i in range(2)]
+    opt = Adam([{"params": ps}] if groups == 1 else [{"params": [p]} for p in ps], max_grad_norm=limit)
+    x = torch.ones(50, device="cuda", requires_grad=True)
+    for turn in range(2):
+        for p in ps:
+            p.grad = torch.ones(50, device="cuda")
+            saved = [(p * p).sum()] + [(x * m).sum() for m in opt.state[p].values()]
+            opt.step()
+            for loss in saved:
+                with pytest.raises(RuntimeError, match="modified by an inplace"):
+                    loss.backward()
+    loss = (ps[0] * ps[0]).sum()                                          # made after the step: fine
+    ps[0].grad = None
+    loss.backward()
+    assert torch.equal(ps[0].grad, 2 * ps[0].detach())
+
+
+def test_adam_function_counts_moments_as_written():
+    from sparc_amd.optim import adam_step_
+    p, g, m, v = (torch.rand(50, device="cuda", generator=gen(i)) for i in range(4))
+    x = torch.ones(50, device="cuda", requires_grad=True)
+    for limit in (None, 1.0):
+        saved = [(x * t).sum() for t in (p, m, v)]
+        read = (x * g).sum()
+        adam_step_([p], [g], [m], [v], 1, max_grad_norm=limit)
+        for loss in saved:
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                loss.backward()
+        read.backward()                                                   # the gradient is only read
