@@ -220,7 +220,6 @@ class Adam(torch.optim.Optimizer):
             live = [p for p in group["params"] if p.grad is not None]
             if not live:
                 continue
-            group["step"] = group.get("step", 0) + 1
             grads, ms, vs = [], [], []
             for p in live:
                 if p.dtype != torch.float32 or p.grad.dtype != torch.float32 or not p.is_cuda or p.grad.is_sparse:
@@ -234,19 +233,19 @@ class Adam(torch.optim.Optimizer):
                 grads.append(p.grad if p.grad.is_contiguous() else p.grad.contiguous())
                 ms.append(st["exp_avg"])
                 vs.append(st["exp_avg_sq"])
-            work.append((group, live, grads, ms, vs))
-        if not work:
-            return loss
-        if max_norm is not None and len(work) > 1:   # the norm over all groups
-            device = work[0][1][0].device
-            require_gpu(device)
-            parts, count = _norm_of(*_grad_records([g for w in work for g in w[2]], device), device)
-            self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
-        for group, live, grads, ms, vs in work:
             dev = live[0].device
             records, once = _adam_records(live, grads, ms, vs, dev)
             rates = (float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
-                     float(group["weight_decay"]), int(group["step"]))
+                     float(group["weight_decay"]), int(group.get("step", 0)) + 1)
+            work.append((group, live, grads, ms, vs, dev, records, once, rates))
+        if not work:
+            return loss
+        if max_norm is not None and len(work) > 1:   # the norm over all groups
+            device = work[0][5]
+            require_gpu(device)
+            parts, count = _norm_of(*_grad_records([g for w in work for g in w[2]], device), device)
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
+        for group, live, _, ms, vs, dev, records, once, rates in work:   # all that can be refused but a rate has been
             if max_norm is None:
                 _adam_launches(records, len(live), rates, dev)
             elif len(work) == 1:
@@ -254,5 +253,6 @@ class Adam(torch.optim.Optimizer):
             else:
                 launch("sparc_adam_step_clipped", lib.sparc_adam_step_clipped, dev, len(live), _address(records), *rates,
                        parts.data_ptr(), count, max_norm, self.grad_norm.data_ptr())
+            group["step"] = rates[-1]
             increment_version([*live, *ms, *vs])
         return loss

@@ -24,3 +24,14 @@ def test_every_clipped_gradient_counts_as_written(monkeypatch):
     assert p.grad._version > 0 and q.grad._version > 0
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         loss.backward()
+
+
+def test_a_refused_adam_step_counts_for_no_group():
+    from sparc_amd.optim import Adam
+    ps = [torch.nn.Parameter(torch.zeros(3)) for _ in range(2)]
+    opt = Adam([{"params": ps[:1]}, {"params": ps[1:]}])
+    for p in ps:
+        p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError):
+        opt.step()                                                        # (host tensors)
+    assert [group.get("step", 0) for group in opt.param_groups] == [0, 0]

@@ -83,3 +83,24 @@ def test_adam_function_counts_moments_as_written():
             with pytest.raises(RuntimeError, match="modified by an inplace"):
                 loss.backward()
         read.backward()                                                   # the gradient is only read
+
+
+@pytest.mark.parametrize("limit", [None, 1.0])
+def test_a_refused_adam_step_changes_nothing(limit):
+    """The second group is refused: neither group moves or counts a step, and the next step is the one it would have been."""
+    from sparc_amd.optim import Adam
+    ps = [torch.nn.Parameter(torch.randn(6, 4, device="cuda", generator=gen(i))) for i in range(2)]
+    opt = Adam([{"params": ps[:1]}, {"params": ps[1:]}], max_grad_norm=limit)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    kept = [t.clone() for p in ps for t in (p.detach(), *opt.state[p].values())]
+    good = opt.state[ps[1]]["exp_avg"]
+    opt.state[ps[1]]["exp_avg"] = good.t().contiguous().t()               # not laid out as the parameter
+    with pytest.raises(ValueError):
+        opt.step()
+    assert [group["step"] for group in opt.param_groups] == [1, 1]
+    assert all(torch.equal(a, b) for a, b in zip(kept, [t for p in ps for t in (p.detach(), *opt.state[p].values())]))
+    opt.state[ps[1]]["exp_avg"] = good
+    opt.step()
+    assert [group["step"] for group in opt.param_groups] == [2, 2] and all(bool((p.detach() != k).all()) for p, k in zip(ps, kept[::3]))
