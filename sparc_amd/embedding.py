@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import lib
@@ -15,6 +16,12 @@ from .graph import _raw_stream, launch, require_gpu
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SPARC_F32, SPARC_BF16, SPARC_F16
 _ID_DTYPES = {torch.int32: 0, torch.int64: 1}
+
+
+def refuse_forward_mode(what: str, *tensors) -> None:
+    """Raises inside a dual level where a tensor carries a tangent: the kernels know nothing of it and it would be lost."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _tokens(ids: torch.Tensor, device) -> torch.Tensor:
@@ -63,7 +70,11 @@ def _lookup(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tenso
 def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: float = 1.0, padding_idx=None) -> torch.Tensor:
     """[rows, dim], in grad's type: row v = scale times the sum of grad[i] over the places i with ids[i] = v (grad: the
     shape of ids and one more dimension, dim).  float32 sums, rounded once.  Rows without a place, and row padding_idx,
-    are zero; places whose token is no row are left out."""
+    are zero; places whose token is no row are left out.  Not differentiable: a grad that requires a gradient (where gradients
+    are recorded) or carries a forward-mode tangent raises."""
+    if grad.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("embedding_grad is not differentiable: detach grad, or call it under torch.no_grad()")
+    refuse_forward_mode("embedding_grad", grad)
     dev = grad.device
     if not grad.is_cuda:
         require_gpu(dev)
@@ -128,9 +139,11 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     """scale * table[ids], of shape ids.shape + (dim,): ids int32 or int64 of any shape, table [rows, dim] float32, bfloat16
     or float16 with contiguous rows (any row stride).  The product is rounded once.  A token that is no row of the table
     gives a row of NaN (nothing is read, nothing synchronises) and no gradient.  padding_idx: this row is read as any
-    other and gets no gradient.  Differentiable once, with respect to the table."""
+    other and gets no gradient.  Differentiable once, with respect to the table, in reverse mode; a table with a forward-mode
+    tangent raises."""
     if padding_idx is not None:
         _padding(padding_idx, table.shape[0])
+    refuse_forward_mode("embedding_lookup", table)
     if table.requires_grad and torch.is_grad_enabled():
         out = EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
         if table.is_leaf:

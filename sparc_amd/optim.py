@@ -13,7 +13,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from ._lib import AdamTensor, lib
-from .embedding import DTYPES
+from .embedding import DTYPES, refuse_forward_mode
 from .graph import launch, require_gpu
 
 MAX_TENSORS = 32
@@ -106,6 +106,7 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros(())
+    refuse_forward_mode("clip_grad_norm_", *grads)
     device = grads[0].device
     if not grads[0].is_cuda:
         require_gpu(device)
@@ -123,6 +124,7 @@ def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
     """(records of the update as the C calls take them; None, or, where parameters share gradients, these once)."""
     n = len(params)
     every = [*params, *grads, *exp_avgs, *exp_avg_sqs]
+    refuse_forward_mode("an Adam step", *every)
     sizes = list(map(_size_of, every))
     if set(map(_type_of, every)) != {torch.float32} or not _dense_on(every, device) or sizes != sizes[:n] * 4:
         raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")

@@ -35,3 +35,30 @@ def test_a_refused_adam_step_counts_for_no_group():
     with pytest.raises(RuntimeError):
         opt.step()                                                        # (host tensors)
     assert [group.get("step", 0) for group in opt.param_groups] == [0, 0]
+
+
+def test_forward_mode_is_refused():
+    """A tangent that the kernels would lose in silence: refused before the device is looked at, also by a frozen table."""
+    from torch.autograd import forward_ad
+    from sparc_amd.embedding import embedding_grad, embedding_lookup
+    from sparc_amd.optim import adam_step_, clip_grad_norm_
+    ids, t = torch.zeros(2, dtype=torch.int64), torch.randn(5, 3)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(t, torch.ones_like(t))
+        p = torch.nn.Parameter(torch.zeros(5, 3))
+        p.grad = d
+        for call in (lambda: embedding_lookup(ids, d), lambda: embedding_grad(ids, d[:2], 5), lambda: clip_grad_norm_([p], 1.0)):
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        q = forward_ad.make_dual(t.clone().requires_grad_(), torch.ones_like(t))
+        with pytest.raises(NotImplementedError):
+            embedding_lookup(ids, q)
+
+
+def test_gradient_of_a_gradient_is_refused():
+    from sparc_amd.embedding import embedding_grad
+    ids, g = torch.zeros(2, dtype=torch.int64), torch.randn(2, 3, requires_grad=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        embedding_grad(ids, g, 5)
