@@ -2,6 +2,7 @@
 rule, frozen tables, forward mode, version counters, memory that tensors share in part, captures beside living graphs.
 
 Tolerances are those of test_gpu_embedding.py and test_gpu_clip.py."""
+import numpy as np
 import pytest
 import torch
 
@@ -134,3 +135,21 @@ def test_tangents_are_refused():
     with torch.no_grad():
         assert torch.equal(embedding_grad(ids, g, 5), leaf.grad)
     assert torch.equal(embedding_grad(ids, g.detach(), 5), leaf.grad)
+
+
+def test_graphed_steps_with_a_frozen_table():
+    """Rows that are not trained: graphed steps go as the eager ones with the same optimiser, and the table stays."""
+    from test_gpu_node_table import ARCH, sharded
+    dev = torch.device("cuda:0")
+    heads = [np.random.RandomState(i).permutation(260)[:ARCH["output_dim"]] for i in range(6)]
+    got = []
+    for graphed in (True, False):
+        tr = sharded(dev, max_grad_norm=0.05, hip_graph=graphed)
+        if not graphed:
+            tr.optimizer = torch.optim.Adam(tr.net.parameters(), lr=torch.tensor(1e-2, device=dev), fused=True, capturable=True)
+        tr.net.node_table.weight.requires_grad_(False)
+        table = tr.net.node_table.weight.clone()
+        losses = [tr.step(s % 2, (s // 2) % 2, heads[s]) for s in range(6)]
+        assert torch.equal(table, tr.net.node_table.weight) and tr.net.node_table.weight.grad is None
+        got.append(torch.stack(losses + [p.detach().double().sum() for p in tr.net.parameters()]))
+    assert torch.equal(*got) and bool(torch.isfinite(got[0]).all())
