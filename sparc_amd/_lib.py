@@ -15,6 +15,9 @@ ERRORS = {-1: "SPARC_ERR_ARG (bad argument)", -2: "SPARC_ERR_WS (workspace too s
           -4: "SPARC_ERR_SIZE (problem larger than the fixed-size entry point supports)"}
 
 
+AUTOGRAD_LIB_PATH = os.path.join(_HERE, "lib", "libsparc_autograd.so")
+
+
 class SparcHipError(RuntimeError):
     pass
 
@@ -112,6 +115,15 @@ for _name, (_res, _args) in _SIGS.items():
     _fn.argtypes = _args
 
 EXPORTS = tuple(_SIGS)
+
+
+def load_autograd():
+    """torch.ops.sparc_amd.leaf_stream (csrc/leaf_stream.cpp)."""
+    import torch
+    if not os.path.exists(AUTOGRAD_LIB_PATH):
+        raise SparcHipError(f"{AUTOGRAD_LIB_PATH} is missing: build the extensions first (python -m sparc_amd.build)")
+    torch.ops.load_library(AUTOGRAD_LIB_PATH)
+    return torch.ops.sparc_amd.leaf_stream
 
 
 _initialised = set()

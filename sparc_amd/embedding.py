@@ -11,8 +11,8 @@ import torch.nn as nn
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
-from ._lib import lib
-from .graph import _raw_stream, launch, require_gpu
+from ._lib import lib, load_autograd
+from .graph import launch, require_gpu
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SPARC_F32, SPARC_BF16, SPARC_F16
 _ID_DTYPES = {torch.int32: 0, torch.int64: 1}
@@ -102,16 +102,14 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
     return out
 
 
-# A leaf's node in the autograd graph lives as long as any graph that it is in and keeps the stream that was current when it
-# was made: written down there by the first lookup.
-_BORN_ON = "sparc_amd.stream"
+_leaf_stream = load_autograd()
 
 
-def refuse_capture_beside_eager_graph(node) -> None:
-    """Raises if a leaf's node was made on the default stream: the backward that is to be captured would let that stream,
-    which cannot be captured, wait for the capture, and the process would end."""
-    if node.metadata.get(_BORN_ON) == 0:
-        raise RuntimeError("embedding_lookup: a backward is to be captured while the graph of an earlier lookup in the same table, "
+def refuse_capture_beside_eager_graph(leaf: torch.Tensor) -> None:
+    """Raises if a node of this leaf lives that was made on the default stream (by whatever operation): the backward that is
+    to be captured would let that stream, which cannot be captured, wait for the capture, and the process would end."""
+    if leaf.requires_grad and _leaf_stream(leaf) == 0:
+        raise RuntimeError(f"a backward is to be captured while an earlier graph of the same parameter, of shape {tuple(leaf.shape)}, "
                            "made on the default stream, is alive. Drop what holds it (its outputs, its loss) before capturing")
 
 
@@ -129,9 +127,10 @@ class EmbeddingLookup(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
-        leaf = ctx.next_functions[1][0]
-        if _BORN_ON in leaf.metadata and torch.cuda.is_current_stream_capturing():
-            refuse_capture_beside_eager_graph(leaf)
+        if torch.cuda.is_current_stream_capturing():
+            leaf = getattr(ctx.next_functions[1][0], "variable", None)   # (None: the table is computed)
+            if leaf is not None:
+                refuse_capture_beside_eager_graph(leaf)
         return None, embedding_grad(ids, g, ctx.rows, ctx.scale, ctx.padding_idx), None, None
 
 
@@ -145,10 +144,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         _padding(padding_idx, table.shape[0])
     refuse_forward_mode("embedding_lookup", table)
     if table.requires_grad and torch.is_grad_enabled():
-        out = EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
-        if table.is_leaf:
-            out.grad_fn.next_functions[1][0].metadata.setdefault(_BORN_ON, _raw_stream(table.device.index))
-        return out
+        return EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
     return _lookup(ids, table, float(scale))
 
 

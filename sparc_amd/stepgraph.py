@@ -85,9 +85,8 @@ class GraphedSteps:
             self.net.orthonorm_weights = self.orth
             return loss.clone()
         if hit is None:
-            table = getattr(self.net, "node_table", None)
-            if table is not None and table.weight.requires_grad:   # (a frozen table has no node)
-                refuse_capture_beside_eager_graph(torch.autograd.graph.get_gradient_edge(table.weight).node)
+            for p in self.net.parameters():
+                refuse_capture_beside_eager_graph(p)
             # the pair's first step runs eagerly on a side stream (it sizes the workspace and configures the
             # kernels); the capture that follows records the pair's NEXT step without executing it
             side = torch.cuda.Stream(device=self.device)

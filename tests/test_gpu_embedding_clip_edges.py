@@ -153,3 +153,51 @@ def test_graphed_steps_with_a_frozen_table():
         assert torch.equal(table, tr.net.node_table.weight) and tr.net.node_table.weight.grad is None
         got.append(torch.stack(losses + [p.detach().double().sum() for p in tr.net.parameters()]))
     assert torch.equal(*got) and bool(torch.isfinite(got[0]).all())
+
+
+def test_capture_asks_for_the_stream_that_made_the_leafs_node():
+    """Not for the stream of the first lookup: the node may be another operation's."""
+    from sparc_amd.embedding import _leaf_stream, embedding_grad, embedding_lookup, refuse_capture_beside_eager_graph
+    table = torch.randn(300, 24, device="cuda", generator=gen(70), requires_grad=True)
+    ids, w = make_ids("zipf", 1000, 300, 71), torch.randn(1000, 24, device="cuda", generator=gen(72))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    assert _leaf_stream(table) == -1 and _leaf_stream(table.detach()) == -1 and _leaf_stream(table * 1) == -1
+    other = (table * 2).sum()                                             # on the default stream, before any lookup
+    with torch.cuda.stream(side):
+        eager = embedding_lookup(ids, table)
+    assert _leaf_stream(table) == 0
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="is alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            embedding_lookup(ids, table).backward(w)
+    del eager, other
+    torch.cuda.synchronize()
+    assert _leaf_stream(table) == -1
+    with torch.cuda.stream(side):
+        other = (table * 2).sum()                                         # on a stream that can join a capture
+    eager = embedding_lookup(ids, table)                                  # on the default stream
+    assert _leaf_stream(table) > 0
+    refuse_capture_beside_eager_graph(table)
+    refuse_capture_beside_eager_graph(table.detach())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        embedding_lookup(ids, table).backward(w)
+    for turn in range(3):
+        w.copy_(torch.randn(w.shape, device="cuda", generator=gen(73 + turn)))
+        graph.replay()
+        assert torch.equal(table.grad, embedding_grad(ids, w, 300))
+        torch.cuda.synchronize()
+
+
+def test_graphed_steps_ask_for_every_parameter():
+    from test_gpu_node_table import ARCH, sharded
+    tr = sharded(torch.device("cuda:0"), hip_graph=True)
+    head = np.arange(ARCH["output_dim"])
+    for p in (tr.net.node_table.weight, tr.net.mlp_parameters()[0], tr.net.mlp_parameters()[-1]):
+        kept = (p * 2).sum()                                              # on the default stream, and alive
+        with pytest.raises(RuntimeError, match="is alive"):
+            tr.step(0, 1, head)
+        del kept
+    assert np.isfinite([float(tr.step(0, 1, head)) for _ in range(3)]).all()
