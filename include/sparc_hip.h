@@ -41,6 +41,7 @@ typedef struct ihipStream_t* sparc_stream_t; /* == hipStream_t */
 #define SPARC_ERR_WS (-2)      /* workspace too small or misaligned */
 #define SPARC_ERR_LAUNCH (-3)  /* the HIP runtime refused a launch */
 #define SPARC_ERR_SIZE (-4)    /* the problem is larger than a fixed-size entry point supports */
+#define SPARC_ERR_OVERLAP (-5) /* tensors that are written share memory with others */
 
 #define SPARC_MAX_K 64
 /* per-row constants used by the per-step kernels, float[m][8] */
@@ -437,7 +438,9 @@ int sparc_label_scores(int64_t n, const int64_t* rowptr, const int64_t* nbr, con
  * every backward (src/SpectralTrainer.py:188, :238; src/AETrainer.py likewise), for all parameter tensors of a
  * model in one launch.  tensors: a HOST array of n_tensors <= SPARC_ADAM_MAX_TENSORS records of device pointers
  * (parameter, its gradient, first and second moment; float32, n elements each); step: the number of this update,
- * counted from 1 (bias corrections 1 - beta^step).  The moments are updated in place. */
+ * counted from 1 (bias corrections 1 - beta^step).  The moments are updated in place.  Records may share gradients; a
+ * parameter or moment that shares memory with any other tensor is refused (SPARC_ERR_OVERLAP).
+ * sparc_adam_check (host only) answers for the tensors of a list longer than one launch takes, before its first. */
 #define SPARC_ADAM_MAX_TENSORS 32
 typedef struct {
     float* p;
@@ -448,6 +451,7 @@ typedef struct {
 } sparc_adam_tensor_t;
 int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
                     double eps, double weight_decay, int64_t step, sparc_stream_t stream);
+int sparc_adam_check(int64_t n_tensors, const sparc_adam_tensor_t* tensors);
 
 /* ---- gradient norm and clipping -------------------------------------------------------
  * The reference steps Adam on the gradients as they are (src/SpectralTrainer.py:237-238) and has no clipping; here the
@@ -459,7 +463,8 @@ int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr
  *   sparc_clip_grad_norm     the same, then g <- c g, rounded to nearest, in place, and *norm_out = N (one device float)
  *   sparc_adam_step_clipped  sparc_adam_step on c g (the gradients themselves stay), any number of tensors, and *norm_out
  *   sparc_clip_adam_step     the same with c of these tensors' own gradients, each counted (parts as in sparc_grad_norm)
- * Whoever scales adds the partial sums up itself, in a fixed order. */
+ * Whoever scales adds the partial sums up itself, in a fixed order.  Tensors that are written and share memory with another,
+ * wholly or in part, are refused before any launch (SPARC_ERR_OVERLAP); what is only read may be shared. */
 #define SPARC_F32 0
 #define SPARC_BF16 1
 #define SPARC_F16 2

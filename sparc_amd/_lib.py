@@ -12,7 +12,8 @@ LIB_PATH = os.environ.get("SPARC_HIP_LIB") or os.path.join(_HERE, "lib", "libspa
 
 ERRORS = {-1: "SPARC_ERR_ARG (bad argument)", -2: "SPARC_ERR_WS (workspace too small or misaligned)",
           -3: "SPARC_ERR_LAUNCH (HIP launch failed)",
-          -4: "SPARC_ERR_SIZE (problem larger than the fixed-size entry point supports)"}
+          -4: "SPARC_ERR_SIZE (problem larger than the fixed-size entry point supports)",
+          -5: "SPARC_ERR_OVERLAP (tensors that are written share memory with others)"}
 
 
 AUTOGRAD_LIB_PATH = os.path.join(_HERE, "lib", "libsparc_autograd.so")
@@ -20,6 +21,10 @@ AUTOGRAD_LIB_PATH = os.path.join(_HERE, "lib", "libsparc_autograd.so")
 
 class SparcHipError(RuntimeError):
     pass
+
+
+class SparcOverlapError(SparcHipError, ValueError):
+    """Tensors that are written share memory with others."""
 
 
 class Tiling(ctypes.Structure):
@@ -94,6 +99,7 @@ _SIGS = {
     "sparc_dgrad_wide_first_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "sparc_dgrad_wide_first": (c_int, [c_int64, c_int, c_int, c_int, P, c_int64, P, P, c_int64, P, P, P, P, c_size_t, P]),
     "sparc_adam_step": (c_int, [c_int, P, c_double, c_double, c_double, c_double, c_double, c_int64, P]),
+    "sparc_adam_check": (c_int, [c_int64, P]),
     "sparc_grad_norm_workspace_bytes": (c_size_t, [c_int64]),
     "sparc_grad_norm": (c_int, [c_int64, P, P, c_size_t, P, P]),
     "sparc_clip_grad_norm": (c_int, [c_int64, P, c_double, P, c_size_t, P, P]),
@@ -141,4 +147,4 @@ def init_device(index: int) -> None:
 
 def check(rc, what):
     if rc != 0:
-        raise SparcHipError(f"{what} failed: {ERRORS.get(rc, rc)}")
+        raise (SparcOverlapError if rc == -5 else SparcHipError)(f"{what} failed: {ERRORS.get(rc, rc)}")

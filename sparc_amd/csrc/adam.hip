@@ -9,6 +9,7 @@
 //     g' = g + weight_decay p;   m = m + (1 - beta1) (g' - m);   v = beta2 v + (1 - beta2) g' g'
 //     p = p - (lr / (1 - beta1^t)) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 #include "common.h"
+#include "ranges.h"
 
 namespace {
 
@@ -57,7 +58,16 @@ __global__ __launch_bounds__(256) void adam_step_kernel(const AdamArgs a) {
     }
 }
 
+bool record_ok(const sparc_adam_tensor_t& t) { return t.n >= 0 && (t.n == 0 || (t.p && t.g && t.m && t.v)); }
+
 }  // namespace
+
+extern "C" int sparc_adam_check(int64_t n_tensors, const sparc_adam_tensor_t* tensors) {
+    if (n_tensors < 0 || !tensors) return SPARC_ERR_ARG;
+    for (int64_t i = 0; i < n_tensors; ++i)
+        if (!record_ok(tensors[i])) return SPARC_ERR_ARG;
+    return check_adam_ranges(n_tensors, tensors);
+}
 
 extern "C" int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors, double lr, double beta1, double beta2,
                                double eps, double weight_decay, int64_t step, sparc_stream_t stream) {
@@ -68,7 +78,7 @@ extern "C" int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors
     int64_t blocks = 0;
     for (int i = 0; i < n_tensors; ++i) {
         const sparc_adam_tensor_t& t = tensors[i];
-        if (t.n < 0 || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v))) return SPARC_ERR_ARG;
+        if (!record_ok(t)) return SPARC_ERR_ARG;
         a.t[i] = t;
         a.first_block[i] = static_cast<int32_t>(blocks);
         blocks += (t.n + ADAM_BLOCK_ELEMS - 1) / ADAM_BLOCK_ELEMS;
@@ -77,6 +87,8 @@ extern "C" int sparc_adam_step(int n_tensors, const sparc_adam_tensor_t* tensors
     a.first_block[n_tensors] = static_cast<int32_t>(blocks);
     a.n_tensors = n_tensors;
     if (blocks == 0) return SPARC_OK;
+    const int apart = check_adam_ranges(n_tensors, tensors);
+    if (apart != SPARC_OK) return apart;
     const double bc1 = 1.0 - pow(beta1, static_cast<double>(step)), bc2 = 1.0 - pow(beta2, static_cast<double>(step));
     a.step_size = static_cast<float>(lr / bc1);
     a.bc2_rsqrt = static_cast<float>(1.0 / sqrt(bc2));

@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "elem.h"
+#include "ranges.h"
 
 namespace {
 
@@ -662,6 +663,11 @@ extern "C" int sparc_clip_grad_norm(int64_t n_tensors, const sparc_grad_tensor_t
                                     size_t parts_bytes, float* norm_out, sparc_stream_t stream) {
     if (!norm_out || !(max_norm >= 0.0) || !parts || !grads_ok(n_tensors, tensors)) return SPARC_ERR_ARG;
     if (!parts_ok(n_tensors, parts, parts_bytes)) return SPARC_ERR_WS;
+    const int apart = check_ranges(n_tensors, [tensors](const int64_t i) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(tensors[i].p);
+        return MemoryRange{from, from + bytes_of(tensors[i]), true};
+    });
+    if (apart != SPARC_OK) return apart;
     int64_t once = 0;
     for (int64_t i = 0; i < n_tensors && once <= ONCE_BLOCKS; ++i) once += (bytes_of(tensors[i]) + ONCE_BYTES - 1) / ONCE_BYTES;
     if (n_tensors <= SPARC_GRAD_MAX_TENSORS && once <= ONCE_BLOCKS) {
@@ -706,6 +712,8 @@ extern "C" int sparc_adam_step_clipped(int64_t n_tensors, const sparc_adam_tenso
                                        double max_norm, float* norm_out, sparc_stream_t stream) {
     const AdamRates rates = {lr, beta1, beta2, eps, weight_decay, step};
     if (!adam_ok(n_tensors, tensors, rates) || !parts || !norm_out || n_parts < 0 || n_parts > PARTS || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
+    const int apart = check_adam_ranges(n_tensors, tensors);
+    if (apart != SPARC_OK) return apart;
     return launch_adam(n_tensors, tensors, rates, Clip{parts, norm_out, max_norm, static_cast<int>(n_parts)}, stream);
 }
 
@@ -715,6 +723,8 @@ extern "C" int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t
     const AdamRates rates = {lr, beta1, beta2, eps, weight_decay, step};
     if (!adam_ok(n_tensors, tensors, rates) || !parts || !norm_out || !(max_norm >= 0.0)) return SPARC_ERR_ARG;
     if (!parts_ok(n_tensors, parts, parts_bytes)) return SPARC_ERR_WS;
+    const int apart = check_adam_ranges(n_tensors, tensors);
+    if (apart != SPARC_OK) return apart;
     int64_t once = 0;
     for (int64_t i = 0; i < n_tensors && once <= ONCE_BLOCKS; ++i) once += (tensors[i].n + ONCE_ELEMS - 1) / ONCE_ELEMS;
     if (n_tensors <= ADAM_MOST && once <= ONCE_BLOCKS) {

@@ -12,7 +12,7 @@ from array import array
 import torch
 from torch.autograd.graph import increment_version
 
-from ._lib import AdamTensor, lib
+from ._lib import AdamTensor, check, lib
 from .embedding import DTYPES, refuse_forward_mode
 from .graph import launch, require_gpu
 
@@ -97,8 +97,8 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the gradients of `parameters` (one tensor or several; those without a gradient are passed over, a gradient met
     twice, the same memory, counts once) in place by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them
     together, and returns the norm before (float32, on the device; nothing synchronises).  float32, bfloat16 and float16
-    gradients may be mixed, each dense in memory (any order of the dimensions, views into a bucket too) and none overlapping
-    another in part; sums in float64.  A norm that is not finite leaves what the formula gives; an infinite max_norm never
+    gradients may be mixed, each dense in memory (any order of the dimensions, views into a bucket too); gradients that overlap
+    in part raise.  Sums in float64.  A norm that is not finite leaves what the formula gives; an infinite max_norm never
     clips."""
     max_norm = _limit(max_norm)
     if torch.is_tensor(parameters):
@@ -143,7 +143,7 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step: int, lr: float = 1e-3
     """Update number `step` (from 1) of torch.optim.Adam on lists of tensors, in place: params, exp_avgs and exp_avg_sqs.
     With max_grad_norm the gradients enter as clip_grad_norm_(..., max_grad_norm) would leave them, but are only read
     (once for the norm, once by the update); returns their norm then, None otherwise.  Gradients may be shared, what is written
-    may not."""
+    may not: it raises where it has memory in common with any other tensor."""
     params = list(params)
     if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs)):
         raise ValueError("as many gradients and moments as parameters")
@@ -180,6 +180,8 @@ def _clipped_step(records, once, n, rates, max_norm, device):
 
 def _adam_launches(records, n, rates, device):
     size = ctypes.sizeof(AdamTensor)
+    if n > MAX_TENSORS:   # nothing moves where a later launch would be refused
+        check(lib.sparc_adam_check(n, _address(records)), "sparc_adam_check")
     for a in range(0, n, MAX_TENSORS):
         launch("sparc_adam_step", lib.sparc_adam_step, device, min(MAX_TENSORS, n - a), _address(records) + a * size, *rates)
 

@@ -1,4 +1,6 @@
 """Edges of the table lookup, its gradient and of gradient clipping that show without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
@@ -62,3 +64,37 @@ def test_gradient_of_a_gradient_is_refused():
     ids, g = torch.zeros(2, dtype=torch.int64), torch.randn(2, 3, requires_grad=True)
     with pytest.raises(RuntimeError, match="not differentiable"):
         embedding_grad(ids, g, 5)
+
+
+P = 1 << 20      # an address that no call below may touch: all are refused
+
+
+def test_memory_written_twice_is_refused():
+    """Before any launch, wherever in the tensors the overlap lies and whatever the order of the list."""
+    from sparc_amd._lib import SparcOverlapError, check, lib
+    records = lambda *rows: (ctypes.c_int64 * sum(map(len, rows)))(*(x for row in rows for x in row))  # noqa: E731
+    clip = lambda *rows: lib.sparc_clip_grad_norm(len(rows), records(*rows), 1.0, P, 1 << 20, P, None)  # noqa: E731
+    assert clip((P, 9, 0), (P + 4 * 5, 9, 0)) == -5                       # float32: bytes [0, 36) and [20, 56)
+    assert clip((P + 4 * 5, 9, 0), (P, 9, 0)) == -5
+    assert clip((P, 9, 0), (P, 9, 0)) == -5
+    assert clip((P, 1000, 1), (P + 10_000, 7, 0), (P + 1998, 1, 2)) == -5  # the last two bytes of 1000 bfloat16
+    assert clip((P, 100_000, 0), (P + 8, 1, 0), (P + 500_000, 3, 0)) == -5  # wholly inside
+    assert clip(*((P + 4096 * i, 1024, 0) for i in range(300)), (P + 4096 * 300 - 4, 2, 0)) == -5
+    adam = lambda *rows: lib.sparc_adam_step(len(rows), records(*rows), 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None)  # noqa: E731
+    clipped = lambda *rows: lib.sparc_adam_step_clipped(len(rows), records(*rows), 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, P, 1, 1.0, P, None)  # noqa: E731
+    both = lambda *rows: lib.sparc_clip_adam_step(len(rows), records(*rows), 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 1.0, P, 1 << 20, P, None)  # noqa: E731
+    at = lambda i: P + 4096 * i  # noqa: E731
+    every = lambda *rows: lib.sparc_adam_check(len(rows), records(*rows))  # noqa: E731
+    assert every((at(0), at(1), at(2), at(3), 1024), (at(4), at(1), at(5), at(6), 1024), (0, 0, 0, 0, 0)) == 0    # a shared gradient
+    assert every(*((at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3), 1024) for i in range(200)), (at(799), at(900), at(901), at(902), 5)) == -5
+    assert every((at(0), 0, at(2), at(3), 1)) == -1 and every((at(0), at(1), at(2), at(3), -1)) == -1
+    for step in (adam, clipped, both, every):
+        for bad in (((at(0), at(1), at(2), at(2) + 396, 100),),                       # moments that share an element
+                    ((at(0), at(1), at(2), at(3), 100), (at(0) + 4, at(5), at(6), at(7), 100)),   # parameters
+                    ((at(0), at(0) + 396, at(2), at(3), 100),),                       # a gradient's first element is a parameter's last
+                    ((at(0), at(1), at(2), at(3), 100), (at(4), at(3) + 200, at(6), at(7), 100)),  # a gradient inside another's moment
+                    ((at(0), at(1), at(2), at(3), 100), (at(4), at(1), at(6), at(1) + 8, 10))):    # a moment inside a shared gradient
+            assert step(*bad) == -5, bad
+    with pytest.raises(ValueError):
+        check(-5, "a step")
+    assert issubclass(SparcOverlapError, RuntimeError)

@@ -201,3 +201,38 @@ def test_graphed_steps_ask_for_every_parameter():
             tr.step(0, 1, head)
         del kept
     assert np.isfinite([float(tr.step(0, 1, head)) for _ in range(3)]).all()
+
+
+@pytest.mark.parametrize("n", [9, 5000, 300_000])
+def test_gradients_that_overlap_in_part_are_refused(n):
+    """And nothing is scaled; neighbours in one bucket, in any order, are no overlap."""
+    from sparc_amd.optim import Adam, adam_step_, clip_grad_norm_
+    from test_gpu_clip import check_clip, params_of
+    for dtype in (torch.float32, torch.bfloat16):
+        flat = torch.randn(2 * n, device="cuda", generator=gen(n)).to(dtype)
+        kept = flat.clone()
+        for bad in ([flat[:n], flat[n - 1:]], [flat[n - 1:], flat[:n]], [flat, flat[3:4]], [flat[1:2], flat[:n], flat[n:]]):
+            with pytest.raises(ValueError):
+                clip_grad_norm_(params_of(bad), 0.1)
+        assert torch.equal(flat, kept)
+        check_clip([flat[n:], flat[1:n], flat[:1]], 0.1)
+    flat = torch.randn(4 * n, device="cuda", generator=gen(n + 1))
+    g, kept = torch.ones(n, device="cuda"), flat.clone()
+    for limit in (None, 1.0):
+        for bad in ((flat[:n], g, flat[n - 1:2 * n - 1], flat[2 * n:3 * n]), (flat[:n], flat[n - 1:2 * n - 1], flat[2 * n:3 * n], flat[3 * n:]),
+                    (flat[:n], g, flat[n:2 * n], flat[2 * n - 1:3 * n - 1])):
+            with pytest.raises(ValueError):
+                adam_step_(*([t] for t in bad), 1, max_grad_norm=limit)
+        a, b = torch.nn.Parameter(flat[:n]), torch.nn.Parameter(flat[n - 1:2 * n - 1])
+        a.grad, b.grad = g, g
+        with pytest.raises(ValueError):
+            Adam([a, b], max_grad_norm=limit).step()
+        many = [[torch.zeros(3, device="cuda") for _ in range(40)] for _ in range(3)]   # (more than one launch takes)
+        many[0][39] = many[1][38][1:]
+        many[1][39], many[2][39] = torch.zeros(2, device="cuda"), torch.zeros(2, device="cuda")
+        with pytest.raises(ValueError):
+            adam_step_(many[0], [torch.ones_like(t) for t in many[0]], *many[1:], 1, max_grad_norm=limit)
+        assert not any(bool((t != 0).any()) for of in many for t in of)
+    assert torch.equal(flat, kept)
+    adam_step_([flat[:n]], [g], [flat[n:2 * n].zero_()], [flat[2 * n:3 * n].zero_()], 1)      # neighbours: fine
+    assert bool((flat[:n] != kept[:n]).all()) and torch.equal(flat[3 * n:], kept[3 * n:])
