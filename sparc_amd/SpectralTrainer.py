@@ -62,6 +62,11 @@ class SpectralNetModel(nn.Module):
                 self.layers.append(nn.Sequential(nn.Linear(current_dim, dim), nn.ReLU()))
                 current_dim = dim
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "node_table" not in self._modules:   # None, or a model pickled before there was one
+            self.node_table = None
+
     def mlp_parameters(self):
         """[W0, b0, W1, b1, ...]: the parameters whose gradients the backward reports layer by layer."""
         return [p for layer in self.layers for p in layer.parameters()]

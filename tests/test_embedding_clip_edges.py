@@ -98,3 +98,14 @@ def test_memory_written_twice_is_refused():
     with pytest.raises(ValueError):
         check(-5, "a step")
     assert issubclass(SparcOverlapError, RuntimeError)
+
+
+def test_a_model_pickled_before_there_was_a_node_table():
+    import pickle
+    from sparc_amd.SpectralTrainer import SpectralNetModel
+    arch = {"n_layers": 2, "hidden_dim1": 16, "output_dim": 4}
+    old = SpectralNetModel(arch, 12, torch.device("cpu"))
+    del old.__dict__["node_table"]
+    assert pickle.loads(pickle.dumps(old)).node_table is None
+    new = pickle.loads(pickle.dumps(SpectralNetModel(arch, 12, torch.device("cpu"), node_table={"rows": 9, "dim": 6})))
+    assert new.node_table.weight.shape == (9, 6) and "node_table.weight" in new.state_dict()
