@@ -96,16 +96,17 @@ def _limit(max_norm) -> float:
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the gradients of `parameters` (one tensor or several; those without a gradient are passed over, a gradient met
     twice, the same memory, counts once) in place by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them
-    together, and returns the norm before (float32, on the device; nothing synchronises).  float32, bfloat16 and float16
+    together, and returns the norm before (float32, on their device; nothing synchronises).  float32, bfloat16 and float16
     gradients may be mixed, each dense in memory (any order of the dimensions, views into a bucket too); gradients that overlap
     in part raise.  Sums in float64.  A norm that is not finite leaves what the formula gives; an infinite max_norm never
     clips."""
     max_norm = _limit(max_norm)
     if torch.is_tensor(parameters):
         parameters = (parameters,)
+    parameters = list(parameters)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
-        return torch.zeros(())
+        return torch.zeros((), device=parameters[0].device if parameters else None)
     refuse_forward_mode("clip_grad_norm_", *grads)
     device = grads[0].device
     if not grads[0].is_cuda:

@@ -236,3 +236,11 @@ def test_gradients_that_overlap_in_part_are_refused(n):
     assert torch.equal(flat, kept)
     adam_step_([flat[:n]], [g], [flat[n:2 * n].zero_()], [flat[2 * n:3 * n].zero_()], 1)      # neighbours: fine
     assert bool((flat[:n] != kept[:n]).all()) and torch.equal(flat[3 * n:], kept[3 * n:])
+
+
+def test_the_norm_of_no_gradient_is_on_the_device():
+    from sparc_amd.optim import clip_grad_norm_
+    p = torch.nn.Parameter(torch.zeros(3, device="cuda"))
+    norm = clip_grad_norm_((x for x in [p]), 1.0)
+    assert norm.device == p.device and norm.dtype == torch.float32 and norm.shape == () and float(norm) == 0.0
+    assert float(clip_grad_norm_([], 1.0)) == 0.0                         # (no tensor to say which device)
