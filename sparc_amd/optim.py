@@ -221,6 +221,7 @@ class Adam(torch.optim.Optimizer):
                 loss = closure()
         max_norm = self._clip_at()
         work = []
+        laid_out = {}   # copies of gradients that are not laid out as their parameters: one of each, or the norm would count them again
         for group in self.param_groups:
             live = [p for p in group["params"] if p.grad is not None]
             if not live:
@@ -235,7 +236,11 @@ class Adam(torch.optim.Optimizer):
                 if not st:
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                grads.append(p.grad if p.grad.is_contiguous() else p.grad.contiguous())
+                g = p.grad
+                if not g.is_contiguous():
+                    key = g.data_ptr(), g.shape, g.stride()
+                    g = laid_out[key] if key in laid_out else laid_out.setdefault(key, g.contiguous())
+                grads.append(g)
                 ms.append(st["exp_avg"])
                 vs.append(st["exp_avg_sq"])
             dev = live[0].device

@@ -244,3 +244,20 @@ def test_the_norm_of_no_gradient_is_on_the_device():
     norm = clip_grad_norm_((x for x in [p]), 1.0)
     assert norm.device == p.device and norm.dtype == torch.float32 and norm.shape == () and float(norm) == 0.0
     assert float(clip_grad_norm_([], 1.0)) == 0.0                         # (no tensor to say which device)
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+def test_a_shared_transposed_gradient_counts_once(groups):
+    """As clip_grad_norm_ counts it, though Adam copies it into the parameters' layout."""
+    from sparc_amd.optim import Adam, clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(6, 4, device="cuda")) for _ in range(3)]
+    g = torch.randn(4, 6, device="cuda", generator=gen(1)).t()
+    ps[0].grad, ps[1].grad, ps[2].grad = g, g, torch.randn(6, 4, device="cuda", generator=gen(2))
+    opt = Adam([{"params": ps}] if groups == 1 else [{"params": ps[:1]}, {"params": ps[1:]}], max_grad_norm=0.5)
+    opt.step()
+    moments = [opt.state[p]["exp_avg"] for p in ps]
+    assert torch.equal(moments[0], moments[1])
+    kept = [p.grad.clone() for p in ps]
+    assert torch.equal(opt.grad_norm, clip_grad_norm_(ps, 0.5))
+    for m, p, k in zip(moments, ps, kept):    # 0.1 of the clipped gradient: factor, product, difference and sum in float32
+        assert bool(((m.double() - 0.1 * p.grad.double()).abs() <= 8 * 2.0 ** -24 * k.double().abs()).all())
