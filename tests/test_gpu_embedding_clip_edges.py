@@ -261,3 +261,22 @@ def test_a_shared_transposed_gradient_counts_once(groups):
     assert torch.equal(opt.grad_norm, clip_grad_norm_(ps, 0.5))
     for m, p, k in zip(moments, ps, kept):    # 0.1 of the clipped gradient: factor, product, difference and sum in float32
         assert bool(((m.double() - 0.1 * p.grad.double()).abs() <= 8 * 2.0 ** -24 * k.double().abs()).all())
+
+
+@pytest.mark.parametrize("pattern", ["uniform", "one", "zipf"])
+@pytest.mark.parametrize("n,rows,dim,dtype", [
+    (8192, 3000, 512, torch.float32), (8192, 3000, 513, torch.float32), (8192, 3000, 1024, torch.float16), (8192, 3000, 1025, torch.float16),
+    (8192, 900, 1024, torch.bfloat16), (8191, 900, 1025, torch.bfloat16), (512, 70, 8192, torch.float32), (513, 70, 8192, torch.float32),
+    (512, 70, 16384, torch.bfloat16), (513, 70, 16384, torch.bfloat16), (4096, 3000, 1024, torch.float32), (4097, 3000, 1024, torch.float32)])
+def test_gradient_on_both_sides_of_the_one_launch_rule(pattern, n, rows, dim, dtype):
+    """One launch takes up to 8192 tokens and 16 MiB of gradient, in rows of up to 32 KiB."""
+    from sparc_amd._lib import lib
+    from sparc_amd.embedding import DTYPES, embedding_grad
+    size = 4 if dtype == torch.float32 else 2
+    sorts = lib.sparc_embedding_grad_workspace_bytes(n, rows, dim, DTYPES[dtype]) > 0
+    assert sorts == (n * dim * size > 16 << 20)
+    ids = make_ids(pattern, n, rows, n + dim)
+    g = torch.randn(n, dim, device="cuda", generator=gen(n + rows)).to(dtype)
+    got = embedding_grad(ids, g, rows, scale=-1.5)
+    check_grad(got, ids, g, rows, -1.5)
+    assert torch.equal(got, embedding_grad(ids.int(), g, rows, scale=-1.5))

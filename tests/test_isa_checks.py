@@ -163,3 +163,29 @@ def test_wide_dgrad_gemm_loop_waits_only_for_the_chunk_it_reads(tmp_path):
         assert sum("v_mfma_f32_32x32x2" in l for l in ins) == 64
     for m in re.finditer(r"\.amdhsa_kernel (\S*linear_narrow_fwd_kernel\S*)(.*?)\.end_amdhsa_kernel", text, re.S):
         assert int(re.search(r"\.amdhsa_private_segment_fixed_size\s+(\d+)", m.group(2)).group(1)) == 0, m.group(1)
+
+
+def test_table_and_clipping_kernels_fit_their_registers(tmp_path):
+    """embedding.hip and clip.hip: nothing spills or lives in scratch memory, few_tokens leaves room for three of its
+    workgroups on a CU (six waves per SIMD: 80 registers), the norm's pass for two of 1024 threads (64), and there is no packed
+    float32 instruction."""
+    from sparc_amd import build
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    flags = [f for f in build.FLAGS if f != "-fPIC"]
+    most = {"few_tokens": (80, 6), "grad_squares_kernel": (64, 2), "row_sums": (128, 12), "digit_scatter": (128, 1), "grad_scale_kernel": (128, 4),
+            "clip_once_kernel": (128, 2), "adam_once_kernel": (128, 2), "adam_clip_kernel": (128, 4)}
+    found = dict.fromkeys(most, 0)
+    for name in ("embedding", "clip"):
+        out = tmp_path / f"{name}.s"
+        subprocess.run([hipcc] + flags + ["-S", "--cuda-device-only", "-o", str(out), os.path.join(ROOT, "sparc_amd", "csrc", f"{name}.hip")],
+                       check=True, cwd=str(tmp_path))
+        text = out.read_text()
+        assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", text)
+        assert set(re.findall(r"\.vgpr_spill_count:\s+(\d+)", text)) == {"0"}
+        for m in re.finditer(r"\.amdhsa_kernel (\S+)(.*?)\.end_amdhsa_kernel", text, re.S):
+            assert int(re.search(r"\.amdhsa_private_segment_fixed_size\s+(\d+)", m.group(2)).group(1)) == 0, m.group(1)
+            for kernel, (registers, _) in most.items():
+                if kernel in m.group(1):
+                    found[kernel] += 1
+                    assert int(re.search(r"\.amdhsa_next_free_vgpr\s+(\d+)", m.group(2)).group(1)) <= registers, m.group(1)
+    assert found == {kernel: n for kernel, (_, n) in most.items()}
