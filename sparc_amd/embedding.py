@@ -18,7 +18,7 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SPARC_F32, 
 _ID_DTYPES = {torch.int32: 0, torch.int64: 1}
 
 
-def refuse_forward_mode(what: str, *tensors) -> None:
+def refuse_forward_mode(what: str, tensors) -> None:
     """Raises inside a dual level where a tensor carries a tangent: the kernels know nothing of it and it would be lost."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
@@ -74,7 +74,7 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: floa
     are recorded) or carries a forward-mode tangent raises."""
     if grad.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("embedding_grad is not differentiable: detach grad, or call it under torch.no_grad()")
-    refuse_forward_mode("embedding_grad", grad)
+    refuse_forward_mode("embedding_grad", (grad,))
     dev = grad.device
     if not grad.is_cuda:
         require_gpu(dev)
@@ -142,7 +142,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     tangent raises."""
     if padding_idx is not None:
         _padding(padding_idx, table.shape[0])
-    refuse_forward_mode("embedding_lookup", table)
+    refuse_forward_mode("embedding_lookup", (table,))
     if table.requires_grad and torch.is_grad_enabled():
         return EmbeddingLookup.apply(ids, table, float(scale), padding_idx)
     return _lookup(ids, table, float(scale))

@@ -107,7 +107,7 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros((), device=parameters[0].device if parameters else None)
-    refuse_forward_mode("clip_grad_norm_", *grads)
+    refuse_forward_mode("clip_grad_norm_", grads)
     device = grads[0].device
     if not grads[0].is_cuda:
         require_gpu(device)
@@ -125,17 +125,14 @@ def _adam_records(params, grads, exp_avgs, exp_avg_sqs, device):
     """(records of the update as the C calls take them; None, or, where parameters share gradients, these once)."""
     n = len(params)
     every = [*params, *grads, *exp_avgs, *exp_avg_sqs]
-    refuse_forward_mode("an Adam step", *every)
+    refuse_forward_mode("an Adam step", every)
     sizes = list(map(_size_of, every))
     if set(map(_type_of, every)) != {torch.float32} or not _dense_on(every, device) or sizes != sizes[:n] * 4:
         raise ValueError("an Adam step takes contiguous float32 tensors of one device, four of a size")
     at = list(map(_address_of, every))
     once = None
-    if len(set(at)) < 4 * n:   # empty tensors, or a gradient that several parameters share: nothing else may occur twice
-        full = [a for a, size in zip(at, sizes) if size]
+    if len(set(at[n:2 * n])) < n:   # (memory that is written and shared: the library refuses it)
         once = _each_once(at[n:2 * n], sizes[:n], [0] * n)
-        if len(set(full)) < len(full) // 4 * 3 + len(once[0]):
-            raise ValueError("an Adam step writes every parameter and moment once")
     return _records(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], sizes[:n]), once
 
 
@@ -250,6 +247,11 @@ class Adam(torch.optim.Optimizer):
             work.append((group, live, grads, ms, vs, dev, records, once, rates))
         if not work:
             return loss
+        if len(work) > 1:   # nothing moves where a later group would be refused
+            every = array("q")
+            for w in work:
+                every.extend(w[6])
+            check(lib.sparc_adam_check(sum(len(w[1]) for w in work), _address(every)), "sparc_adam_check")
         if max_norm is not None and len(work) > 1:   # the norm over all groups
             device = work[0][5]
             require_gpu(device)

@@ -280,3 +280,23 @@ def test_gradient_on_both_sides_of_the_one_launch_rule(pattern, n, rows, dim, dt
     got = embedding_grad(ids, g, rows, scale=-1.5)
     check_grad(got, ids, g, rows, -1.5)
     assert torch.equal(got, embedding_grad(ids.int(), g, rows, scale=-1.5))
+
+
+@pytest.mark.parametrize("limit", [None, 1.0])
+def test_memory_that_groups_share_is_refused_before_any_moves(limit):
+    from sparc_amd.optim import Adam
+    flat = torch.randn(3000, device="cuda", generator=gen(8))
+    kept = flat.clone()
+    for second in (flat[999:2000], flat[:1000]):
+        ps = [torch.nn.Parameter(flat[:1000]), torch.nn.Parameter(second)]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt = Adam([{"params": [p]} for p in ps], max_grad_norm=limit)
+        with pytest.raises(ValueError):
+            opt.step()
+        assert torch.equal(flat, kept) and [group.get("step", 0) for group in opt.param_groups] == [0, 0]
+    ps = [torch.nn.Parameter(flat[:1000]), torch.nn.Parameter(flat[1000:2000])]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    Adam([{"params": [p]} for p in ps], max_grad_norm=limit).step()
+    assert bool((flat[:2000] != kept[:2000]).all()) and torch.equal(flat[2000:], kept[2000:])
