@@ -159,7 +159,7 @@ __device__ __forceinline__ void preact_steps(v2f_t (&a)[2], const float xr, cons
     if constexpr (K0 < KMAX) {
         if (K0 < K) {   // uniform
             const float xk = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(xr), 0x150 + K0, 0xf, 0xf, false));
-            a[0] = __builtin_elementwise_fma(v2f_t{xk, xk}, w[0][K0], a[0]);   // packed: two columns per instruction
+            a[0] = __builtin_elementwise_fma(v2f_t{xk, xk}, w[0][K0], a[0]);   // (a pair of columns: two instructions, packed ones being switched off)
             a[1] = __builtin_elementwise_fma(v2f_t{xk, xk}, w[1][K0], a[1]);
             preact_steps<K0 + 1, KMAX>(a, xr, w, K);
         }
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(256) void linear_narrow_in_fwd_kernel(int64_t m, in
     const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
     const bool live = c < N;
     typedef float v2f __attribute__((ext_vector_type(2)));
-    v2f w[2][KMAX], bias[2];    // column pairs (c, c + 1) and (c + 2, c + 3): packed fp32 multiply-adds
+    v2f w[2][KMAX], bias[2];    // column pairs (c, c + 1) and (c + 2, c + 3)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         bias[t] = live ? v2f{b[c + 2 * t], b[c + 2 * t + 1]} : v2f{0.f, 0.f};
