@@ -492,8 +492,8 @@ int sparc_clip_adam_step(int64_t n_tensors, const sparc_adam_tensor_t* tensors, 
  * (src/SpectralTrainer.py:28-39) and has no table.  table [rows][dim] with row stride ld (elements), out and g rows with
  * strides ldo and ldg; dtype of table, out and g: SPARC_F32, SPARC_BF16 or SPARC_F16; ids: n tokens, int32, or int64 with
  * ids_64 != 0; any element alignment.
- *   sparc_embedding_fwd   out[i] = round(scale * table[ids[i]]), product in float32; a token outside [0, rows) reads
- *                         nothing and gives a row of NaN.
+ *   sparc_embedding_fwd   out[i] = round(scale * table[ids[i]]), the product in float32 or (halves in narrow rows) unrounded; a
+ *                         token outside [0, rows) reads nothing and gives a row of NaN.
  *   sparc_embedding_grad  out[v] = round(scale * sum over ids[i] = v of g[i]) for ALL rows v (dense [rows][dim]; rows
  *                         without a token, and row padding_idx when it is a row, are 0); tokens outside the table are left
  *                         out.  Sums in float32, of long rows joined in float64, in an order fixed by the tokens alone.
